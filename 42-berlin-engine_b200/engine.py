@@ -15,6 +15,7 @@ LIB_PATH = os.path.join(HERE, "libengine_cuda.so")
 EC_OK, EC_ERR_ARG, EC_ERR_CUDA, EC_ERR_OOM, EC_ERR_STATE = 0, -1, -2, -3, -4
 EC_ERR_UNSUPPORTED, EC_ERR_TIMEOUT = -5, -6
 EC_W_INT8, EC_W_FP8, EC_W_BF16 = 0, 1, 2
+EC_T_F32, EC_T_BF16, EC_T_F16 = 0, 1, 2
 EC_ATTN_REFERENCE, EC_ATTN_SPLIT = 0, 1
 EC_WQ, EC_WK, EC_WV, EC_WO, EC_W1, EC_W2, EC_W3, EC_ATTN_NORM, EC_FFN_NORM = range(9)
 EC_EMBEDDING, EC_FINAL_NORM, EC_LM_HEAD = 16, 17, 18
@@ -37,6 +38,7 @@ EXPORTS = [
     "ec_gemm_tc_bytes", "ec_gemm_tc_pack", "ec_op_gemm_tc", "ec_prefill", "ec_set_weight_bf16",
     "ec_tp_unique_id", "ec_create_tp", "ec_verify", "ec_lsh_attn_build_paged",
     "ec_op_sample_top_p", "ec_op_sample_temperature", "ec_set_context_bias",
+    "ec_op_add_rmsnorm_quant", "ec_op_silu_mul_quant", "ec_op_gemm_w8a8", "ec_op_token_logprobs",
 ]
 K_NAMES = ["gemv_qkv", "gemv_o", "gemv_gateup", "gemv_down", "gemv_lm", "kv_append", "select",
            "attention", "embed", "argmax", "gemv_chain", "tc_gemm", "tc_quant", "tc_combine"]
@@ -78,7 +80,7 @@ def lib():
         if not os.path.exists(LIB_PATH):
             raise RuntimeError(f"{LIB_PATH} missing: run __graft_entry__.build()")
         L = C.CDLL(LIB_PATH)
-        vp, i, f = C.c_void_p, C.c_int, C.c_float
+        vp, i, f, ll = C.c_void_p, C.c_int, C.c_float, C.c_int64
         sig = {
             "ec_last_error": (C.c_char_p, []),
             "ec_config_default": (i, [C.POINTER(ModelConfig)]),
@@ -117,6 +119,10 @@ def lib():
             "ec_op_sample_top_p": (i, [vp, i, i, vp, vp, i, f, f, f, i, vp, vp, vp]),
             "ec_op_sample_temperature": (i, [vp, i, i, f, vp, vp, vp]),
             "ec_set_context_bias": (i, [vp, vp, vp, vp, i]),
+            "ec_op_add_rmsnorm_quant": (i, [i, vp, ll, vp, ll, vp, ll, vp, f, i, i, vp, ll, vp, vp]),
+            "ec_op_silu_mul_quant": (i, [i, vp, vp, ll, i, i, vp, ll, vp, vp]),
+            "ec_op_gemm_w8a8": (i, [vp, ll, vp, vp, ll, vp, i, vp, ll, i, i, i, vp, vp]),
+            "ec_op_token_logprobs": (i, [i, vp, ll, i, i, vp, f, i, vp, vp, vp, vp, vp]),
             "ec_op_paged_append": (i, [C.POINTER(PagedView), vp, vp, i, vp]),
             "ec_op_paged_attention": (i, [C.POINTER(PagedView), vp, vp, i, i, i, vp, vp, vp]),
             "ec_op_paged_attention_static": (i, [C.POINTER(PagedView), vp, vp, i, i, i, vp, vp,
@@ -338,6 +344,17 @@ class Engine:
             C.c_void_p(history_len_ptr) if history_len_ptr else None, int(history_stride),
             float(temperature), float(top_p), float(penalty), int(block_token0),
             C.c_void_p(r_ptr), C.c_void_p(out_ptr), self.stream()))
+
+    def logprobs_device(self, B, tokens_ptr=None, logprob_ptr=None, entropy_ptr=None, top_k=0,
+                        top_ids_ptr=None, top_logprobs_ptr=None, temperature=1.0):
+        """Log probabilities of one token per row, entropy and the top
+        alternatives (ec_op_token_logprobs) of the last step's device logits,
+        on the context's stream.  Call it before sample_device, which
+        modifies the logits."""
+        check(lib().ec_op_token_logprobs(
+            EC_T_F32, lib().ec_logits_device(self.h), self.c.vocab_size, self.c.vocab_size, B,
+            tokens_ptr, float(temperature), int(top_k), logprob_ptr, entropy_ptr, top_ids_ptr,
+            top_logprobs_ptr, self.stream()))
 
     def step_device(self, tokens_ptr, pos_ptr, B, feedback=True):
         check(lib().ec_decode_step_device(self.h, C.c_void_p(tokens_ptr), C.c_void_p(pos_ptr),

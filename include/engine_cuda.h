@@ -40,6 +40,12 @@ extern "C" {
 # define EC_W_FP8 1    /* E4M3 [rows][cols] + one fp32 scale per matrix */
 # define EC_W_BF16 2   /* bf16 [rows][cols], no scale (per-op GEMV only) */
 
+/* element types of activation rows (the 8-bit row operators, token log
+** probabilities) */
+# define EC_T_F32 0
+# define EC_T_BF16 1
+# define EC_T_F16 2
+
 /* matrix ids for ec_set_weight (layer >= 0) */
 # define EC_WQ 0
 # define EC_WK 1
@@ -368,6 +374,81 @@ int		ec_op_sample_top_p(float *logits, int n, int rows, const int *history,
 ** returns n). */
 int		ec_op_sample_temperature(const float *logits, int n, int rows,
 			float temperature, const float *r, int *out, void *stream);
+
+/* ------------------------------------------------------------------------ */
+/* 8-bit activation rows: the projections of a prompt or a batch with INT8   */
+/* activations (one scale per token) against INT8 weights (one scale per     */
+/* channel).  The reference keeps f32 activations throughout; these have no  */
+/* counterpart in it.  One layer's feed-forward is                           */
+/*   ec_op_add_rmsnorm_quant -> ec_op_gemm_w8a8 (gate and up stacked) ->     */
+/*   ec_op_silu_mul_quant -> ec_op_gemm_w8a8 -> the next                     */
+/*   ec_op_add_rmsnorm_quant, which adds the product to the residual.        */
+/* All device pointers, on the current device; asynchronous on `stream`; no  */
+/* allocation, no workspace, nothing kept between calls: calls on different  */
+/* streams and captured graphs share nothing.  Row strides (ld*) count       */
+/* elements and may exceed the row; elements behind a row's end are neither  */
+/* read nor written.  Results do not depend on scheduling: equal inputs give */
+/* equal bits.                                                               */
+/*                                                                           */
+/* The 8-bit rule of a row y (ec_set_weight_bf16's rounding):                */
+/*   scale = amax / 127, q = y * (127 / amax) to the nearest integer, ties   */
+/*   to even, amax = max |y|.  amax below 2^-100: the row counts as zero     */
+/*   (q = 0, scale = 1).  A row with a NaN or an infinity: q = 0, scale NaN, */
+/*   so that whatever is computed from it is NaN.                            */
+/* ------------------------------------------------------------------------ */
+
+/* h = x + residual (rounded to `type`), sum_out = h,
+** y = h / sqrt(mean(h^2) + eps) * w, and y's rows in 8 bits.  residual and
+** sum_out may be NULL (no addition / the sum is not kept); w (bf16 [n], as
+** every norm weight here) may be NULL (all ones).  sum_out may be x or
+** residual itself (same pointer and stride); other overlaps are not
+** allowed.  `type` (EC_T_*) is that of x, residual and sum_out.  A row whose
+** sum of squares passes the range of f32 counts as one with an infinity.
+** n <= 57344 (else EC_ERR_UNSUPPORTED). */
+int		ec_op_add_rmsnorm_quant(int type, const void *x, int64_t ldx,
+			const void *residual, int64_t ldr, void *sum_out, int64_t lds,
+			const uint16_t *w, float eps, int rows, int n, int8_t *q,
+			int64_t ldq, float *scales, void *stream);
+
+/* y = gate / (1 + exp(-gate)) * up, and y's rows in 8 bits.  gate and up
+** share the stride ld: with both in one buffer [rows][2n], up = gate + n and
+** ld = 2n.  The exponential is exact to f32 rounding, unlike op_silu_mul's
+** approximation.  n <= 57344 (else EC_ERR_UNSUPPORTED). */
+int		ec_op_silu_mul_quant(int type, const void *gate, const void *up,
+			int64_t ld, int rows, int n, int8_t *q, int64_t ldq, float *scales,
+			void *stream);
+
+/* y[t][c] = (x_scale[t] * sum_k x[t][k] w[c][k]) * w_scale[c] for t < nb,
+** c < m, rounded to `type` (EC_T_*): INT8 x [nb][k] and row-major INT8
+** weights w [m][k] (the form ec_set_weight takes).  The sum is exact in
+** int32 (k <= 131071, else EC_ERR_UNSUPPORTED); y differs from the exact
+** value by the conversion to f32, two products and the rounding to `type`.
+** x and w must be 16-byte aligned with strides that are multiples of 16
+** (else EC_ERR_ARG); m, k and nb are free.  status (device int, may be
+** NULL): a bounded device wait that gives up stores EC_ERR_TIMEOUT there
+** (and NaN in its part of y); it is not written otherwise. */
+int		ec_op_gemm_w8a8(const int8_t *x, int64_t ldx, const float *x_scale,
+			const int8_t *w, int64_t ldw, const float *w_scale, int type,
+			void *y, int64_t ldy, int m, int k, int nb, int *status,
+			void *stream);
+
+/* Log probabilities under softmax(logits / temperature), `rows` rows of n
+** logits (type EC_T_*, ld elements apart, not modified; temperature 2^-100
+** to 2^100):
+**   logprob[row] of token tokens[row] (both NULL: none).  A token of -1
+**     marks a row without one (a prompt's last, padding): 0 is stored; any
+**     other token outside 0..n-1 gives NaN.
+**   entropy[row] (NULL: not computed), in nats.
+**   top_ids, top_logprobs [rows][top_k]: the top_k (0..32, at most n) largest
+**     logits, equal ones by index, and their log probabilities.
+** A logit of -inf has probability 0 and adds nothing to the entropy; a row
+** of nothing else has log probabilities -inf and entropy 0.  A NaN or +inf
+** makes the row's log probabilities and entropy NaN; NaN orders below -inf
+** among the top_k.  No allocation. */
+int		ec_op_token_logprobs(int type, const void *logits, int64_t ld, int n,
+			int rows, const int *tokens, float temperature, int top_k,
+			float *logprob, float *entropy, int *top_ids, float *top_logprobs,
+			void *stream);
 
 /* One layer's paged INT8 KV cache in device memory
 ** (t_kv_block / t_block_manager, src/memory/paged.h:53-88).  Blocks hold 16

@@ -1,0 +1,272 @@
+"""ec_op_add_rmsnorm_quant and ec_op_silu_mul_quant (through the C ABI)
+against the formulas in 64 bits.
+
+Tolerances, from the arithmetic: u = 2^-24 is one f32 rounding.
+  RMSNorm: each thread adds at most n / 64 squares one after the other, then
+    at most 16 partial sums meet, so the sum of squares (all terms positive)
+    is off by at most (n / 64 + 16) u; the root halves that; division, root,
+    the two products and the mean add 6 u.
+  SwiGLU: exp within 4 u of itself and of its argument's rounding, which
+    counts |g| u; 1 + exp, quotient (4 u), product: 12 u + |g| u.
+A value is then rounded to 8 bits: q is within 0.5 of y * 127 / amax, and of
+what 127 times the error above, of y and of amax, can move it.
+"""
+import numpy as np
+import pytest
+
+from conftest import load_pkg_module
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+TYPES = ["f32", "bf16", "f16"]
+
+
+@pytest.fixture(scope="module")
+def eng():
+    return load_pkg_module("engine")
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    return torch
+
+
+def dtype(torch, kind):
+    return {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[kind]
+
+
+CODE = {"f32": 0, "bf16": 1, "f16": 2}
+
+
+def padded(torch, t, ld, offset=0, fill=float("nan")):
+    """t's rows ld elements apart, `offset` elements into a buffer of `fill`."""
+    rows, n = t.shape
+    buf = torch.full((offset + rows * ld,), fill, dtype=t.dtype, device="cuda")
+    view = buf[offset:].view(rows, ld)[:, :n]
+    view.copy_(t)
+    return buf, view
+
+
+def check_rows(y, rel, q, scale):
+    """q, scale (device results) against y (64 bits), of which every value may
+    be off by `rel` (scalar or per value) of itself."""
+    amax = np.abs(y).max(1, keepdims=True)
+    rel = np.broadcast_to(np.asarray(rel), y.shape)
+    top = rel.max(1, keepdims=True)
+    assert np.all(np.abs(scale[:, None] - amax / 127) <= (top + 2 * U) * amax / 127)
+    t = y * 127 / amax
+    off = np.abs(q - t)
+    assert np.all(off <= 0.5 + np.abs(t) * (rel + top + 3 * U)), off.max()
+    assert np.all(np.abs(q).max(1) == 127)
+
+
+def run_norm(eng, torch, kind, x, r, w, eps, ldx=None, ldr=None, lds=None, ldq=None, offset=0,
+             keep=True, alias=None, stream=None):
+    rows, n = x.shape
+    _, xv = padded(torch, x, ldx or n, offset)
+    rv = padded(torch, r, ldr or n, offset)[1] if r is not None else None
+    hb = hv = None
+    if alias == "x":
+        hv, lds = xv, ldx or n
+    elif alias == "r":
+        hv, lds = rv, ldr or n
+    elif keep:
+        hb, hv = padded(torch, torch.zeros_like(x), lds or n, offset, 7.0)
+    qb, qv = padded(torch, torch.zeros(rows, n, dtype=torch.int8, device="cuda"), ldq or n, offset, 99)
+    sc = torch.full((rows + 1,), -5.0, device="cuda")
+    eng.check(eng.lib().ec_op_add_rmsnorm_quant(
+        CODE[kind], xv.data_ptr(), ldx or n, rv.data_ptr() if r is not None else None, ldr or n,
+        hv.data_ptr() if hv is not None else None, lds or n,
+        w.data_ptr() if w is not None else None, eps, rows, n, qv.data_ptr(), ldq or n,
+        sc.data_ptr(), stream))
+    torch.cuda.synchronize()
+    # nothing behind a row's end is written
+    if ldq and ldq > n:
+        assert (qb[offset:].view(rows, ldq)[:, n:] == 99).all() and (qb[:offset] == 99).all()
+    if hb is not None and lds and lds > n:
+        assert (hb[offset:].view(rows, lds)[:, n:] == 7.0).all()
+    assert sc[rows] == -5.0
+    return (hv.clone() if hv is not None else None), qv.clone(), sc[:rows]
+
+
+def norm64(h, w, eps):
+    h = h.double().cpu().numpy()
+    y = h / np.sqrt((h * h).mean(1, keepdims=True) + eps)
+    return y * w.double().cpu().numpy() if w is not None else y
+
+
+def norm_rel(n):
+    return ((n / 64 + 16) / 2 + 6) * U
+
+
+def inputs(torch, kind, rows, n, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    dt = dtype(torch, kind)
+    x = torch.randn(rows, n, generator=g, device="cuda").to(dt)
+    r = (torch.randn(rows, n, generator=g, device="cuda") * 3).to(dt)
+    w = (1 + 0.3 * torch.randn(n, generator=g, device="cuda")).to(torch.bfloat16)
+    return x, r, w
+
+
+SHAPES = [(1, 1), (3, 2), (1, 7), (5, 31), (2, 64), (7, 257), (4, 1000), (3, 1024), (2, 2047),
+          (2, 4096), (9, 4100), (3, 5003), (2, 8192), (2, 14336), (1, 16385), (2, 28672),
+          (1, 57343), (1, 57344), (301, 512)]
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows,n", SHAPES)
+def test_norm(eng, torch, kind, rows, n):
+    x, r, w = inputs(torch, kind, rows, n, n)
+    h, q, sc = run_norm(eng, torch, kind, x, r, w, 1e-5)
+    want = (x.float() + r.float()).to(x.dtype)
+    assert torch.equal(h, want)  # one rounding of an exact sum
+    check_rows(norm64(want, w, 1e-5), norm_rel(n), q.cpu().numpy().astype(np.float64),
+               sc.double().cpu().numpy())
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("offset,pad", [(0, 16), (1, 3), (3, 0), (0, 1), (8, 8)])
+def test_norm_strides_and_alignment(eng, torch, kind, offset, pad):
+    rows, n = 6, 1003 if pad else 1008
+    x, r, w = inputs(torch, kind, rows, n, 5)
+    h, q, sc = run_norm(eng, torch, kind, x, r, w, 1e-6, n + pad, n + 2 * pad, n + pad, n + pad,
+                        offset)
+    h0, q0, sc0 = run_norm(eng, torch, kind, x, r, w, 1e-6)
+    assert torch.equal(h, h0)
+    check_rows(norm64(h, w, 1e-6), norm_rel(n), q.cpu().numpy().astype(np.float64),
+               sc.double().cpu().numpy())
+    check_rows(norm64(h, w, 1e-6), norm_rel(n), q0.cpu().numpy().astype(np.float64),
+               sc0.double().cpu().numpy())
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n", [1003, 4096])
+def test_norm_optional_operands_and_aliases(eng, torch, kind, n):
+    x, r, w = inputs(torch, kind, 4, n, 6)
+    full = run_norm(eng, torch, kind, x, r, w, 1e-5)
+    for alias in ("x", "r"):  # the sum in the place of an input
+        got = run_norm(eng, torch, kind, x, r, w, 1e-5, alias=alias)
+        assert all(torch.equal(a, b) for a, b in zip(full, got)), alias
+    _, q, sc = run_norm(eng, torch, kind, x, r, w, 1e-5, keep=False)  # the sum not kept
+    assert torch.equal(q, full[1]) and torch.equal(sc, full[2])
+    h, q, sc = run_norm(eng, torch, kind, x, None, w, 1e-5)  # no residual: the sum is x
+    assert torch.equal(h, x)
+    check_rows(norm64(x, w, 1e-5), norm_rel(n), q.cpu().numpy().astype(np.float64),
+               sc.double().cpu().numpy())
+    _, q, sc = run_norm(eng, torch, kind, x, r, None, 1e-5, keep=False)  # no weight
+    check_rows(norm64(full[0], None, 1e-5), norm_rel(n), q.cpu().numpy().astype(np.float64),
+               sc.double().cpu().numpy())
+
+
+@pytest.mark.parametrize("n", [5, 1003, 4096, 28672])
+def test_norm_rows_without_a_finite_scale(eng, torch, n):
+    x, r, w = inputs(torch, "f32", 6, n, 7)
+    x, r = x.clone(), torch.zeros_like(r)
+    x[0] = 0
+    x[1, n // 2] = float("nan")
+    x[2, n - 1] = float("inf")
+    x[3, 0] = -float("inf")
+    x[4] *= 1e25  # the sum of squares passes f32
+    _, q, sc = run_norm(eng, torch, "f32", x, r, w, 1e-5)
+    assert sc[0] == 1 and (q[0] == 0).all()
+    for k in (1, 2, 3, 4):
+        assert sc[k].isnan() and (q[k] == 0).all(), k
+    assert sc[5].isfinite() and q[5].abs().max() == 127  # the neighbours are not touched
+
+
+def test_norm_tiny_rows_count_as_zero(eng, torch):
+    w = torch.ones(64, dtype=torch.bfloat16, device="cuda")
+    x = torch.zeros(2, 64, device="cuda")
+    x[0, 3], x[1, 3] = 1e-33, 1e-20  # with eps 1: y = x * 1, below and above 2^-100
+    _, q, sc = run_norm(eng, torch, "f32", x, None, w, 1.0)
+    assert sc[0] == 1 and (q[0] == 0).all()
+    assert q[1, 3] == 127 and abs(float(sc[1]) * 127 / 1e-20 - 1) < 1e-6
+
+
+def run_silu(eng, torch, kind, g, u, ldq=None, apart=False, offset=0, pad=0, stream=None):
+    rows, n = g.shape
+    if apart:  # two buffers of one stride
+        ld = n + pad
+        gb, gv = padded(torch, g, ld, offset)
+        ub, uv = padded(torch, u, ld, offset)
+    else:      # halves of one buffer
+        ld = 2 * n + pad
+        buf, both = padded(torch, torch.cat([g, u], 1), ld, offset)
+        gv, uv = both[:, :n], both[:, n:]
+    qb, qv = padded(torch, torch.zeros(rows, n, dtype=torch.int8, device="cuda"), ldq or n, offset, 99)
+    sc = torch.full((rows + 1,), -5.0, device="cuda")
+    eng.check(eng.lib().ec_op_silu_mul_quant(CODE[kind], gv.data_ptr(), uv.data_ptr(), ld, rows, n,
+                                             qv.data_ptr(), ldq or n, sc.data_ptr(), stream))
+    torch.cuda.synchronize()
+    if ldq and ldq > n:
+        assert (qb[offset:].view(rows, ldq)[:, n:] == 99).all()
+    assert sc[rows] == -5.0
+    return qv.clone(), sc[:rows]
+
+
+def silu64(g, u):
+    g, u = g.double().cpu().numpy(), u.double().cpu().numpy()
+    with np.errstate(over="ignore"):
+        return g / (1 + np.exp(-g)) * u
+
+
+def silu_rel(g):
+    return (12 + np.abs(g.double().cpu().numpy())) * U
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows,n", SHAPES)
+def test_silu(eng, torch, kind, rows, n):
+    g, u, _ = inputs(torch, kind, rows, n, n + 1)
+    g = (g.float() * 4).to(g.dtype)
+    q, sc = run_silu(eng, torch, kind, g, u)
+    check_rows(silu64(g, u), silu_rel(g), q.cpu().numpy().astype(np.float64),
+               sc.double().cpu().numpy())
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("apart,offset,pad", [(True, 0, 0), (True, 1, 5), (False, 0, 16),
+                                              (False, 3, 1), (True, 8, 8)])
+def test_silu_strides_and_alignment(eng, torch, kind, apart, offset, pad):
+    for n in (1003, 1024):
+        g, u, _ = inputs(torch, kind, 5, n, 9)
+        q, sc = run_silu(eng, torch, kind, g, u, n + pad, apart, offset, pad)
+        check_rows(silu64(g, u), silu_rel(g), q.cpu().numpy().astype(np.float64),
+                   sc.double().cpu().numpy())
+
+
+def test_silu_far_gates(eng, torch):
+    """Gates from -2000 to 2000: exp overflows on one side, vanishes on the
+    other; the product is 0 or gate * up."""
+    g = torch.linspace(-2000, 2000, 4001, device="cuda")[None].contiguous()
+    u = torch.ones_like(g)
+    q, sc = run_silu(eng, torch, "f32", g, u)
+    check_rows(silu64(g, u), 12 * U + np.abs(g.cpu().numpy()) * U * (g.cpu().numpy() < 0),
+               q.cpu().numpy().astype(np.float64), sc.double().cpu().numpy())
+
+
+def test_silu_rows_without_a_finite_scale(eng, torch):
+    for n in (5, 4096):
+        g, u, _ = inputs(torch, "f32", 5, n, 8)
+        g, u = g.clone(), u.clone()
+        g[0] = 0
+        u[1, n - 1] = float("nan")
+        g[2, 0] = float("inf")
+        g[3, 1], u[3, 1] = -200.0, float("inf")  # 0 * inf
+        q, sc = run_silu(eng, torch, "f32", g, u)
+        assert sc[0] == 1 and (q[0] == 0).all()
+        for k in (1, 2, 3):
+            assert sc[k].isnan() and (q[k] == 0).all(), k
+        assert sc[4].isfinite() and q[4].abs().max() == 127
+
+
+def test_equal_calls_give_equal_bits(eng, torch):
+    x, r, w = inputs(torch, "bf16", 600, 4096, 3)
+    one = run_norm(eng, torch, "bf16", x, r, w, 1e-5)
+    two = run_norm(eng, torch, "bf16", x, r, w, 1e-5)
+    assert all(torch.equal(a, b) for a, b in zip(one, two))
+    alone = run_norm(eng, torch, "bf16", x[77:78].contiguous(), r[77:78].contiguous(), w, 1e-5)
+    assert torch.equal(alone[1][0], one[1][77]) and alone[2][0] == one[2][77]  # whatever the batch

@@ -1,0 +1,231 @@
+"""ec_op_token_logprobs (through the C ABI) against the formulas in 64 bits.
+
+Tolerance: u = 2^-24 is one f32 rounding.  (z - m) is rounded twice: 2 u of
+itself.  The sum S has terms off by (|d| + 8) u each, weighted by e^d <= 1,
+where |d| e^d < 1: at most 10 u in the mean; at most n / 64 are added in a
+row, then 32 meet: (n / 64 + 32) u.  log S is off by that, absolutely, and by
+2 u of itself.  The entropy is log S less a mean of (z - m) with the same
+relative error.
+"""
+import numpy as np
+import pytest
+
+from conftest import load_pkg_module
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+TYPES = ["f32", "bf16", "f16"]
+CODE = {"f32": 0, "bf16": 1, "f16": 2}
+INF = float("inf")
+
+
+@pytest.fixture(scope="module")
+def eng():
+    return load_pkg_module("engine")
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    return torch
+
+
+def dtype(torch, kind):
+    return {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[kind]
+
+
+def run(eng, torch, kind, l, tokens, temperature=1.0, top=0, ld=None, offset=0, stream=None):
+    rows, n = l.shape
+    ld = ld or n
+    buf = torch.full((offset + rows * ld,), float("nan"), dtype=l.dtype, device="cuda")
+    v = buf[offset:].view(rows, ld)[:, :n]
+    v.copy_(l)
+    tok = torch.as_tensor(tokens, dtype=torch.int32, device="cuda") if tokens is not None else None
+    lp = torch.full((rows + 1,), 7.0, device="cuda")
+    en = torch.full((rows + 1,), 7.0, device="cuda")
+    ids = torch.full((rows * top + 1,), -7, dtype=torch.int32, device="cuda")
+    tlp = torch.full((rows * top + 1,), 7.0, device="cuda")
+    eng.check(eng.lib().ec_op_token_logprobs(
+        CODE[kind], v.data_ptr(), ld, n, rows, tok.data_ptr() if tok is not None else None,
+        temperature, top, lp.data_ptr() if tok is not None else None, en.data_ptr(),
+        ids.data_ptr() if top else None, tlp.data_ptr() if top else None, stream))
+    torch.cuda.synchronize()
+    assert lp[rows] == 7 and en[rows] == 7 and ids[rows * top] == -7 and tlp[rows * top] == 7
+    return (lp[:rows].double().cpu().numpy(), en[:rows].double().cpu().numpy(),
+            ids[:-1].view(rows, top).cpu().numpy(), tlp[:-1].view(rows, top).double().cpu().numpy())
+
+
+def exact(l, temperature):
+    """log probabilities and entropy in 64 bits (l: float64 array)."""
+    z = l / temperature
+    m = z.max(1, keepdims=True)
+    m = np.where(np.isneginf(m), 0.0, m)
+    with np.errstate(divide="ignore", invalid="ignore"):
+        lp = z - m - np.log(np.exp(z - m).sum(1, keepdims=True))
+        lp = np.where(np.isneginf(z), -INF, lp)
+        p = np.exp(lp)
+        return lp, -(np.where(p > 0, p * lp, 0.0)).sum(1)
+
+
+def check(l, tokens, temperature, top, got, n):
+    l64 = l.double().cpu().numpy()
+    lp, en = exact(l64, temperature)
+    glp, gen, ids, tlp = got
+    tol = (n / 64 + 48) * U
+    z = l64 / temperature
+    span = np.abs(lp)
+
+    def near(a, b, size):
+        fine = np.isfinite(b)
+        assert np.array_equal(a[~fine], b[~fine])
+        assert np.all(np.abs(a - b)[fine] <= tol + 4 * U * size[fine]), np.abs(a - b)[fine].max()
+
+    rows = np.arange(l64.shape[0])
+    if tokens is not None:
+        t = np.asarray(tokens)
+        # the difference to the maximum is at most |logprob| + log n
+        near(glp, lp[rows, t], span[rows, t] + np.log(n))
+    near(gen, en, (1 + 2 * np.log(n)) * (1 + n / 64) * np.ones_like(en))
+    if top:
+        order = np.lexsort((np.broadcast_to(np.arange(n), l64.shape), -l64), axis=1)[:, :top]
+        assert np.array_equal(ids, order)
+        want = np.take_along_axis(lp, order, 1)
+        near(tlp.ravel(), want.ravel(), np.abs(want).ravel() + np.log(n))
+    return z
+
+
+SHAPES = [(1, 1), (2, 2), (3, 7), (1, 33), (4, 255), (2, 1000), (3, 4099), (1, 32000), (5, 32003),
+          (2, 128256), (1, 130001), (150, 3000), (700, 257)]
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows,n", SHAPES)
+def test_rows(eng, torch, kind, rows, n):
+    g = torch.Generator(device="cuda").manual_seed(n)
+    l = (torch.randn(rows, n, generator=g, device="cuda") * 4).to(dtype(torch, kind))
+    rng = np.random.default_rng(n)
+    tokens = rng.integers(0, n, rows)
+    for top in sorted({0, 1, min(n, 5), min(n, 20), min(n, 32)}):
+        for temperature in (1.0, 0.7):
+            got = run(eng, torch, kind, l, tokens, temperature, top)
+            check(l, tokens, np.float64(np.float32(temperature)), top, got, n)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("offset,pad", [(0, 1), (1, 0), (3, 5), (8, 8)])
+def test_strides_and_alignment(eng, torch, kind, offset, pad):
+    g = torch.Generator(device="cuda").manual_seed(4)
+    for n in (1001, 4096, 40960):
+        l = (torch.randn(3, n, generator=g, device="cuda") * 3).to(dtype(torch, kind))
+        got = run(eng, torch, kind, l, [0, n - 1, n // 2], 1.0, 7, n + pad, offset)
+        check(l, [0, n - 1, n // 2], 1.0, 7, got, n)
+
+
+@pytest.mark.parametrize("n", [50, 5000, 128256])
+def test_ties_go_to_the_lowest_index(eng, torch, n):
+    l = torch.zeros(4, n, device="cuda")
+    l[1] = torch.arange(n, device="cuda") % 3
+    l[2, :] = -0.0
+    l[2, n // 2] = 0.0  # equal to -0
+    l[3] = torch.arange(n, 0, -1, device="cuda") // 7
+    got = run(eng, torch, "f32", l, [0, 1, 2, 3], 1.0, 32)
+    check(l, [0, 1, 2, 3], 1.0, 32, got, n)
+
+
+@pytest.mark.parametrize("n", [40, 3001, 128256])
+@pytest.mark.parametrize("order", ["up", "down"])
+def test_sorted_rows(eng, torch, n, order):
+    """Rows in order: every value (or none) displaces an alternative."""
+    l = torch.arange(n, device="cuda").float()[None] * 1e-3
+    l = (l if order == "up" else -l).contiguous()
+    got = run(eng, torch, "f32", l, [n - 1], 1.0, 32)
+    check(l, [n - 1], 1.0, 32, got, n)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n", [64, 4099, 128256])
+def test_masked_rows(eng, torch, kind, n):
+    g = torch.Generator(device="cuda").manual_seed(6)
+    l = torch.randn(6, n, generator=g, device="cuda") * 3
+    l[0, 1:] = -INF                      # one token left
+    l[1] = -INF                          # none left
+    l[2, : n - 9] = -INF                 # fewer left than alternatives asked for
+    l[3, 5:] = torch.finfo(dtype(torch, kind)).min  # the type's lowest value is not -inf
+    l[4, ::2] = -INF
+    l = l.to(dtype(torch, kind))
+    tokens = [0, 3, 0, 1, 0, 5]
+    got = run(eng, torch, kind, l, tokens, 1.0, 20)
+    check(l, tokens, 1.0, 20, got, n)
+    assert got[0][0] == 0 and got[1][0] == 0 and got[1][1] == 0
+    assert got[0][1] == -INF and np.all(got[3][1] == -INF)
+    assert np.array_equal(got[2][1], np.arange(20))
+
+
+@pytest.mark.parametrize("n", [64, 4099, 128256])
+def test_nan_and_infinity(eng, torch, n):
+    l = torch.randn(4, n, generator=torch.Generator().manual_seed(2)).cuda()
+    l[0, n - 1] = float("nan")
+    l[1, 3] = INF
+    l[3] = -INF
+    l[3, 7] = float("nan")
+    lp, en, ids, tlp = run(eng, torch, "f32", l, [0, 1, 2, 3], 1.0, 8)
+    for k in (0, 1, 3):
+        assert np.isnan(lp[k]) and np.isnan(en[k]) and np.isnan(tlp[k]).all(), k
+    assert np.isfinite(lp[2]) and np.isfinite(en[2]) and np.isfinite(tlp[2]).all()
+    assert ids[1][0] == 3 and n - 1 not in ids[0] and 7 not in ids[3]
+
+
+def test_tokens_outside_the_row(eng, torch):
+    l = torch.randn(5, 1000, generator=torch.Generator().manual_seed(2)).cuda()
+    lp, en, _, _ = run(eng, torch, "f32", l, [-1, 1000, -2, 2 ** 31 - 1, 999])
+    assert lp[0] == 0 and np.isnan(lp[1:4]).all() and np.isfinite(lp[4])
+    want, went = exact(l.double().cpu().numpy(), 1.0)
+    assert abs(lp[4] - want[4, 999]) < 1e-5 and np.all(np.abs(en - went) < 1e-5)
+
+
+def test_peaked_and_far_logits(eng, torch):
+    """Logits that exp cannot hold (the maximum is taken off first), and a
+    distribution that is one token."""
+    l = torch.tensor([[3e4, 2.9e4, -3e4, 1.0], [-3e38, 3e38, 0.0, 1.0], [1e-30, 0, -1e-30, 0]],
+                     device="cuda")
+    got = run(eng, torch, "f32", l, [0, 1, 2], 1.0, 4)
+    lp, en = exact(l.double().cpu().numpy(), 1.0)
+    assert got[0][0] == 0 and got[0][1] == 0 and abs(got[0][2] + np.log(4)) < 4 * U
+    assert np.all(np.abs(got[1] - en) < 8 * U)
+
+
+def test_equal_calls_give_equal_bits(eng, torch):
+    l = torch.randn(64, 50000, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
+    a = run(eng, torch, "f32", l, list(range(64)), 0.9, 16)
+    b = run(eng, torch, "f32", l, list(range(64)), 0.9, 16)
+    assert all(np.array_equal(x, y) for x, y in zip(a, b))
+
+
+def test_engine_logits(eng, torch, synth):
+    """Engine.logprobs_device on a decode step's own logits, before sampling."""
+    cfg = synth.TINY
+    model = synth.make_model(cfg, seed=7)
+    e = eng.Engine(cfg)
+    e.load(model)
+    tok = torch.tensor([5], dtype=torch.int32, device="cuda")
+    pos = torch.tensor([0], dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    e.step_device(tok.data_ptr(), pos.data_ptr(), 1, feedback=True)  # tok: the greedy token
+    lp = torch.zeros(1, device="cuda")
+    en = torch.zeros(1, device="cuda")
+    ids = torch.zeros(1, 4, dtype=torch.int32, device="cuda")
+    tlp = torch.zeros(1, 4, device="cuda")
+    torch.cuda.synchronize()
+    e.logprobs_device(1, tok.data_ptr(), lp.data_ptr(), en.data_ptr(), 4, ids.data_ptr(),
+                      tlp.data_ptr(), temperature=0.7)
+    e.sync()
+    logits = e.state(6, n=cfg.vocab_size)[None].astype(np.float64)
+    want, went = exact(logits, np.float64(np.float32(0.7)))
+    t = int(tok.item())
+    assert t == ids[0, 0].item() == int(np.argmax(logits[0]))
+    tol = (cfg.vocab_size / 64 + 48) * U + 8 * U * np.log(cfg.vocab_size)
+    assert abs(lp.item() - want[0, t]) <= tol and lp.item() == tlp[0, 0].item()
+    assert abs(en.item() - went[0]) <= tol * (1 + 2 * np.log(cfg.vocab_size))
+    e.close()

@@ -1,0 +1,304 @@
+"""ec_op_gemm_w8a8 (through the C ABI) against the integer product in 64 bits,
+and the feed-forward and scoring runs that its neighbours make with it.
+
+Tolerance of the product: the int32 sum is exact; its conversion to f32 and
+the two scalings are three roundings of 2^-24 of the result, and the rounding
+to the output's type is half a step of it.
+"""
+import numpy as np
+import pytest
+
+from conftest import load_pkg_module
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+TYPES = ["f32", "bf16", "f16"]
+CODE = {"f32": 0, "bf16": 1, "f16": 2}
+
+
+@pytest.fixture(scope="module")
+def eng():
+    return load_pkg_module("engine")
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    return torch
+
+
+def dtype(torch, kind):
+    return {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[kind]
+
+
+def int8_rows(torch, rows, k, ld, seed, lo=-128, hi=128):
+    """Every byte value, rows ld apart; what lies behind a row's end is 101."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    buf = torch.full((rows, ld), 101, dtype=torch.int8, device="cuda")
+    buf[:, :k] = torch.randint(lo, hi, (rows, k), generator=g, device="cuda", dtype=torch.int32)
+    return buf
+
+
+def run(eng, torch, kind, x, w, sx, sw, k, ldy=None, offset=0, stream=None, y=None):
+    nb, m = x.shape[0], w.shape[0]
+    ldy = ldy or m
+    buf = torch.full((offset + nb * ldy + 1,), 7.0, dtype=dtype(torch, kind), device="cuda")
+    yv = buf[offset:offset + nb * ldy].view(nb, ldy)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    eng.check(eng.lib().ec_op_gemm_w8a8(
+        x.data_ptr(), x.stride(0), sx.data_ptr(), w.data_ptr(), w.stride(0), sw.data_ptr(),
+        CODE[kind], yv.data_ptr(), ldy, m, k, nb, status.data_ptr(), stream))
+    torch.cuda.synchronize()
+    assert status.item() == 0
+    assert (buf[:offset] == 7).all() and (yv[:, m:] == 7).all() and buf[-1] == 7
+    return yv[:, :m]
+
+
+def exact(torch, x, w, sx, sw, k):
+    acc = x[:, :k].double() @ w[:, :k].double().t()  # below 2^53: exact
+    return acc * sx.double()[:, None] * sw.double()
+
+
+def check(torch, kind, y, want):
+    half = torch.finfo(dtype(torch, kind)).eps / 2
+    floor = torch.finfo(dtype(torch, kind)).tiny * half if kind == "f16" else 0.0
+    err = (y.double() - want).abs()
+    tol = want.abs() * (3.01 * U + (half if kind != "f32" else 0.0)) + floor
+    assert bool((err <= tol).all()), float((err - tol).max())
+
+
+def scales(torch, nb, m, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.rand(nb, generator=g, device="cuda") * 0.05 + 0.001,
+            torch.rand(m, generator=g, device="cuda") * 1e-3 + 1e-5)
+
+
+SHAPES = [  # tokens, channels, k
+    (1, 1, 1), (1, 1, 16), (2, 3, 5), (1, 128, 128), (1, 129, 127), (16, 128, 128), (17, 100, 129),
+    (1, 4096, 4096), (1, 6144, 4096), (3, 5003, 513), (8, 1024, 14336), (16, 28672, 512),
+    (31, 777, 1000), (32, 512, 512), (33, 32000, 512), (48, 130, 4096), (64, 4096, 1024),
+    (65, 257, 4095), (80, 300, 300), (127, 129, 2048), (128, 256, 256), (129, 1000, 640),
+    (200, 4096, 512), (255, 255, 255), (256, 256, 4096), (257, 513, 1025), (384, 2000, 384),
+    (512, 512, 512), (517, 5003, 1433), (700, 128, 8192), (1000, 1000, 100), (1024, 6144, 256),
+    (2048, 4096, 512), (2049, 700, 129), (5000, 64, 64), (1, 1, 131071), (300, 1, 70), (1, 128256, 512)]
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("nb,m,k", SHAPES)
+def test_product(eng, torch, kind, nb, m, k):
+    ld = -(-k // 16) * 16
+    x, w = int8_rows(torch, nb, k, ld, nb), int8_rows(torch, m, k, ld, m + 1)
+    sx, sw = scales(torch, nb, m, k)
+    y = run(eng, torch, kind, x, w, sx, sw, k)
+    check(torch, kind, y, exact(torch, x, w, sx, sw, k))
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("nb", [1, 20, 100, 300, 600])
+def test_strides(eng, torch, kind, nb):
+    """Long row strides, an output at any element, odd output strides."""
+    m, k = 333, 777
+    x, w = int8_rows(torch, nb, k, 784 + 48, 1), int8_rows(torch, m, k, 784 + 160, 2)
+    sx, sw = scales(torch, nb, m, 3)
+    for ldy, offset in ((m, 1), (m + 1, 0), (m + 3, 5), (m + 51, 0)):
+        y = run(eng, torch, kind, x, w, sx, sw, k, ldy, offset)
+        check(torch, kind, y, exact(torch, x, w, sx, sw, k))
+
+
+@pytest.mark.parametrize("nb", [1, 40, 200, 513])
+def test_largest_sums(eng, torch, nb):
+    """Rows of the extreme byte values: the int32 sum at its limits."""
+    for k in (4096, 131071):
+        ld = -(-k // 16) * 16
+        x = torch.full((nb, ld), -128, dtype=torch.int8, device="cuda")
+        w = torch.full((130, ld), -128, dtype=torch.int8, device="cuda")
+        w[1::2] = 127
+        sx, sw = torch.ones(nb, device="cuda"), torch.ones(130, device="cuda")
+        y = run(eng, torch, "f32", x, w, sx, sw, k)
+        check(torch, "f32", y, exact(torch, x, w, sx, sw, k))
+
+
+def test_nan_scales_stay_in_their_rows(eng, torch):
+    """A row whose 8-bit scale is NaN (see the 8-bit rule) gives a NaN row."""
+    for nb in (5, 300):
+        x, w = int8_rows(torch, nb, 256, 256, 1), int8_rows(torch, 200, 256, 256, 2)
+        sx, sw = scales(torch, nb, 200, 4)
+        sx[3] = float("nan")
+        x[3] = 0
+        y = run(eng, torch, "f32", x, w, sx, sw, 256)
+        assert y[3].isnan().all() and y[:3].isfinite().all() and y[4:].isfinite().all()
+
+
+def test_status_may_be_left_out(eng, torch):
+    x, w = int8_rows(torch, 9, 512, 512, 1), int8_rows(torch, 300, 512, 512, 2)
+    sx, sw = scales(torch, 9, 300, 4)
+    y = torch.empty(9, 300, device="cuda")
+    eng.check(eng.lib().ec_op_gemm_w8a8(x.data_ptr(), 512, sx.data_ptr(), w.data_ptr(), 512,
+                                        sw.data_ptr(), 0, y.data_ptr(), 300, 300, 512, 9, None,
+                                        None))
+    torch.cuda.synchronize()
+    check(torch, "f32", y, exact(torch, x, w, sx, sw, 512))
+
+
+def test_two_streams_at_once(eng, torch):
+    """Calls in flight on two streams share nothing."""
+    sets = []
+    for j, (nb, m, k) in enumerate([(40, 4096, 2048), (700, 2048, 1024), (3, 6000, 4096),
+                                    (300, 1024, 2048)]):
+        x, w = int8_rows(torch, nb, k, k, j), int8_rows(torch, m, k, k, j + 9)
+        sx, sw = scales(torch, nb, m, j)
+        sets.append((x, w, sx, sw, k, torch.zeros(nb, m, device="cuda")))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for rep in range(6):
+        for j, (x, w, sx, sw, k, y) in enumerate(sets):
+            eng.check(eng.lib().ec_op_gemm_w8a8(
+                x.data_ptr(), k, sx.data_ptr(), w.data_ptr(), k, sw.data_ptr(), 0, y.data_ptr(),
+                y.shape[1], y.shape[1], k, y.shape[0], None, streams[j % 2].cuda_stream))
+    torch.cuda.synchronize()
+    for x, w, sx, sw, k, y in sets:
+        check(torch, "f32", y, exact(torch, x, w, sx, sw, k))
+
+
+# ------------------------------------------------------------------ runs --
+
+
+class Block:
+    """One feed-forward block and the scoring of its result: bf16 rows, INT8
+    weights, the calls in the order a user makes them, on one stream."""
+
+    def __init__(self, torch, nb, d, f, v, seed=0):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+
+        def rand(*s):
+            return torch.randn(*s, generator=g, device="cuda")
+
+        def weight(m, k):
+            w = rand(m, k) * k ** -0.5
+            s = w.abs().amax(1) / 127
+            return torch.round(w / s[:, None]).to(torch.int8), s
+
+        bf = torch.bfloat16
+        self.nb, self.d, self.f, self.v = nb, d, f, v
+        self.x, self.res = rand(nb, d).to(bf), (rand(nb, d) * 2).to(bf)
+        self.n1, self.n2 = (1 + 0.1 * rand(d)).to(bf), (1 + 0.1 * rand(d)).to(bf)
+        self.w13, self.w2, self.lm = weight(2 * f, d), weight(d, f), weight(v, d)
+        self.tokens = torch.randint(0, v, (nb,), generator=g, device="cuda", dtype=torch.int32)
+        e = lambda *s, dt=bf: torch.zeros(*s, dtype=dt, device="cuda")  # noqa: E731
+        self.h1, self.h2 = e(nb, d), e(nb, d)
+        self.q1, self.q2, self.q3 = (e(nb, n, dt=torch.int8) for n in (d, f, d))
+        self.s1, self.s2, self.s3 = (e(nb, dt=torch.float32) for _ in range(3))
+        self.gu, self.down, self.logits = e(nb, 2 * f), e(nb, d), e(nb, v, dt=torch.float32)
+        self.lp, self.en = e(nb, dt=torch.float32), e(nb, dt=torch.float32)
+        self.ids, self.tlp = e(nb, 5, dt=torch.int32), e(nb, 5, dt=torch.float32)
+
+    def call(self, eng, stream):
+        L, c, nb, d, f, v = eng.lib(), eng.check, self.nb, self.d, self.f, self.v
+        p = lambda t: t.data_ptr()  # noqa: E731
+        c(L.ec_op_add_rmsnorm_quant(1, p(self.x), d, p(self.res), d, p(self.h1), d, p(self.n1),
+                                    1e-5, nb, d, p(self.q1), d, p(self.s1), stream))
+        c(L.ec_op_gemm_w8a8(p(self.q1), d, p(self.s1), p(self.w13[0]), d, p(self.w13[1]), 1,
+                            p(self.gu), 2 * f, 2 * f, d, nb, None, stream))
+        c(L.ec_op_silu_mul_quant(1, p(self.gu), p(self.gu) + 2 * f, 2 * f, nb, f, p(self.q2), f,
+                                 p(self.s2), stream))
+        c(L.ec_op_gemm_w8a8(p(self.q2), f, p(self.s2), p(self.w2[0]), f, p(self.w2[1]), 1,
+                            p(self.down), d, d, f, nb, None, stream))
+        c(L.ec_op_add_rmsnorm_quant(1, p(self.down), d, p(self.h1), d, p(self.h2), d, p(self.n2),
+                                    1e-5, nb, d, p(self.q3), d, p(self.s3), stream))
+        c(L.ec_op_gemm_w8a8(p(self.q3), d, p(self.s3), p(self.lm[0]), d, p(self.lm[1]), 0,
+                            p(self.logits), v, v, d, nb, None, stream))
+        c(L.ec_op_token_logprobs(0, p(self.logits), v, v, nb, p(self.tokens), 1.0, 5, p(self.lp),
+                                 p(self.en), p(self.ids), p(self.tlp), stream))
+
+    def results(self):
+        return [t.clone() for t in (self.h1, self.h2, self.q3, self.s3, self.logits, self.lp,
+                                    self.en, self.ids, self.tlp)]
+
+    def want(self, torch):
+        """The block in 64 bits, without any 8-bit rounding of activations."""
+        def norm(h, w):
+            return h / (h.square().mean(1, keepdim=True) + 1e-5).sqrt() * w.double()
+
+        def mul(y, w):
+            return y @ (w[0].double() * w[1].double()[:, None]).t()
+
+        h1 = self.x.double() + self.res.double()
+        gu = mul(norm(h1, self.n1), self.w13)
+        act = torch.sigmoid(gu[:, :self.f]) * gu[:, :self.f] * gu[:, self.f:]
+        h2 = h1 + mul(act, self.w2)
+        logits = mul(norm(h2, self.n2), self.lm)
+        return h2, torch.log_softmax(logits, 1)
+
+
+def rel(a, b):
+    return float((a.double() - b).norm() / b.norm())
+
+
+@pytest.mark.parametrize("nb", [1, 5, 64, 300])
+def test_block_and_scoring(eng, torch, nb):
+    """The run of the operators as they are used together.
+
+    8-bit rows: a value is off by at most half a step, amax / 254; normal rows
+    of these widths have amax below 5.5 of their root mean square, so the error
+    is below 5.5 / 254 / sqrt(3) = 0.0125 of it; SwiGLU rows are heavier:
+    amax below 25, 0.057.  bf16 rounds to 2^-9 in the mean.  The gate/up
+    product carries the first, the activation at most 3 times that and its
+    own, the sum h2 that of its part (smaller than the residual's)."""
+    b = Block(torch, nb, 512, 1408, 4096, seed=nb)
+    b.call(eng, None)
+    torch.cuda.synchronize()
+    h2, lsm = b.want(torch)
+    assert rel(b.h2, h2) < 0.0125 * 3 + 0.057 + 3 * 2 ** -9
+    at = lsm.gather(1, b.tokens.long()[:, None])[:, 0]
+    # logits are of root mean square 1; the log probability's error is a
+    # difference of two of them: 6 standard deviations of the bound above
+    assert float((b.lp.double() - at).abs().max()) < 6 * 1.5 * (0.0125 * 4 + 0.057)
+    # inside the scoring the numbers agree with one another to f32
+    own = torch.log_softmax(b.logits.double(), 1)
+    assert float((own.gather(1, b.ids.long()) - b.tlp).abs().max()) < 1e-5
+    assert torch.equal(b.ids[:, 0].long(), b.logits.argmax(1))
+
+
+def test_block_captured_and_replayed(eng, torch):
+    """Two captured graphs of the run replay on new inputs and interleave with
+    eager calls; every replay gives the eager call's bits."""
+    blocks = [Block(torch, 40, 512, 1408, 4096, seed=1), Block(torch, 200, 512, 1408, 4096, seed=2)]
+    other = [Block(torch, 40, 512, 1408, 4096, seed=3), Block(torch, 200, 512, 1408, 4096, seed=4)]
+    eager = []
+    for b, o in zip(blocks, other):
+        b.call(eng, None)
+        torch.cuda.synchronize()
+        first = b.results()
+        keep = b.x.clone(), b.res.clone()
+        b.x.copy_(o.x)
+        b.res.copy_(o.res)
+        torch.cuda.synchronize()
+        b.call(eng, None)
+        torch.cuda.synchronize()
+        eager.append((first, b.results()))
+        b.x.copy_(keep[0])
+        b.res.copy_(keep[1])
+    graphs = []
+    for b in blocks:
+        g = torch.cuda.CUDAGraph()
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.graph(g, stream=s):
+            b.call(eng, torch.cuda.current_stream().cuda_stream)
+        graphs.append(g)
+    for k in (0, 1):
+        if k:
+            for b, o in zip(blocks, other):
+                b.x.copy_(o.x)
+                b.res.copy_(o.res)
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        for rep in range(3):
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        for b, want in zip(blocks, eager):
+            assert all(torch.equal(p, q) for p, q in zip(b.results(), want[k]))
