@@ -3,61 +3,468 @@
 //
 //   y[t][c] = (x_scale[t] * sum_k x[t][k] w[c][k]) * w_scale[c]
 //
-// A 64 x 64 tile per CTA from shared memory, four byte products an instruction.
+// Both operands are K-major bytes as the caller keeps them; TMA boxes of
+// 128 bytes of K bring them into shared memory in the 128-byte swizzle, and
+// tcgen05.mma kind::i8 multiplies them with the channels as the MMA's M and
+// the tokens as its N, into int32 accumulators in TMEM: one TMEM lane is one
+// channel, so a warp's store of one token is contiguous in y.  Columns of K
+// behind k are zero (the tensor map's fill); rows of a tile behind the last
+// channel or token are whatever shared memory held, and land in accumulators
+// that are not stored.
+//
+// The sum is exact in int32, so neither the tiles nor the split over K change
+// a bit of the result.
+//
+// gemm_w8a8_kernel: a tile is R <= 128 channels x up to 256 tokens.  With few
+// tokens the weights' bytes are the bound, and R is chosen so that the tiles
+// fill whole rounds of the SMs (every SM streams the same share of the
+// weights); the MMA computes its 128 rows whatever R is, which costs
+// nothing there.  With C > 1 a cluster of C CTAs splits K: the partial
+// accumulators meet in distributed shared memory, each CTA finishing a part of
+// the token columns.  Warp 0 streams, warp 1 issues the MMAs, warps 2-5 drain
+// TMEM; two TMEM buffers let a tile's epilogue run under the next one's MMAs.
+#include <cuda.h>
+
 #include "typed.cuh"
 
 namespace ec {
 namespace {
 
 constexpr int kMaxK = 131071;  // 128 * 128 * k < 2^31
+constexpr int kKb = 128;       // K bytes of one TMA box: one 128-byte swizzle row
+constexpr int kThreads = 192;
+constexpr int kMaxStages = 24;
+constexpr int kHdr = 1024;
+constexpr int kSmemMax = 227 * 1024;
+constexpr int kMaxCluster = 8;
 
 struct W8A8Args {
-  const int8_t* x;
-  const int8_t* w;
   const float* sx;
   const float* sw;
   void* y;
-  long ldx, ldw, ldy;
-  int m, k, nb;
+  long ldy;
+  int m, nb;
+  int chunks;   // 128-byte blocks of K
+  int R, Tn;    // a tile's channels and tokens (Tn a multiple of 16)
+  int mt, nt;   // tiles
+  int xrows;    // token rows of one box: min(Tn, nb)
+  int ks, S;    // blocks of K per stage, stages
+  int C;        // CTAs that share a tile's K
   int* status;
 };
 
-__device__ __forceinline__ int load4(const int8_t* row, int k0, int k) {
-  if (k0 + 4 <= k) return *reinterpret_cast<const int*>(row + k0);
-  unsigned v = 0;
-  for (int i = 0; i < 4; i++)
-    if (k0 + i < k) v |= (unsigned)(uint8_t)row[k0 + i] << (8 * i);
-  return (int)v;
+// ------------------------------------------------------------ tcgen05 --
+
+// K-major, 128-byte swizzle: start address, 1024 bytes between groups of 8
+// rows, descriptor version 1, layout 2.  A step of 32 bytes along K inside
+// the swizzle row is a step of the start address.
+__device__ __forceinline__ uint64_t sw128_desc(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t acc) {
+  asm volatile(
+      "{ .reg .pred p; setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p; }" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+// D s32, A and B signed 8 bit, both K-major
+__host__ __device__ constexpr uint32_t i8_idesc(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(m >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+          smem_u32(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void tc_fence_after() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tc_fence_before() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, int* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y,
+                                       uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, "
+      "{%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// this CTA's shared address -> the same place in CTA `rank` of the cluster
+__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void st_peer(uint32_t addr, int v) {
+  asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+__device__ __forceinline__ float scaled(int acc, float sx, float sw) {
+  return __fmul_rn(__fmul_rn((float)acc, sx), sw);
+}
+
+// ---------------------------------------------------------------- kernel --
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+    gemm_w8a8_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mw,
+                     const W8A8Args a) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem);
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* tfull = empty + kMaxStages;
+  uint64_t* tempty = tfull + 2;
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(tempty + 2);
+  int* failed = reinterpret_cast<int*>(tslot + 1);
+  uint8_t* stg = smem + kHdr;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int C = a.C, rank = C > 1 ? (int)cluster_rank() : 0;
+  const int first = blockIdx.x / C, step = gridDim.x / C, tiles = a.mt * a.nt;
+  // this CTA's blocks of K
+  const int c0 = (int)((long)rank * a.chunks / C), c1 = (int)((long)(rank + 1) * a.chunks / C);
+  const int per_tile = (c1 - c0 + a.ks - 1) / a.ks;  // stages of one tile
+  const uint32_t xbytes = (uint32_t)a.Tn * kKb, wbytes = (uint32_t)((a.R + 7) & ~7) * kKb;
+  const uint32_t block = xbytes + wbytes, stage = block * a.ks;
+  const uint32_t block_tx = (uint32_t)(a.xrows + a.R) * kKb;
+  const uint32_t tcols = a.Tn <= 16 ? 32u : a.Tn <= 32 ? 64u : a.Tn <= 64 ? 128u : a.Tn <= 128 ? 256u : 512u;
+
+  if (tid == 0) {
+    for (int s = 0; s < a.S; s++) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], 4);
+    }
+    *failed = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tslot)), "r"(tcols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = *tslot;
+  bool ok = true;
+
+  if (warp == 0) {
+    // ---------------------------------------------------------- producer
+    if (lane == 0) {
+      int u = 0;
+      for (int tile = first; tile < tiles && ok; tile += step) {
+        const int c = tile / a.nt * a.R, t = tile % a.nt * a.Tn;
+        for (int i = 0; i < per_tile && ok; i++, u++) {
+          const int s = u % a.S;
+          if (u >= a.S) {
+            ok = mbar_wait(&empty[s], (uint32_t)((u / a.S - 1) & 1), a.status);
+            if (!ok) break;
+          }
+          const int b0 = c0 + i * a.ks, nblk = min(a.ks, c1 - b0);
+          mbar_expect_tx(&full[s], block_tx * nblk);
+          const uint32_t bar = smem_u32(&full[s]);
+          uint32_t dst = smem_u32(stg) + s * stage;
+          for (int b = 0; b < nblk; b++, dst += block) {
+            tma_2d(dst, &mx, (b0 + b) * kKb, t, bar);
+            tma_2d(dst + xbytes, &mw, (b0 + b) * kKb, c, bar);
+          }
+        }
+      }
+      if (!ok)  // the copies in flight land before the CTA may end
+        for (int v = max(0, u - a.S); v < u; v++)
+          mbar_wait(&full[v % a.S], (uint32_t)((v / a.S) & 1), a.status);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // -------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      const uint32_t idesc = i8_idesc(128, a.Tn);
+      int u = 0, n = 0;
+      for (int tile = first; tile < tiles && ok; tile += step, n++) {
+        const int buf = n & 1;
+        if (n >= 2) ok = mbar_wait(&tempty[buf], (uint32_t)(((n >> 1) - 1) & 1), a.status);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t d = tbase + (uint32_t)(buf * (tcols >> 1));
+        for (int i = 0; i < per_tile; i++, u++) {
+          const int s = u % a.S;
+          ok = mbar_wait(&full[s], (uint32_t)((u / a.S) & 1), a.status);
+          if (!ok) break;
+          tc_fence_after();
+          const int nblk = min(a.ks, c1 - c0 - i * a.ks);
+          uint32_t src = smem_u32(stg) + s * stage;
+          for (int b = 0; b < nblk; b++, src += block) {
+            const uint64_t db = sw128_desc(src), da = sw128_desc(src + xbytes);
+#pragma unroll
+            for (int j = 0; j < kKb / 32; j++)
+              mma_i8(d, da + 2 * j, db + 2 * j, idesc, (i > 0 || b > 0 || j > 0) ? 1u : 0u);
+          }
+          mma_commit(&empty[s]);
+        }
+        if (!ok) {
+          *failed = 1;
+          __threadfence_block();
+        }
+        // also where a wait gave up: the MMAs in flight end before the rest
+        mma_commit(&tfull[buf]);
+      }
+    }
+    __syncwarp();
+  } else if (C == 1) {
+    // ----------------------------------------------------------- epilogue
+    const int q = warp & 3;  // TMEM lanes 32q .. 32q + 31 (this warp's quadrant)
+    const int r = q * 32 + lane;
+    int n = 0;
+    for (int tile = first; tile < tiles; tile += step, n++) {
+      const int c = tile / a.nt * a.R + r, t0 = tile % a.nt * a.Tn;
+      const bool mine = r < a.R && c < a.m;
+      const int buf = n & 1;
+      ok = ok && mbar_wait(&tfull[buf], (uint32_t)((n >> 1) & 1), a.status) &&
+           *reinterpret_cast<volatile int*>(failed) == 0;
+      tc_fence_after();
+      const uint32_t ta = tbase + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * (tcols >> 1));
+      float sw = mine ? a.sw[c] : 0.0f;
+      if (!ok) sw = __uint_as_float(0x7fc00000u);
+      const int tn = min(a.Tn, a.nb - t0);
+      T* y = static_cast<T*>(a.y) + (long)t0 * a.ldy + c;
+      for (int j0 = 0; j0 < tn; j0 += 16) {
+        const float sxl = a.sx[t0 + min(j0 + (lane & 15), tn - 1)];
+        int acc[16];
+        tmem_ld16(ta + j0, acc);
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+          const float sx = __shfl_sync(0xffffffffu, sxl, j);
+          if (mine && j0 + j < tn)
+            y[(long)(j0 + j) * a.ldy] = from_f32<T>(scaled(acc[j], sx, sw));
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tempty[buf]);
+    }
+  }
+  if (C > 1) {
+    // One tile per cluster.  The stages become the exchange buffer
+    // [CTA of the cluster][its token columns][128 channels] once every CTA's
+    // MMAs have read them.
+    const int wc = (a.Tn + C - 1) / C;  // token columns each CTA finishes
+    const int q = warp & 3, r = q * 32 + lane;
+    const int c = first / a.nt * a.R + r, t0 = first % a.nt * a.Tn;
+    if (warp >= 2) {
+      ok = mbar_wait(&tfull[0], 0, a.status);
+      tc_fence_after();
+    }
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    if (warp >= 2) {
+      ok = ok && *reinterpret_cast<volatile int*>(failed) == 0;
+      if (!ok && lane == 0)
+        for (int p = 0; p < C; p++) st_peer(peer_addr(smem_u32(failed), p), 1);
+      const uint32_t at = smem_u32(stg) + (uint32_t)(rank * wc * 512 + r * 4);
+      const uint32_t ta = tbase + ((uint32_t)(q * 32) << 16);
+      int owner = 0, col = 0;  // of the next column
+      uint32_t dst = peer_addr(at, 0);
+      for (int j0 = 0; j0 < a.Tn; j0 += 16) {
+        int acc[16];
+        tmem_ld16(ta + j0, acc);
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+          st_peer(dst, acc[j]);
+          dst += 512;
+          if (++col == wc) {
+            col = 0;
+            if (++owner < C) dst = peer_addr(at, owner);
+          }
+        }
+      }
+      tc_fence_before();
+    }
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    if (warp >= 2 && r < a.R && c < a.m) {
+      const int tn = min(min(a.Tn, a.nb - t0), (rank + 1) * wc) - rank * wc;
+      const int* part = reinterpret_cast<const int*>(stg) + r;
+      const float sw =
+          *reinterpret_cast<volatile int*>(failed) ? __uint_as_float(0x7fc00000u) : a.sw[c];
+      const int tt = t0 + rank * wc;
+      T* y = static_cast<T*>(a.y) + (long)tt * a.ldy + c;
+      for (int j = 0; j < tn; j++) {
+        int acc = 0;
+        for (int p = 0; p < C; p++) acc += part[(p * wc + j) * 128];
+        y[(long)j * a.ldy] = from_f32<T>(scaled(acc, a.sx[tt + j], sw));
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(tcols)
+                 : "memory");
+  }
+}
+
+// ------------------------------------------------------------------ host --
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// The driver's encoder, looked up through the runtime: the library itself
+// does not need libcuda to load.
+EncodeTiled encoder() {
+  static EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) !=
+            cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+
+// rows of k bytes, ld apart, in boxes of 128 bytes x `box` rows
+bool byte_map(CUtensorMap* map, const void* p, long k, long rows, long ld, int box) {
+  const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld};
+  const cuuint32_t boxes[2] = {(cuuint32_t)kKb, (cuuint32_t)box};
+  const cuuint32_t ones[2] = {1, 1};
+  return encoder()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides,
+                   boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct Plan {
+  int R, Tn, mt, nt, C;
+  double cost;
+};
+
+inline int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
+
+// The tile for m x k weights and nb tokens on n_sm SMs: the cheapest of the
+// token splits and cluster sizes under the model below (cycles).
+Plan plan_tiles(int m, int chunks, int nb, int n_sm) {
+  Plan best{0, 0, 0, 0, 0, 1e300};
+  const int nt0 = ceil_div(nb, 256);
+  for (int nt = nt0; nt <= nt0 * 4 && (nt == nt0 || nb >= 64 * nt); nt *= 2) {
+    const int Tn = ceil_div(ceil_div(nb, nt), 16) * 16;
+    const int cols = ceil_div(nb, Tn);
+    for (int C = 1; C <= kMaxCluster; C++) {
+      if (C > chunks) break;
+      const int slots = n_sm / C;
+      int rounds = ceil_div((long)ceil_div(m, 128) * cols, slots);
+      if (C > 1 && rounds > 1) break;
+      // the most tiles those rounds hold, then the rows each needs
+      int mt = (int)((long)rounds * slots / cols);
+      int R = ceil_div(m, mt);
+      if (R > 128) R = 128;
+      R = R < 8 ? (m < 8 ? m : 8) : R;
+      mt = ceil_div(m, R);
+      const double per_sm = (double)rounds * ceil_div(chunks, C);  // blocks of K per SM
+      const double load = per_sm * (R + Tn) * kKb / 34.0;          // bytes a cycle into an SM
+      const double mma = per_sm * (Tn < 32 ? 64.0 : 2.0 * Tn);
+      const double join = C > 1 ? 2000.0 + 20.0 * Tn : 0.0;
+      const double cost = (load > mma ? load : mma) + join;
+      if (cost < best.cost) best = Plan{R, Tn, mt, cols, C, cost};
+    }
+  }
+  return best;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) gemm_w8a8_kernel(W8A8Args a) {
-  __shared__ int xs[64][17], ws[64][17];
-  const int c0 = blockIdx.x * 64, t0 = blockIdx.y * 64;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  int acc[4][4] = {};
-  for (int k0 = 0; k0 < a.k; k0 += 64) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-      const int r = i >> 4, kk = (i & 15) * 4;
-      xs[r][i & 15] = t0 + r < a.nb ? load4(a.x + (t0 + r) * a.ldx, k0 + kk, a.k) : 0;
-      ws[r][i & 15] = c0 + r < a.m ? load4(a.w + (c0 + r) * a.ldw, k0 + kk, a.k) : 0;
-    }
-    __syncthreads();
-    for (int kk = 0; kk < 16; kk++)
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-          acc[i][j] = __dp4a(xs[ty + 16 * i][kk], ws[tx + 16 * j][kk], acc[i][j]);
+int launch(const int8_t* x, long ldx, const int8_t* w, long ldw, int k, W8A8Args a,
+           cudaStream_t st) {
+  if (!encoder()) {
+    ec_set_last_error("ec_op_gemm_w8a8: the driver has no tensor-map encoder");
+    return EC_ERR_CUDA;
   }
-  for (int i = 0; i < 4; i++)
-    for (int j = 0; j < 4; j++) {
-      const int t = t0 + ty + 16 * i, c = c0 + tx + 16 * j;
-      if (t < a.nb && c < a.m)
-        static_cast<T*>(a.y)[t * a.ldy + c] =
-            from_f32<T>(__fmul_rn(__fmul_rn((float)acc[i][j], a.sx[t]), a.sw[c]));
-    }
+  int dev = 0, n_sm = 0;
+  EC_CUDA_TRY(cudaGetDevice(&dev));
+  EC_CUDA_TRY(cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, dev));
+  a.chunks = ceil_div(k, kKb);
+  const Plan p = plan_tiles(a.m, a.chunks, a.nb, n_sm);
+  a.R = p.R;
+  a.Tn = p.Tn;
+  a.mt = p.mt;
+  a.nt = p.nt;
+  a.C = p.C;
+  a.xrows = a.nb < a.Tn ? a.nb : a.Tn;
+  const int block = (a.Tn + ((a.R + 7) & ~7)) * kKb;
+  const int share = ceil_div(a.chunks, a.C);
+  a.ks = 1;
+  while (a.ks < 4 && block * a.ks < 12288 && a.ks * 2 <= share) a.ks *= 2;
+  // the last block's MMA reads 128 rows from its weights on
+  const int slack = 128 * kKb;
+  a.S = (kSmemMax - kHdr - slack) / (block * a.ks);
+  if (a.S > kMaxStages) a.S = kMaxStages;
+  const size_t smem = kHdr + (size_t)a.S * block * a.ks + slack;
+  CUtensorMap mx, mw;
+  if (!byte_map(&mx, x, k, a.nb, ldx, a.xrows) || !byte_map(&mw, w, k, a.m, ldw, a.R)) {
+    ec_set_last_error("ec_op_gemm_w8a8: tensor map refused");
+    return EC_ERR_CUDA;
+  }
+  const auto kern = gemm_w8a8_kernel<T>;
+  EC_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax));
+  const int tiles = a.mt * a.nt;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.C > 1 ? tiles * a.C : tiles < n_sm ? tiles : n_sm);
+  cfg.blockDim = dim3(kThreads);
+  // more than half of an SM's shared memory: no two CTAs of these kernels ever
+  // share an SM's TMEM, so clusters cannot wait for one another's columns
+  cfg.dynamicSmemBytes = smem > 120 * 1024 ? smem : 120 * 1024;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)a.C;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  EC_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, mx, mw, a));
+  return EC_OK;
 }
 
 }  // namespace
@@ -75,13 +482,16 @@ extern "C" int ec_op_gemm_w8a8(const int8_t* x, int64_t ldx, const float* x_scal
        (uintptr_t)ldw) & 15)
     return ec::arg_error("ec_op_gemm_w8a8: x, w, ldx and ldw must be multiples of 16 bytes");
   if (k > ec::kMaxK) return ec::unsupported("ec_op_gemm_w8a8: k > 131071");
-  const ec::W8A8Args a{x, w, x_scale, w_scale, y, (long)ldx, (long)ldw, (long)ldy, m, k, nb, status};
-  const dim3 grid((m + 63) / 64, (nb + 63) / 64);
-  if (grid.y > 65535) return ec::unsupported("ec_op_gemm_w8a8: too many rows");
+  ec::W8A8Args a{};
+  a.sx = x_scale;
+  a.sw = w_scale;
+  a.y = y;
+  a.ldy = (long)ldy;
+  a.m = m;
+  a.nb = nb;
+  a.status = status;
   return ec::with_type(type, [&](auto t) {
-    ec::gemm_w8a8_kernel<decltype(t)>
-        <<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(a);
-    EC_CUDA_TRY(cudaGetLastError());
-    return EC_OK;
+    return ec::launch<decltype(t)>(x, (long)ldx, w, (long)ldw, k, a,
+                                   static_cast<cudaStream_t>(stream));
   });
 }
