@@ -23,6 +23,9 @@
 // accumulators meet in distributed shared memory, each CTA finishing a part of
 // the token columns.  Warp 0 streams, warp 1 issues the MMAs, warps 2-5 drain
 // TMEM; two TMEM buffers let a tile's epilogue run under the next one's MMAs.
+#include <atomic>
+#include <mutex>
+
 #include <cuda.h>
 
 #include "typed.cuh"
@@ -133,6 +136,12 @@ __device__ __forceinline__ void st_peer(uint32_t addr, int v) {
   asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
+__device__ __forceinline__ void st_peer4(uint32_t addr, const int* v) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3])
+               : "memory");
+}
+
 __device__ __forceinline__ float scaled(int acc, float sx, float sw) {
   return __fmul_rn(__fmul_rn((float)acc, sx), sw);
 }
@@ -183,21 +192,21 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_launch_dependents();
   const uint32_t tbase = *tslot;
   bool ok = true;
 
   if (warp == 0) {
     // ---------------------------------------------------------- producer
     if (lane == 0) {
-      int u = 0;
+      pdl_wait();
+      int u = 0, s = 0;
+      uint32_t phase = 1;  // a fresh barrier's previous phase counts as complete
       for (int tile = first; tile < tiles && ok; tile += step) {
         const int c = tile / a.nt * a.R, t = tile % a.nt * a.Tn;
-        for (int i = 0; i < per_tile && ok; i++, u++) {
-          const int s = u % a.S;
-          if (u >= a.S) {
-            ok = mbar_wait(&empty[s], (uint32_t)((u / a.S - 1) & 1), a.status);
-            if (!ok) break;
-          }
+        for (int i = 0; i < per_tile; i++, u++) {
+          ok = mbar_wait(&empty[s], phase, a.status);
+          if (!ok) break;
           const int b0 = c0 + i * a.ks, nblk = min(a.ks, c1 - b0);
           mbar_expect_tx(&full[s], block_tx * nblk);
           const uint32_t bar = smem_u32(&full[s]);
@@ -205,6 +214,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int b = 0; b < nblk; b++, dst += block) {
             tma_2d(dst, &mx, (b0 + b) * kKb, t, bar);
             tma_2d(dst + xbytes, &mw, (b0 + b) * kKb, c, bar);
+          }
+          if (++s == a.S) {
+            s = 0;
+            phase ^= 1;
           }
         }
       }
@@ -217,16 +230,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     // -------------------------------------------------------- MMA issuer
     if (lane == 0) {
       const uint32_t idesc = i8_idesc(128, a.Tn);
-      int u = 0, n = 0;
+      int n = 0, s = 0;
+      uint32_t phase = 0;
       for (int tile = first; tile < tiles && ok; tile += step, n++) {
         const int buf = n & 1;
         if (n >= 2) ok = mbar_wait(&tempty[buf], (uint32_t)(((n >> 1) - 1) & 1), a.status);
         if (!ok) break;
         tc_fence_after();
         const uint32_t d = tbase + (uint32_t)(buf * (tcols >> 1));
-        for (int i = 0; i < per_tile; i++, u++) {
-          const int s = u % a.S;
-          ok = mbar_wait(&full[s], (uint32_t)((u / a.S) & 1), a.status);
+        for (int i = 0; i < per_tile; i++) {
+          ok = mbar_wait(&full[s], phase, a.status);
           if (!ok) break;
           tc_fence_after();
           const int nblk = min(a.ks, c1 - c0 - i * a.ks);
@@ -238,6 +251,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               mma_i8(d, da + 2 * j, db + 2 * j, idesc, (i > 0 || b > 0 || j > 0) ? 1u : 0u);
           }
           mma_commit(&empty[s]);
+          if (++s == a.S) {
+            s = 0;
+            phase ^= 1;
+          }
         }
         if (!ok) {
           *failed = 1;
@@ -252,6 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ----------------------------------------------------------- epilogue
     const int q = warp & 3;  // TMEM lanes 32q .. 32q + 31 (this warp's quadrant)
     const int r = q * 32 + lane;
+    pdl_wait();  // the scales, and y as the previous kernel used it
     int n = 0;
     for (int tile = first; tile < tiles; tile += step, n++) {
       const int c = tile / a.nt * a.R + r, t0 = tile % a.nt * a.Tn;
@@ -283,12 +301,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (C > 1) {
     // One tile per cluster.  The stages become the exchange buffer
-    // [CTA of the cluster][its token columns][128 channels] once every CTA's
-    // MMAs have read them.
-    const int wc = (a.Tn + C - 1) / C;  // token columns each CTA finishes
+    // [CTA of the cluster][its token columns / 4][128 channels][4] once every
+    // CTA's MMAs have read them.
+    const int wc = ((a.Tn + C - 1) / C + 3) & ~3;  // token columns each CTA finishes
     const int q = warp & 3, r = q * 32 + lane;
     const int c = first / a.nt * a.R + r, t0 = first % a.nt * a.Tn;
     if (warp >= 2) {
+      pdl_wait();
       ok = mbar_wait(&tfull[0], 0, a.status);
       tc_fence_after();
     }
@@ -299,21 +318,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = ok && *reinterpret_cast<volatile int*>(failed) == 0;
       if (!ok && lane == 0)
         for (int p = 0; p < C; p++) st_peer(peer_addr(smem_u32(failed), p), 1);
-      const uint32_t at = smem_u32(stg) + (uint32_t)(rank * wc * 512 + r * 4);
+      const uint32_t at = smem_u32(stg) + (uint32_t)(rank * wc * 512 + r * 16);
       const uint32_t ta = tbase + ((uint32_t)(q * 32) << 16);
-      int owner = 0, col = 0;  // of the next column
-      uint32_t dst = peer_addr(at, 0);
       for (int j0 = 0; j0 < a.Tn; j0 += 16) {
         int acc[16];
         tmem_ld16(ta + j0, acc);
 #pragma unroll
-        for (int j = 0; j < 16; j++) {
-          st_peer(dst, acc[j]);
-          dst += 512;
-          if (++col == wc) {
-            col = 0;
-            if (++owner < C) dst = peer_addr(at, owner);
-          }
+        for (int j = 0; j < 16; j += 4) {
+          const int owner = (j0 + j) / wc, col = (j0 + j) - owner * wc;
+          st_peer4(peer_addr(at, owner) + col * 512, acc + j);
         }
       }
       tc_fence_before();
@@ -323,15 +336,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     cluster_wait();
     if (warp >= 2 && r < a.R && c < a.m) {
       const int tn = min(min(a.Tn, a.nb - t0), (rank + 1) * wc) - rank * wc;
-      const int* part = reinterpret_cast<const int*>(stg) + r;
+      const int4* part = reinterpret_cast<const int4*>(stg) + r;
       const float sw =
           *reinterpret_cast<volatile int*>(failed) ? __uint_as_float(0x7fc00000u) : a.sw[c];
       const int tt = t0 + rank * wc;
       T* y = static_cast<T*>(a.y) + (long)tt * a.ldy + c;
-      for (int j = 0; j < tn; j++) {
-        int acc = 0;
-        for (int p = 0; p < C; p++) acc += part[(p * wc + j) * 128];
-        y[(long)j * a.ldy] = from_f32<T>(scaled(acc, a.sx[tt + j], sw));
+      for (int j = 0; j < tn; j += 4) {
+        int4 acc = part[j * 32];
+        for (int p = 1; p < C; p++) {
+          const int4 v = part[(p * wc + j) * 32];
+          acc.x += v.x;
+          acc.y += v.y;
+          acc.z += v.z;
+          acc.w += v.w;
+        }
+        const int sum[4] = {acc.x, acc.y, acc.z, acc.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (j + i < tn)
+            y[(long)(j + i) * a.ldy] = from_f32<T>(scaled(sum[i], a.sx[tt + j + i], sw));
       }
     }
   }
@@ -383,11 +406,56 @@ struct Plan {
   double cost;
 };
 
+// What a device runs at once: SMs, and clusters of each size.  Clusters live
+// inside a GPC, so e.g. 33 clusters of 4 fit on 148 SMs, not 37.
+struct Slots {
+  int clusters[kMaxCluster + 1];  // [1]: SMs
+};
+
+cudaError_t device_slots(const Slots** out) {
+  static Slots table[64];
+  static std::atomic<int> known[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  static std::mutex lock;
+  if (!known[dev].load(std::memory_order_acquire)) {
+    std::lock_guard<std::mutex> hold(lock);
+    const void* kernels[3] = {(const void*)gemm_w8a8_kernel<float>,
+                              (const void*)gemm_w8a8_kernel<__nv_bfloat16>,
+                              (const void*)gemm_w8a8_kernel<__half>};
+    for (const void* k : kernels) {
+      e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
+      if (e != cudaSuccess) return e;
+    }
+    Slots s{};
+    for (int c = 1; c <= kMaxCluster; c++) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(c);
+      cfg.blockDim = dim3(kThreads);
+      cfg.dynamicSmemBytes = kSmemMax;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = (unsigned)c;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      e = cudaOccupancyMaxActiveClusters(&s.clusters[c], kernels[0], &cfg);
+      if (e != cudaSuccess) return e;
+    }
+    table[dev] = s;
+    known[dev].store(1, std::memory_order_release);
+  }
+  *out = &table[dev];
+  return cudaSuccess;
+}
+
 inline int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 
 // The tile for m x k weights and nb tokens on n_sm SMs: the cheapest of the
 // token splits and cluster sizes under the model below (cycles).
-Plan plan_tiles(int m, int chunks, int nb, int n_sm) {
+Plan plan_tiles(int m, int chunks, int nb, const Slots& at_once) {
   Plan best{0, 0, 0, 0, 0, 1e300};
   const int nt0 = ceil_div(nb, 256);
   for (int nt = nt0; nt <= nt0 * 4 && (nt == nt0 || nb >= 64 * nt); nt *= 2) {
@@ -395,7 +463,8 @@ Plan plan_tiles(int m, int chunks, int nb, int n_sm) {
     const int cols = ceil_div(nb, Tn);
     for (int C = 1; C <= kMaxCluster; C++) {
       if (C > chunks) break;
-      const int slots = n_sm / C;
+      const int slots = at_once.clusters[C];
+      if (slots < 1) continue;
       int rounds = ceil_div((long)ceil_div(m, 128) * cols, slots);
       if (C > 1 && rounds > 1) break;
       // the most tiles those rounds hold, then the rows each needs
@@ -407,7 +476,7 @@ Plan plan_tiles(int m, int chunks, int nb, int n_sm) {
       const double per_sm = (double)rounds * ceil_div(chunks, C);  // blocks of K per SM
       const double load = per_sm * (R + Tn) * kKb / 34.0;          // bytes a cycle into an SM
       const double mma = per_sm * (Tn < 32 ? 64.0 : 2.0 * Tn);
-      const double join = C > 1 ? 2000.0 + 20.0 * Tn : 0.0;
+      const double join = C > 1 ? 1500.0 + 20.0 * Tn : 0.0;
       const double cost = (load > mma ? load : mma) + join;
       if (cost < best.cost) best = Plan{R, Tn, mt, cols, C, cost};
     }
@@ -422,11 +491,11 @@ int launch(const int8_t* x, long ldx, const int8_t* w, long ldw, int k, W8A8Args
     ec_set_last_error("ec_op_gemm_w8a8: the driver has no tensor-map encoder");
     return EC_ERR_CUDA;
   }
-  int dev = 0, n_sm = 0;
-  EC_CUDA_TRY(cudaGetDevice(&dev));
-  EC_CUDA_TRY(cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, dev));
+  const Slots* slots = nullptr;
+  EC_CUDA_TRY(device_slots(&slots));
+  const int n_sm = slots->clusters[1];
   a.chunks = ceil_div(k, kKb);
-  const Plan p = plan_tiles(a.m, a.chunks, a.nb, n_sm);
+  const Plan p = plan_tiles(a.m, a.chunks, a.nb, *slots);
   a.R = p.R;
   a.Tn = p.Tn;
   a.mt = p.mt;
@@ -436,7 +505,7 @@ int launch(const int8_t* x, long ldx, const int8_t* w, long ldw, int k, W8A8Args
   const int block = (a.Tn + ((a.R + 7) & ~7)) * kKb;
   const int share = ceil_div(a.chunks, a.C);
   a.ks = 1;
-  while (a.ks < 4 && block * a.ks < 12288 && a.ks * 2 <= share) a.ks *= 2;
+  while (a.ks < 8 && block * a.ks * 2 <= 40960 && a.ks * 2 <= share) a.ks *= 2;
   // the last block's MMA reads 128 rows from its weights on
   const int slack = 128 * kKb;
   a.S = (kSmemMax - kHdr - slack) / (block * a.ks);
@@ -448,7 +517,6 @@ int launch(const int8_t* x, long ldx, const int8_t* w, long ldw, int k, W8A8Args
     return EC_ERR_CUDA;
   }
   const auto kern = gemm_w8a8_kernel<T>;
-  EC_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax));
   const int tiles = a.mt * a.nt;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.C > 1 ? tiles * a.C : tiles < n_sm ? tiles : n_sm);
@@ -457,12 +525,14 @@ int launch(const int8_t* x, long ldx, const int8_t* w, long ldw, int k, W8A8Args
   // share an SM's TMEM, so clusters cannot wait for one another's columns
   cfg.dynamicSmemBytes = smem > 120 * 1024 ? smem : 120 * 1024;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)a.C;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)a.C;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = a.C > 1 ? 2 : 1;
   EC_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, mx, mw, a));
   return EC_OK;
 }
