@@ -4,15 +4,29 @@
 //   z = l / T;  m = max z;  S = sum exp(z - m);  W = sum exp(z - m) (z - m)
 //   logprob(i) = (z_i - m) - log S;  H = log S - W / S
 //
-// One CTA per row: a pass for the maximum, one for the sums, one for each
-// alternative (the largest key below the last one's).
+// One pass over the row, which its bytes bound: every thread keeps a running
+// maximum with the sums S and W under it (rescaled when the maximum grows;
+// exponents in base 2, e = 2^((l - m) log2(e) / T)), and every warp the sorted
+// top_k of what it has seen, one entry a lane.  A warp looks for entries only
+// in chunks whose maximum passes its threshold: the larger of its own last
+// entry and of the value that the block's warps together already hold top_k
+// times.  On rows in random order few chunks do.
+//
+// A row is split over a cluster of CTAs while the rows alone do not fill the
+// SMs; the statistics and lists meet in a fixed order through (distributed)
+// shared memory, so equal inputs give equal bits.
 #include "typed.cuh"
 
 namespace ec {
 namespace {
 
 constexpr int kThr = 256;
+constexpr int kMaxWarps = 16;
 constexpr int kMaxTop = 32;
+constexpr int kMaxCl = 8;
+constexpr int kChunk = 16;  // values a lane handles at once
+constexpr int kMany = 6;    // entries at once that are merged sorted, not one by one
+constexpr float kFar = -10000.0f;  // an exponent whose power is 0
 
 typedef unsigned long long u64;
 
@@ -23,88 +37,387 @@ struct LogprobArgs {
   const int* tokens;
   float inv_t;
   int top;
+  int cl;  // CTAs of a row
   float* logprob;
   float* entropy;
   int* ids;
   float* top_lp;
 };
 
-// Larger logit first, then smaller index, in one unsigned integer: the float's
-// bits made monotonic (-0 as +0, NaN below -inf), then the inverted index.
-__device__ __forceinline__ u64 order_key(float v, int i) {
-  unsigned b = __float_as_uint(v == 0.0f ? 0.0f : v);
-  b = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-  if (v != v) b = 0;
-  return ((u64)b << 32) | (unsigned)~i;
+// ------------------------------------------------------------ the order --
+
+// A float's bits made monotonic: -0 as +0, NaN (1) below -inf, 0 for nothing.
+__device__ __forceinline__ unsigned order_of(float v) {
+  const unsigned b = __float_as_uint(__fadd_rn(v, 0.0f));
+  return v != v ? 1u : (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(unsigned o) {
+  return __uint_as_float((o & 0x80000000u) ? o ^ 0x80000000u : ~o);
+}
+// The order before one (0 has a single order, so the one of -0 is passed over)
+__device__ __forceinline__ unsigned order_below(unsigned o) {
+  return o == 0x80000000u ? o - 2 : o - 1;
+}
+// The value before an order; NaN (no bound) where that is not a number.
+__device__ __forceinline__ float just_below(unsigned o) {
+  return o > 0x007fffffu ? value_of(order_below(o)) : __uint_as_float(0x7fc00000u);
+}
+// Larger logit first, then smaller index, in one integer.
+__device__ __forceinline__ u64 key_of(float v, int i) {
+  return ((u64)order_of(v) << 32) | (unsigned)~i;
 }
 
-template <typename T, typename Op>
-__device__ T block_all(T v, T* red, Op op) {
+// c into the warp's descending list (entry of rank i in lane i, `top` of them)
+__device__ __forceinline__ void insert(u64& key, u64 c, int top, int lane) {
+  const int pos = __popc(__ballot_sync(0xffffffffu, key > c));
+  const u64 up = __shfl_up_sync(0xffffffffu, key, 1);
+  if (lane == pos && pos < top) key = c;
+  if (lane > pos && lane < top) key = up;
+}
+
+// The 32 largest of two descending lists, descending: the pairwise maxima of
+// one and the other reversed are a bitonic sequence of them.
+__device__ __forceinline__ u64 merge_lists(u64 a, u64 b_reversed, int lane) {
+  u64 x = a > b_reversed ? a : b_reversed;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  T t = red[0];
-  for (int i = 1; i < kThr / 32; i++) t = op(t, red[i]);
-  return t;
+  for (int s = 16; s > 0; s >>= 1) {
+    const u64 o = __shfl_xor_sync(0xffffffffu, x, s);
+    x = ((lane & s) == 0) == (x > o) ? x : o;
+  }
+  return x;
 }
 
-// log probability from the logit, the row's maximum and log S
-__device__ __forceinline__ float logprob_of(float v, float m, float inv_t, float logs) {
-  if (m == -INFINITY) return v == v ? -INFINITY : v;  // every token barred
-  return __fsub_rn(__fmul_rn(__fsub_rn(v, m), inv_t), logs);
+// Many new keys at once (0: none in this lane): sorted ascending, they are a
+// reversed descending list.
+__device__ __noinline__ u64 merge_keys(u64 list, u64 x, int lane) {
+#pragma unroll
+  for (int k = 2; k <= 32; k <<= 1) {
+#pragma unroll
+    for (int s = k >> 1; s > 0; s >>= 1) {
+      const u64 o = __shfl_xor_sync(0xffffffffu, x, s);
+      const bool up = (lane & k) == 0 || k == 32;
+      x = (((lane & s) == 0) == up) == (x < o) ? x : o;
+    }
+  }
+  return merge_lists(list, x, lane);
+}
+
+// the rank-th largest (from 0) of the lanes' values
+__device__ __forceinline__ unsigned nth_largest(unsigned x, int rank, int lane) {
+#pragma unroll
+  for (int k = 2; k <= 32; k <<= 1) {
+#pragma unroll
+    for (int s = k >> 1; s > 0; s >>= 1) {
+      const unsigned o = __shfl_xor_sync(0xffffffffu, x, s);
+      const bool up = (lane & k) == 0 || k == 32;
+      x = ((lane & s) == 0) == up ? min(x, o) : max(x, o);
+    }
+  }
+  return __shfl_sync(0xffffffffu, x, 31 - rank);
+}
+
+// ------------------------------------------------------- the statistics --
+
+struct Stat {
+  float m, s, w;  // maximum logit; S and W (base 2) under it
+};
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float exp2_of(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// (l - m) in units of log 2; where it is -inf or undefined, far enough below
+// for its power to be 0 (and 0 times it to be 0)
+__device__ __forceinline__ float below(float l, float m, float c2) {
+  return fmaxf(__fmul_rn(__fsub_rn(l, m), c2), kFar);
+}
+
+__device__ __forceinline__ void rescale(Stat& a, float m, float c2) {
+  const float d = below(a.m, m, c2), f = exp2_of(d);
+  a.w = __fmul_rn(f, __fmaf_rn(a.s, d, a.w));
+  a.s = __fmul_rn(f, a.s);
+  a.m = m;
+}
+
+__device__ __forceinline__ Stat join(Stat a, Stat b, float c2) {
+  const float m = max_nan(a.m, b.m);
+  rescale(a, m, c2);
+  rescale(b, m, c2);
+  return Stat{m, __fadd_rn(a.s, b.s), __fadd_rn(a.w, b.w)};
+}
+
+__device__ __forceinline__ Stat warp_join(Stat a, float c2) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const Stat b{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o),
+                 __shfl_xor_sync(0xffffffffu, a.w, o)};
+    a = join(a, b, c2);
+  }
+  return a;
+}
+
+// ------------------------------------------------------------ a warp's view --
+
+struct Warp {
+  Stat st;
+  u64 key;     // the list
+  float thr;   // only values above it can enter; NaN: any can
+  int lane, warp, warps, top, share;
+  unsigned* held;  // [warps]: order of each warp's share-th entry
+  float* stage;    // [kChunk][32] of the warp: values by number
+
+  // The threshold after the list has changed.  `share` = ceil(top / warps)
+  // entries of every warp are top entries at least, so the smallest of the
+  // warps' share-th values bounds the row's last entry from below (values
+  // equal to it may still enter, by their index).
+  __device__ __forceinline__ void update() {
+    const unsigned own = (unsigned)(__shfl_sync(0xffffffffu, key, top - 1) >> 32);
+    const unsigned mine = (unsigned)(__shfl_sync(0xffffffffu, key, share - 1) >> 32);
+    volatile unsigned* h = held;
+    if (lane == 0) h[warp] = mine;
+    __syncwarp();
+    const unsigned all = __reduce_min_sync(0xffffffffu, lane < warps ? h[lane] : 0xffffffffu);
+    const unsigned o = max(own, all ? order_below(all) : 0u);
+    thr = o ? value_of(o) : __uint_as_float(0x7fc00000u);
+  }
+
+  // kChunk values a lane; bit j of `valid` says that v[j] is one of the row's,
+  // at index i0 + index_of(j), else it is -inf.  All indices lie behind those
+  // of earlier chunks, so an equal value never displaces an earlier one, and
+  // "above the threshold" needs no index.
+  template <int kPer>
+  __device__ __forceinline__ void take(const float* v, int i0, unsigned valid, float c2) {
+    float cm = v[0];
+#pragma unroll
+    for (int j = 1; j < kChunk; j++) cm = max_nan(cm, v[j]);
+    if (!(cm <= st.m)) rescale(st, max_nan(cm, st.m), c2);
+#pragma unroll
+    for (int j = 0; j < kChunk; j++) {
+      const float d = below(v[j], st.m, c2), e = exp2_of(d);
+      st.s = __fadd_rn(st.s, e);
+      st.w = __fmaf_rn(e, d, st.w);
+    }
+    if (top && __any_sync(0xffffffffu, !(cm <= thr))) {
+      // at first: top values at least reach the top-th of the lanes' maxima
+      if (thr != thr) thr = just_below(nth_largest(order_of(cm), top - 1, lane));
+      unsigned mine = 0;  // the lane's values that can enter
+#pragma unroll
+      for (int j = 0; j < kChunk; j++) {
+        stage[j * 32 + lane] = v[j];
+        if (!(v[j] <= thr)) mine |= 1u << j;
+      }
+      mine &= valid;
+      // one of each lane's at a time, as long as any can
+#pragma unroll 1
+      while (true) {
+        u64 k = 0;
+        if (mine) {
+          const int j = __ffs(mine) - 1;
+          mine &= mine - 1;
+          const float x = stage[j * 32 + lane];
+          if (!(x <= thr)) k = key_of(x, i0 + (j / kPer) * 32 * kPer + j % kPer);
+        }
+        unsigned in = __ballot_sync(0xffffffffu, k != 0);
+        if (in) {
+          if (__popc(in) > kMany) {
+            key = merge_keys(key, k, lane);
+          } else {
+#pragma unroll 1
+            for (; in; in &= in - 1)
+              insert(key, __shfl_sync(0xffffffffu, k, __ffs(in) - 1), top, lane);
+          }
+          // within a chunk an equal value may come with a smaller index
+          const unsigned own = (unsigned)(__shfl_sync(0xffffffffu, key, top - 1) >> 32);
+          thr = fmaxf(thr, just_below(own));
+        }
+        if (!__any_sync(0xffffffffu, mine != 0)) break;
+      }
+      update();
+    }
+  }
+};
+
+// ------------------------------------------------------------------ kernel --
+
+template <typename T>
+__global__ void __launch_bounds__(kMaxWarps * 32) token_logprobs_kernel(LogprobArgs a) {
+  constexpr int kPer = 16 / (int)sizeof(T);    // values of one 16-byte load
+  constexpr int kLoads = kChunk / kPer;
+  __shared__ unsigned held[kMaxWarps];
+  __shared__ Stat stats[kMaxWarps];
+  __shared__ u64 lists[kMaxWarps][32];
+  __shared__ float stage[kMaxWarps][kChunk * 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int rank = blockIdx.x % a.cl;
+  const long row = blockIdx.x / a.cl;
+  if (threadIdx.x < kMaxWarps) held[threadIdx.x] = 0;
+  __syncthreads();
+  pdl_wait();
+  pdl_launch_dependents();
+  const T* l = static_cast<const T*>(a.l) + row * a.ld;
+  const float c2 = __fmul_rn(a.inv_t, 1.44269504f);
+  Warp w{};
+  w.st = Stat{-INFINITY, 0.0f, 0.0f};
+  w.thr = __uint_as_float(0x7fc00000u);
+  w.lane = lane;
+  w.warp = warp;
+  w.warps = warps;
+  w.top = a.top;
+  w.share = (a.top + warps - 1) / warps;
+  w.held = held;
+  w.stage = stage[warp];
+
+  // [0, head) and [head + nv * kPer, n) lie outside whole 16-byte pieces
+  const int mis = (int)((reinterpret_cast<uintptr_t>(l) & 15) / sizeof(T));
+  const int head = min(a.n, mis ? kPer - mis : 0);
+  const int nv = (a.n - head) / kPer;
+  const int v0 = (int)((long)nv * rank / a.cl), v1 = (int)((long)nv * (rank + 1) / a.cl);
+  const T* body = l + head;
+  const int first = v0 + warp * 32 * kLoads, step = warps * 32 * kLoads;
+  // the ends (fewer than kPer values each) are chunks of warp 0: before its
+  // first and behind its last
+  const bool front = rank == 0 && warp == 0 && head > 0;
+  const bool back = rank == a.cl - 1 && warp == 0 && head + nv * kPer < a.n;
+  auto fetch = [&](uint4* raw, int b) {
+#pragma unroll
+    for (int u = 0; u < kLoads; u++) {
+      const int i = b + u * 32 + lane;
+      if (i < v1) raw[u] = *reinterpret_cast<const uint4*>(body + (long)i * kPer);
+    }
+  };
+  uint4 next[kLoads];
+  fetch(next, first);
+#pragma unroll 1
+  for (int b = front ? first - step : first; b < v1 || (back && b < v1 + step); b += step) {
+    float v[kChunk];
+    unsigned valid;
+    int i0;
+    if (b >= first && b < v1) {
+      uint4 raw[kLoads];
+#pragma unroll
+      for (int u = 0; u < kLoads; u++) raw[u] = next[u];
+      fetch(next, b + step);  // under this chunk's arithmetic
+      i0 = head + (b + lane) * kPer;
+      valid = 0;
+#pragma unroll
+      for (int u = 0; u < kLoads; u++) {
+        const T* e = reinterpret_cast<const T*>(&raw[u]);
+        const bool in = b + u * 32 + lane < v1;
+        if (in) valid |= ((1u << kPer) - 1u) << (u * kPer);
+#pragma unroll
+        for (int k = 0; k < kPer; k++) v[u * kPer + k] = in ? to_f32(e[k]) : -INFINITY;
+      }
+    } else {
+      const int from = b < first ? 0 : head + nv * kPer, to = b < first ? head : a.n;
+      i0 = from + lane;
+      valid = i0 < to ? 1u : 0u;
+#pragma unroll
+      for (int j = 0; j < kChunk; j++) v[j] = -INFINITY;
+      if (valid) v[0] = to_f32(l[i0]);
+    }
+    w.take<kPer>(v, i0, valid, c2);
+  }
+
+  // the block's statistics and list
+  w.st = warp_join(w.st, c2);
+  if (lane == 0) stats[warp] = w.st;
+  lists[warp][lane] = w.key;
+  __syncthreads();
+  for (int s = 1; s < warps; s <<= 1) {
+    if (warp % (2 * s) == 0 && warp + s < warps) {
+      w.key = merge_lists(w.key, lists[warp + s][31 - lane], lane);
+      lists[warp][lane] = w.key;
+    }
+    __syncthreads();
+  }
+  if (warp == 0)
+    w.st = warp_join(lane < warps ? stats[lane] : Stat{-INFINITY, 0.0f, 0.0f}, c2);
+  if (a.cl > 1) {
+    if (warp == 0 && lane == 0) stats[0] = w.st;
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (rank == 0 && warp == 0) {
+      u64 other[kMaxCl - 1];
+      Stat st[kMaxCl - 1];
+#pragma unroll
+      for (int p = 1; p < kMaxCl; p++) {
+        if (p < a.cl) {
+          uint32_t at, sat;
+          asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(&lists[0][31 - lane])), "r"(p));
+          asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(sat) : "r"(smem_u32(&stats[0])), "r"(p));
+          asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(other[p - 1]) : "r"(at) : "memory");
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(st[p - 1].m) : "r"(sat) : "memory");
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(st[p - 1].s) : "r"(sat + 4) : "memory");
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(st[p - 1].w) : "r"(sat + 8) : "memory");
+        }
+      }
+#pragma unroll
+      for (int p = 1; p < kMaxCl; p++) {
+        if (p < a.cl) {
+          w.key = merge_lists(w.key, other[p - 1], lane);
+          w.st = join(w.st, st[p - 1], c2);
+        }
+      }
+    }
+    // the others' shared memory has been read
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+  if (rank != 0 || warp != 0) return;
+  const float nan = __uint_as_float(0x7fc00000u);
+  const Stat st = w.st;
+  const float logs = logf(st.s);
+  const bool none = st.m == -INFINITY;           // every token barred
+  const bool lost = !(st.m < INFINITY);          // a NaN or +inf
+  auto logprob = [&](float x) {
+    return lost ? nan : none ? -INFINITY : __fsub_rn(__fmul_rn(__fsub_rn(x, st.m), a.inv_t), logs);
+  };
+  if (lane == 0) {
+    if (a.entropy)
+      a.entropy[row] = lost ? nan : none ? 0.0f
+                       : __fsub_rn(logs, __fmul_rn(__fdiv_rn(st.w, st.s), 0.693147181f));
+    if (a.logprob) {
+      const int t = a.tokens[row];
+      a.logprob[row] = t == -1 ? 0.0f : t >= 0 && t < a.n ? logprob(to_f32(l[t])) : nan;
+    }
+  }
+  if (lane < a.top) {
+    a.ids[row * a.top + lane] = (int)~(unsigned)w.key;
+    a.top_lp[row * a.top + lane] = logprob(value_of((unsigned)(w.key >> 32)));
+  }
+}
+
+// CTAs of a row: as many as fill the SMs twice, each with 4096 values at least.
+inline int cluster_for(int rows, int n) {
+  int cl = 1;
+  while (cl < kMaxCl && rows * cl * 2 <= 2 * 148 && n / (cl * 2) >= 4096) cl *= 2;
+  return cl;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThr) token_logprobs_kernel(LogprobArgs a) {
-  __shared__ float red[kThr / 32];
-  __shared__ u64 redk[kThr / 32];
-  const long row = blockIdx.x;
-  const T* l = static_cast<const T*>(a.l) + row * a.ld;
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < a.n; i += kThr) {
-    const float v = to_f32(l[i]);
-    m = (v > m || v != v) ? v : m;  // a NaN stays
-    if (m != m) break;
-  }
-  m = block_all(m, red, [](float p, float q) { return (p != p || p > q) ? p : q; });
-  float s = 0.0f, w = 0.0f;
-  if (m != -INFINITY) {
-    for (int i = threadIdx.x; i < a.n; i += kThr) {
-      const float d = __fmul_rn(__fsub_rn(to_f32(l[i]), m), a.inv_t);
-      const float e = expf(d);
-      s = __fadd_rn(s, e);
-      if (e != 0.0f) w = __fmaf_rn(e, d, w);
-    }
-  }
-  auto add = [](float p, float q) { return __fadd_rn(p, q); };
-  s = block_all(s, red, add);
-  w = block_all(w, red, add);
-  const float logs = logf(s);
-  if (threadIdx.x == 0) {
-    if (a.entropy) a.entropy[row] = m == -INFINITY ? 0.0f : __fsub_rn(logs, __fdiv_rn(w, s));
-    if (a.logprob) {
-      const int t = a.tokens[row];
-      float lp = t == -1 ? 0.0f : __uint_as_float(0x7fc00000u);
-      if (t >= 0 && t < a.n) lp = logprob_of(to_f32(l[t]), m, a.inv_t, logs);
-      a.logprob[row] = lp;
-    }
-  }
-  u64 last = ~0ull;
-  for (int j = 0; j < a.top; j++) {
-    u64 best = 0;
-    for (int i = threadIdx.x; i < a.n; i += kThr) {
-      const u64 k = order_key(to_f32(l[i]), i);
-      if (k < last && k > best) best = k;
-    }
-    last = block_all(best, redk, [](u64 p, u64 q) { return p > q ? p : q; });
-    if (threadIdx.x == 0) {
-      const int i = (int)~(unsigned)last;
-      a.ids[row * a.top + j] = i;
-      a.top_lp[row * a.top + j] = logprob_of(to_f32(l[i]), m, a.inv_t, logs);
-    }
-  }
+int launch_logprobs(LogprobArgs a, int rows, cudaStream_t st) {
+  a.cl = cluster_for(rows, a.n);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)rows * a.cl);
+  cfg.blockDim = dim3(a.cl > 1 ? 512 : kThr);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)a.cl;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = a.cl > 1 ? 2 : 1;
+  EC_CUDA_TRY(cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, a));
+  return EC_OK;
 }
 
 }  // namespace
@@ -122,12 +435,9 @@ extern "C" int ec_op_token_logprobs(int type, const void* logits, int64_t ld, in
     return ec::arg_error("ec_op_token_logprobs: tokens and logprob go together; top_k 0..n with "
                          "both outputs");
   if (top_k > ec::kMaxTop) return ec::unsupported("ec_op_token_logprobs: top_k > 32");
-  const ec::LogprobArgs a{logits, (long)ld, n, tokens, 1.0f / temperature, top_k, logprob, entropy,
-                          top_ids, top_logprobs};
+  const ec::LogprobArgs a{logits, (long)ld, n, tokens, 1.0f / temperature, top_k, 1, logprob,
+                          entropy, top_ids, top_logprobs};
   return ec::with_type(type, [&](auto t) {
-    ec::token_logprobs_kernel<decltype(t)>
-        <<<rows, ec::kThr, 0, static_cast<cudaStream_t>(stream)>>>(a);
-    EC_CUDA_TRY(cudaGetLastError());
-    return EC_OK;
+    return ec::launch_logprobs<decltype(t)>(a, rows, static_cast<cudaStream_t>(stream));
   });
 }
