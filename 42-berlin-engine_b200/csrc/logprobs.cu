@@ -20,12 +20,11 @@
 namespace ec {
 namespace {
 
-constexpr int kThr = 256;
 constexpr int kMaxWarps = 16;
 constexpr int kMaxTop = 32;
 constexpr int kMaxCl = 8;
 constexpr int kChunk = 16;  // values a lane handles at once
-constexpr int kMany = 6;    // entries at once that are merged sorted, not one by one
+constexpr int kMany = 4;    // entries at once that are merged sorted, not one by one
 constexpr float kFar = -10000.0f;  // an exponent whose power is 0
 
 typedef unsigned long long u64;
@@ -67,12 +66,11 @@ __device__ __forceinline__ u64 key_of(float v, int i) {
   return ((u64)order_of(v) << 32) | (unsigned)~i;
 }
 
-// c into the warp's descending list (entry of rank i in lane i, `top` of them)
-__device__ __forceinline__ void insert(u64& key, u64 c, int top, int lane) {
+// c into the warp's descending list (the entry of rank i in lane i)
+__device__ __forceinline__ u64 insert(u64 key, u64 c, int lane) {
   const int pos = __popc(__ballot_sync(0xffffffffu, key > c));
   const u64 up = __shfl_up_sync(0xffffffffu, key, 1);
-  if (lane == pos && pos < top) key = c;
-  if (lane > pos && lane < top) key = up;
+  return lane < pos ? key : lane == pos ? c : up;
 }
 
 // The 32 largest of two descending lists, descending: the pairwise maxima of
@@ -146,19 +144,15 @@ __device__ __forceinline__ void rescale(Stat& a, float m, float c2) {
   a.m = m;
 }
 
-__device__ __forceinline__ Stat join(Stat a, Stat b, float c2) {
-  const float m = max_nan(a.m, b.m);
-  rescale(a, m, c2);
-  rescale(b, m, c2);
-  return Stat{m, __fadd_rn(a.s, b.s), __fadd_rn(a.w, b.w)};
-}
-
+// The join of the lanes' statistics, in every lane: the largest maximum (NaN if
+// any is), then the sums rescaled to it, in one tree.
 __device__ __forceinline__ Stat warp_join(Stat a, float c2) {
+  const float m = value_of(__reduce_max_sync(0xffffffffu, order_of(a.m)));
+  rescale(a, __any_sync(0xffffffffu, a.m != a.m) ? __uint_as_float(0x7fc00000u) : m, c2);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const Stat b{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o),
-                 __shfl_xor_sync(0xffffffffu, a.w, o)};
-    a = join(a, b, c2);
+    a.s = __fadd_rn(a.s, __shfl_xor_sync(0xffffffffu, a.s, o));
+    a.w = __fadd_rn(a.w, __shfl_xor_sync(0xffffffffu, a.w, o));
   }
   return a;
 }
@@ -171,12 +165,12 @@ struct Warp {
   float thr;   // only values above it can enter; NaN: any can
   int lane, warp, warps, top, share;
   unsigned* held;  // [warps]: order of each warp's share-th entry
-  float* stage;    // [kChunk][32] of the warp: values by number
 
   // The threshold after the list has changed.  `share` = ceil(top / warps)
   // entries of every warp are top entries at least, so the smallest of the
   // warps' share-th values bounds the row's last entry from below (values
-  // equal to it may still enter, by their index).
+  // equal to it may still enter, by their index).  All values to come have
+  // larger indices than the list's, so one equal to its last does not enter.
   __device__ __forceinline__ void update() {
     const unsigned own = (unsigned)(__shfl_sync(0xffffffffu, key, top - 1) >> 32);
     const unsigned mine = (unsigned)(__shfl_sync(0xffffffffu, key, share - 1) >> 32);
@@ -184,16 +178,16 @@ struct Warp {
     if (lane == 0) h[warp] = mine;
     __syncwarp();
     const unsigned all = __reduce_min_sync(0xffffffffu, lane < warps ? h[lane] : 0xffffffffu);
-    const unsigned o = max(own, all ? order_below(all) : 0u);
-    thr = o ? value_of(o) : __uint_as_float(0x7fc00000u);
+    thr = fmaxf(fmaxf(thr, just_below(all)), own > 1u ? value_of(own) : just_below(0u));
   }
 
-  // kChunk values a lane; bit j of `valid` says that v[j] is one of the row's,
-  // at index i0 + index_of(j), else it is -inf.  All indices lie behind those
-  // of earlier chunks, so an equal value never displaces an earlier one, and
-  // "above the threshold" needs no index.
-  template <int kPer>
-  __device__ __forceinline__ void take(const float* v, int i0, unsigned valid, float c2) {
+  // A chunk: kChunk values a lane, the j-th also at `kept` (this lane's, run
+  // j / kPer of 512 bytes a warp) and at index i0 + (j / kPer) * 32 * kPer +
+  // j % kPer; bit j of `valid`: it is one of the row's, else it is -inf.  All
+  // indices lie behind those of earlier chunks.
+  template <typename T, int kPer>
+  __device__ __forceinline__ void take(const float* v, const T* kept, int i0, unsigned valid,
+                                       float c2) {
     float cm = v[0];
 #pragma unroll
     for (int j = 1; j < kChunk; j++) cm = max_nan(cm, v[j]);
@@ -209,10 +203,8 @@ struct Warp {
       if (thr != thr) thr = just_below(nth_largest(order_of(cm), top - 1, lane));
       unsigned mine = 0;  // the lane's values that can enter
 #pragma unroll
-      for (int j = 0; j < kChunk; j++) {
-        stage[j * 32 + lane] = v[j];
+      for (int j = 0; j < kChunk; j++)
         if (!(v[j] <= thr)) mine |= 1u << j;
-      }
       mine &= valid;
       // one of each lane's at a time, as long as any can
 #pragma unroll 1
@@ -221,39 +213,65 @@ struct Warp {
         if (mine) {
           const int j = __ffs(mine) - 1;
           mine &= mine - 1;
-          const float x = stage[j * 32 + lane];
+          const float x = to_f32(kept[(j / kPer) * 32 * kPer + j % kPer]);
           if (!(x <= thr)) k = key_of(x, i0 + (j / kPer) * 32 * kPer + j % kPer);
         }
         unsigned in = __ballot_sync(0xffffffffu, k != 0);
-        if (in) {
-          if (__popc(in) > kMany) {
-            key = merge_keys(key, k, lane);
-          } else {
+        if (__popc(in) > kMany) {
+          key = merge_keys(key, k, lane);
+        } else {
 #pragma unroll 1
-            for (; in; in &= in - 1)
-              insert(key, __shfl_sync(0xffffffffu, k, __ffs(in) - 1), top, lane);
-          }
-          // within a chunk an equal value may come with a smaller index
-          const unsigned own = (unsigned)(__shfl_sync(0xffffffffu, key, top - 1) >> 32);
-          thr = fmaxf(thr, just_below(own));
+          for (; in; in &= in - 1)
+            key = insert(key, __shfl_sync(0xffffffffu, k, __ffs(in) - 1), lane);
         }
         if (!__any_sync(0xffffffffu, mine != 0)) break;
+        // within a chunk an equal value may come with a smaller index
+        thr = fmaxf(thr, just_below((unsigned)(__shfl_sync(0xffffffffu, key, top - 1) >> 32)));
       }
       update();
     }
   }
 };
 
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// a value of CTA `rank` of the cluster, by this CTA's address of it
+__device__ __forceinline__ u64 peer_u64(uint32_t addr, int rank) {
+  u64 v;
+  asm volatile("{ .reg .b32 a; mapa.shared::cluster.u32 a, %1, %2; ld.shared::cluster.b64 %0, [a]; }"
+               : "=l"(v) : "r"(addr), "r"(rank) : "memory");
+  return v;
+}
+__device__ __forceinline__ float peer_f32(uint32_t addr, int rank) {
+  float v;
+  asm volatile("{ .reg .b32 a; mapa.shared::cluster.u32 a, %1, %2; ld.shared::cluster.f32 %0, [a]; }"
+               : "=f"(v) : "r"(addr), "r"(rank) : "memory");
+  return v;
+}
+
+// Bytes of a chunk of 32 lanes, and chunks that a warp has under way: 8 KB of it,
+// so that some 200 KB are in flight on an SM whatever its warps work at.
+template <typename T>
+constexpr int kChunkBytes = 32 * kChunk * (int)sizeof(T);
+template <typename T>
+__host__ __device__ constexpr int ring_depth() {
+  return 6144 / kChunkBytes<T>;
+}
+
 // ------------------------------------------------------------------ kernel --
 
 template <typename T>
-__global__ void __launch_bounds__(kMaxWarps * 32) token_logprobs_kernel(LogprobArgs a) {
-  constexpr int kPer = 16 / (int)sizeof(T);    // values of one 16-byte load
+__global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(LogprobArgs a) {
+  constexpr int kPer = 16 / (int)sizeof(T);    // values of one 16-byte copy
   constexpr int kLoads = kChunk / kPer;
+  constexpr int D = ring_depth<T>();
+  extern __shared__ __align__(16) uint8_t ring_mem[];  // [warp][D][kLoads][32 lanes][16]
+  __shared__ T ends[32 * kPer];  // warp 0's: the values outside whole pieces
   __shared__ unsigned held[kMaxWarps];
   __shared__ Stat stats[kMaxWarps];
   __shared__ u64 lists[kMaxWarps][32];
-  __shared__ float stage[kMaxWarps][kChunk * 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int rank = blockIdx.x % a.cl;
   const long row = blockIdx.x / a.cl;
@@ -272,7 +290,6 @@ __global__ void __launch_bounds__(kMaxWarps * 32) token_logprobs_kernel(LogprobA
   w.top = a.top;
   w.share = (a.top + warps - 1) / warps;
   w.held = held;
-  w.stage = stage[warp];
 
   // [0, head) and [head + nv * kPer, n) lie outside whole 16-byte pieces
   const int mis = (int)((reinterpret_cast<uintptr_t>(l) & 15) / sizeof(T));
@@ -285,30 +302,36 @@ __global__ void __launch_bounds__(kMaxWarps * 32) token_logprobs_kernel(LogprobA
   // first and behind its last
   const bool front = rank == 0 && warp == 0 && head > 0;
   const bool back = rank == a.cl - 1 && warp == 0 && head + nv * kPer < a.n;
-  auto fetch = [&](uint4* raw, int b) {
+  // Every lane copies its own pieces D chunks ahead and reads back only what it
+  // copied itself, so its own wait is all the synchronisation.
+  T* ring = reinterpret_cast<T*>(ring_mem + (size_t)warp * D * kChunkBytes<T>) + lane * kPer;
+  constexpr int kSlot = kChunkBytes<T> / (int)sizeof(T);
+  auto fetch = [&](int slot, int b) {
 #pragma unroll
     for (int u = 0; u < kLoads; u++) {
       const int i = b + u * 32 + lane;
-      if (i < v1) raw[u] = *reinterpret_cast<const uint4*>(body + (long)i * kPer);
+      if (i < v1) cp_async16(ring + slot * kSlot + u * 32 * kPer, body + (long)i * kPer);
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  uint4 next[kLoads];
-  fetch(next, first);
+#pragma unroll
+  for (int d = 0; d < D; d++) fetch(d, first + d * step);
+  int slot = 0;
 #pragma unroll 1
   for (int b = front ? first - step : first; b < v1 || (back && b < v1 + step); b += step) {
     float v[kChunk];
     unsigned valid;
     int i0;
-    if (b >= first && b < v1) {
-      uint4 raw[kLoads];
-#pragma unroll
-      for (int u = 0; u < kLoads; u++) raw[u] = next[u];
-      fetch(next, b + step);  // under this chunk's arithmetic
+    T* kept = ring + slot * kSlot;
+    const bool whole = b >= first && b < v1;
+    if (whole) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
       i0 = head + (b + lane) * kPer;
       valid = 0;
 #pragma unroll
       for (int u = 0; u < kLoads; u++) {
-        const T* e = reinterpret_cast<const T*>(&raw[u]);
+        const uint4 raw = *reinterpret_cast<const uint4*>(kept + u * 32 * kPer);
+        const T* e = reinterpret_cast<const T*>(&raw);
         const bool in = b + u * 32 + lane < v1;
         if (in) valid |= ((1u << kPer) - 1u) << (u * kPer);
 #pragma unroll
@@ -316,59 +339,66 @@ __global__ void __launch_bounds__(kMaxWarps * 32) token_logprobs_kernel(LogprobA
       }
     } else {
       const int from = b < first ? 0 : head + nv * kPer, to = b < first ? head : a.n;
+      kept = ends + lane * kPer;
       i0 = from + lane;
       valid = i0 < to ? 1u : 0u;
 #pragma unroll
       for (int j = 0; j < kChunk; j++) v[j] = -INFINITY;
-      if (valid) v[0] = to_f32(l[i0]);
+      if (valid) {
+        kept[0] = l[i0];
+        v[0] = to_f32(kept[0]);
+      }
     }
-    w.take<kPer>(v, i0, valid, c2);
+    w.take<T, kPer>(v, kept, i0, valid, c2);
+    if (whole) {
+      fetch(slot, b + D * step);
+      slot = slot == D - 1 ? 0 : slot + 1;
+    }
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 
   // the block's statistics and list
   w.st = warp_join(w.st, c2);
   if (lane == 0) stats[warp] = w.st;
   lists[warp][lane] = w.key;
   __syncthreads();
-  for (int s = 1; s < warps; s <<= 1) {
-    if (warp % (2 * s) == 0 && warp + s < warps) {
-      w.key = merge_lists(w.key, lists[warp + s][31 - lane], lane);
-      lists[warp][lane] = w.key;
+  auto merge_tree = [&](int count) {
+    for (int s = 1; s < count; s <<= 1) {
+      if (warp % (2 * s) == 0 && warp + s < count) {
+        w.key = merge_lists(w.key, lists[warp + s][31 - lane], lane);
+        lists[warp][lane] = w.key;
+      }
+      __syncthreads();
     }
-    __syncthreads();
-  }
+  };
+  if (a.top) merge_tree(warps);
   if (warp == 0)
     w.st = warp_join(lane < warps ? stats[lane] : Stat{-INFINITY, 0.0f, 0.0f}, c2);
   if (a.cl > 1) {
-    if (warp == 0 && lane == 0) stats[0] = w.st;
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    if (rank == 0 && warp == 0) {
-      u64 other[kMaxCl - 1];
-      Stat st[kMaxCl - 1];
-#pragma unroll
-      for (int p = 1; p < kMaxCl; p++) {
-        if (p < a.cl) {
-          uint32_t at, sat;
-          asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(&lists[0][31 - lane])), "r"(p));
-          asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(sat) : "r"(smem_u32(&stats[0])), "r"(p));
-          asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(other[p - 1]) : "r"(at) : "memory");
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(st[p - 1].m) : "r"(sat) : "memory");
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(st[p - 1].s) : "r"(sat + 4) : "memory");
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(st[p - 1].w) : "r"(sat + 8) : "memory");
-        }
+    // the same over the cluster's CTAs, in the first
+    __shared__ u64 block_list[32];
+    __shared__ Stat block_stat;
+    if (warp == 0) {
+      block_list[lane] = w.key;
+      if (lane == 0) block_stat = w.st;
+    }
+    cluster_sync();
+    if (rank == 0) {
+      if (a.top && warp < a.cl) {
+        w.key = peer_u64(smem_u32(&block_list[lane]), warp);
+        lists[warp][lane] = w.key;
       }
-#pragma unroll
-      for (int p = 1; p < kMaxCl; p++) {
-        if (p < a.cl) {
-          w.key = merge_lists(w.key, other[p - 1], lane);
-          w.st = join(w.st, st[p - 1], c2);
+      if (warp == 0) {
+        Stat p{-INFINITY, 0.0f, 0.0f};
+        if (lane < a.cl) {
+          const uint32_t at = smem_u32(&block_stat);
+          p = Stat{peer_f32(at, lane), peer_f32(at + 4, lane), peer_f32(at + 8, lane)};
         }
+        w.st = warp_join(p, c2);
       }
     }
-    // the others' shared memory has been read
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_sync();  // the others' shared memory has been read
+    if (rank == 0 && a.top) merge_tree(a.cl);
   }
   if (rank != 0 || warp != 0) return;
   const float nan = __uint_as_float(0x7fc00000u);
@@ -404,9 +434,15 @@ inline int cluster_for(int rows, int n) {
 template <typename T>
 int launch_logprobs(LogprobArgs a, int rows, cudaStream_t st) {
   a.cl = cluster_for(rows, a.n);
+  // a chunk for every warp, up to 8 warps (16 of a cluster's CTA)
+  const int most = a.cl > 1 ? 16 : 8, chunks = (a.n / a.cl + 32 * kChunk - 1) / (32 * kChunk);
+  int warps = 1;
+  while (warps < most && warps < chunks) warps *= 2;
+  if (warps < a.cl) warps = a.cl;  // the cluster's lists meet in a warp each
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)rows * a.cl);
-  cfg.blockDim = dim3(a.cl > 1 ? 512 : kThr);
+  cfg.blockDim = dim3(warps * 32);
+  cfg.dynamicSmemBytes = (size_t)warps * ring_depth<T>() * kChunkBytes<T>;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -416,6 +452,9 @@ int launch_logprobs(LogprobArgs a, int rows, cudaStream_t st) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = a.cl > 1 ? 2 : 1;
+  EC_CUDA_TRY(cudaFuncSetAttribute(token_logprobs_kernel<T>,
+                                   cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   kMaxWarps * ring_depth<T>() * kChunkBytes<T>));
   EC_CUDA_TRY(cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, a));
   return EC_OK;
 }
