@@ -157,28 +157,61 @@ __device__ __forceinline__ Stat warp_join(Stat a, float c2) {
   return a;
 }
 
+// A lane's running statistics: the sums in two halves (paired f32
+// arithmetic), joined at the end.
+struct Running {
+  float m;
+  uint64_t s, w;
+};
+
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  return pack2(__float_as_uint(a), __float_as_uint(b));
+}
+__device__ __forceinline__ void rescale(Running& a, float m, float c2) {
+  const float d = below(a.m, m, c2), f = exp2_of(d);
+  fma2(a.w, a.s, pair_of(d, d));
+  a.w = mul2(a.w, pair_of(f, f));
+  a.s = mul2(a.s, pair_of(f, f));
+  a.m = m;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// the maximum of kChunk values (NaN if any is)
+__device__ __forceinline__ float max_of(const float* v) {
+  float m = max_nan(v[0], v[1]);
+#pragma unroll
+  for (int j = 2; j < kChunk; j += 2) m = max3_nan(m, v[j], v[j + 1]);
+  return m;
+}
+
 // ------------------------------------------------------------ a warp's view --
 
 struct Warp {
-  Stat st;
+  Running st;
   u64 key;     // the list
   float thr;   // only values above it can enter; NaN: any can
   int lane, warp, warps, top, share;
   unsigned* held;  // [warps]: order of each warp's share-th entry
 
-  // The threshold after the list has changed.  `share` = ceil(top / warps)
-  // entries of every warp are top entries at least, so the smallest of the
-  // warps' share-th values bounds the row's last entry from below (values
-  // equal to it may still enter, by their index).  All values to come have
-  // larger indices than the list's, so one equal to its last does not enter.
+  // `share` = ceil(top / warps) values of every warp are top values at least,
+  // so the smallest of the warps' share-th values bounds the row's last entry
+  // from below (values equal to it may still enter, by their index).
+  __device__ __forceinline__ unsigned all_hold() {
+    volatile unsigned* h = held;
+    return __reduce_min_sync(0xffffffffu, lane < warps ? h[lane] : 0xffffffffu);
+  }
+  // The threshold after the list has changed.  All values to come have larger
+  // indices than the list's, so one equal to its last does not enter.
   __device__ __forceinline__ void update() {
     const unsigned own = (unsigned)(__shfl_sync(0xffffffffu, key, top - 1) >> 32);
     const unsigned mine = (unsigned)(__shfl_sync(0xffffffffu, key, share - 1) >> 32);
     volatile unsigned* h = held;
-    if (lane == 0) h[warp] = mine;
+    if (lane == 0 && warp < warps && mine > h[warp]) h[warp] = mine;
     __syncwarp();
-    const unsigned all = __reduce_min_sync(0xffffffffu, lane < warps ? h[lane] : 0xffffffffu);
-    thr = fmaxf(fmaxf(thr, just_below(all)), own > 1u ? value_of(own) : just_below(0u));
+    thr = fmaxf(fmaxf(thr, just_below(all_hold())), own > 1u ? value_of(own) : just_below(0u));
   }
 
   // A chunk: kChunk values a lane, the j-th also at `kept` (this lane's, run
@@ -188,19 +221,19 @@ struct Warp {
   template <typename T, int kPer>
   __device__ __forceinline__ void take(const float* v, const T* kept, int i0, unsigned valid,
                                        float c2) {
-    float cm = v[0];
-#pragma unroll
-    for (int j = 1; j < kChunk; j++) cm = max_nan(cm, v[j]);
+    const float cm = max_of(v);
     if (!(cm <= st.m)) rescale(st, max_nan(cm, st.m), c2);
+    const uint64_t m2 = pair_of(-st.m, -st.m), c22 = pair_of(c2, c2);
 #pragma unroll
-    for (int j = 0; j < kChunk; j++) {
-      const float d = below(v[j], st.m, c2), e = exp2_of(d);
-      st.s = __fadd_rn(st.s, e);
-      st.w = __fmaf_rn(e, d, st.w);
+    for (int j = 0; j < kChunk; j += 2) {
+      // (l - m) in units of log 2; -inf and undefined ones far enough below
+      const uint64_t x = mul2(add2(pair_of(v[j], v[j + 1]), m2), c22);
+      const float d0 = fmaxf(lo_f(x), kFar), d1 = fmaxf(hi_f(x), kFar);
+      const uint64_t e = pair_of(exp2_of(d0), exp2_of(d1));
+      st.s = add2(st.s, e);
+      fma2(st.w, e, pair_of(d0, d1));
     }
     if (top && __any_sync(0xffffffffu, !(cm <= thr))) {
-      // at first: top values at least reach the top-th of the lanes' maxima
-      if (thr != thr) thr = just_below(nth_largest(order_of(cm), top - 1, lane));
       unsigned mine = 0;  // the lane's values that can enter
 #pragma unroll
       for (int j = 0; j < kChunk; j++)
@@ -282,13 +315,11 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
   const T* l = static_cast<const T*>(a.l) + row * a.ld;
   const float c2 = __fmul_rn(a.inv_t, 1.44269504f);
   Warp w{};
-  w.st = Stat{-INFINITY, 0.0f, 0.0f};
+  w.st = Running{-INFINITY, 0ull, 0ull};
   w.thr = __uint_as_float(0x7fc00000u);
   w.lane = lane;
   w.warp = warp;
-  w.warps = warps;
   w.top = a.top;
-  w.share = (a.top + warps - 1) / warps;
   w.held = held;
 
   // [0, head) and [head + nv * kPer, n) lie outside whole 16-byte pieces
@@ -316,6 +347,35 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
   };
 #pragma unroll
   for (int d = 0; d < D; d++) fetch(d, first + d * step);
+  // a chunk's values, -inf where the row has none; which are the row's
+  auto read = [&](float* v, const T* kept, int b) {
+    unsigned valid = 0;
+#pragma unroll
+    for (int u = 0; u < kLoads; u++) {
+      const uint4 raw = *reinterpret_cast<const uint4*>(kept + u * 32 * kPer);
+      const T* e = reinterpret_cast<const T*>(&raw);
+      const bool in = b + u * 32 + lane < v1;
+      if (in) valid |= ((1u << kPer) - 1u) << (u * kPer);
+#pragma unroll
+      for (int k = 0; k < kPer; k++) v[u * kPer + k] = in ? to_f32(e[k]) : -INFINITY;
+    }
+    return valid;
+  };
+  // the warps with a chunk, and the first threshold: the share-th largest of
+  // each one's lane maxima
+  w.warps = max(1, min(warps, (v1 - v0 + 32 * kLoads - 1) / (32 * kLoads)));
+  w.share = (a.top + w.warps - 1) / w.warps;
+  if (a.top) {
+    if (warp < w.warps) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
+      float v[kChunk];
+      read(v, ring, first);
+      const unsigned o = nth_largest(order_of(max_of(v)), w.share - 1, lane);
+      if (lane == 0) held[warp] = o;
+    }
+    __syncthreads();
+    w.thr = just_below(w.all_hold());
+  }
   int slot = 0;
 #pragma unroll 1
   for (int b = front ? first - step : first; b < v1 || (back && b < v1 + step); b += step) {
@@ -327,16 +387,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
     if (whole) {
       asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
       i0 = head + (b + lane) * kPer;
-      valid = 0;
-#pragma unroll
-      for (int u = 0; u < kLoads; u++) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(kept + u * 32 * kPer);
-        const T* e = reinterpret_cast<const T*>(&raw);
-        const bool in = b + u * 32 + lane < v1;
-        if (in) valid |= ((1u << kPer) - 1u) << (u * kPer);
-#pragma unroll
-        for (int k = 0; k < kPer; k++) v[u * kPer + k] = in ? to_f32(e[k]) : -INFINITY;
-      }
+      valid = read(v, kept, b);
     } else {
       const int from = b < first ? 0 : head + nv * kPer, to = b < first ? head : a.n;
       kept = ends + lane * kPer;
@@ -358,8 +409,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
   asm volatile("cp.async.wait_all;" ::: "memory");
 
   // the block's statistics and list
-  w.st = warp_join(w.st, c2);
-  if (lane == 0) stats[warp] = w.st;
+  Stat st = warp_join(Stat{w.st.m, __fadd_rn(lo_f(w.st.s), hi_f(w.st.s)),
+                           __fadd_rn(lo_f(w.st.w), hi_f(w.st.w))}, c2);
+  if (lane == 0) stats[warp] = st;
   lists[warp][lane] = w.key;
   __syncthreads();
   auto merge_tree = [&](int count) {
@@ -373,14 +425,14 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
   };
   if (a.top) merge_tree(warps);
   if (warp == 0)
-    w.st = warp_join(lane < warps ? stats[lane] : Stat{-INFINITY, 0.0f, 0.0f}, c2);
+    st = warp_join(lane < warps ? stats[lane] : Stat{-INFINITY, 0.0f, 0.0f}, c2);
   if (a.cl > 1) {
     // the same over the cluster's CTAs, in the first
     __shared__ u64 block_list[32];
     __shared__ Stat block_stat;
     if (warp == 0) {
       block_list[lane] = w.key;
-      if (lane == 0) block_stat = w.st;
+      if (lane == 0) block_stat = st;
     }
     cluster_sync();
     if (rank == 0) {
@@ -394,7 +446,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
           const uint32_t at = smem_u32(&block_stat);
           p = Stat{peer_f32(at, lane), peer_f32(at + 4, lane), peer_f32(at + 8, lane)};
         }
-        w.st = warp_join(p, c2);
+        st = warp_join(p, c2);
       }
     }
     cluster_sync();  // the others' shared memory has been read
@@ -402,7 +454,6 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
   }
   if (rank != 0 || warp != 0) return;
   const float nan = __uint_as_float(0x7fc00000u);
-  const Stat st = w.st;
   const float logs = logf(st.s);
   const bool none = st.m == -INFINITY;           // every token barred
   const bool lost = !(st.m < INFINITY);          // a NaN or +inf
