@@ -6,12 +6,16 @@
 //   y = g / (1 + exp(-g)) * u
 //   amax = max |y|;  q = rint(y * (127 / amax));  scale = amax / 127
 //
-// Bytes bound both (3 or 4 passes over a row's memory for two operations a
-// byte), so a row is read once and held on chip until its scale is known:
-// one CTA per row, kF values a thread in registers (rows_kernel), 16 bytes a
-// load, several rows' CTAs on an SM to cover one another's reductions.
-// Rows past 1024 threads' registers stay in shared memory instead
-// (wide_kernel).
+// Bytes bound both (a few operations a byte), so a row is read once and held
+// in registers, F values a thread, until its scale is known (rows_kernel).
+// CTAs walk over rows; the next row is copied into shared memory while this
+// one is reduced and stored, so loads stay under way through the reductions.
+// Aligned rows: every thread copies and reads back its own 16-byte pieces, and
+// needs no barrier for them.  Others: the 16-byte pieces inside the row at
+// their own alignment, the ends one by one, read back one element a lane.
+// Rows past 1024 threads' registers stay in shared memory as f32 (wide_kernel).
+#include <type_traits>
+
 #include "typed.cuh"
 
 namespace ec {
@@ -28,7 +32,7 @@ struct NormArgs {
   long ldx, ldr, ldh;
   const uint16_t* w;
   float eps;
-  int n;
+  int rows, n;
   int8_t* q;
   long ldq;
   float* scale;
@@ -38,7 +42,7 @@ struct SiluArgs {
   const void* g;
   const void* u;
   long ld;
-  int n;
+  int rows, n;
   int8_t* q;
   long ldq;
   float* scale;
@@ -69,15 +73,27 @@ __device__ __forceinline__ float quant_factor(unsigned amax_bits, float* scale) 
 __device__ __forceinline__ unsigned quant_byte(float y, float f) {
   return __float_as_uint(__fmaf_rn(y, f, 12582912.0f)) & 0xffu;
 }
-__device__ __forceinline__ unsigned quant4(const float* y, float f) {
-  const unsigned a = __float_as_uint(__fmaf_rn(y[0], f, 12582912.0f));
-  const unsigned b = __float_as_uint(__fmaf_rn(y[1], f, 12582912.0f));
-  const unsigned c = __float_as_uint(__fmaf_rn(y[2], f, 12582912.0f));
-  const unsigned d = __float_as_uint(__fmaf_rn(y[3], f, 12582912.0f));
-  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+__device__ __forceinline__ uint64_t both(float v) {
+  return pack2(__float_as_uint(v), __float_as_uint(v));
+}
+__device__ __forceinline__ uint64_t quant_pair(uint64_t y, uint64_t f) {
+  uint64_t t = both(12582912.0f);
+  fma2(t, y, f);
+  return t;
+}
+__device__ __forceinline__ unsigned quant4(uint64_t y01, uint64_t y23, uint64_t f) {
+  const uint64_t a = quant_pair(y01, f), b = quant_pair(y23, f);
+  return __byte_perm(__byte_perm((unsigned)a, (unsigned)(a >> 32), 0x0040),
+                     __byte_perm((unsigned)b, (unsigned)(b >> 32), 0x0040), 0x5410);
 }
 
 __device__ __forceinline__ unsigned abs_bits(float y) { return __float_as_uint(y) & 0x7fffffffu; }
+// max(m, |a|, |b|), NaN if any is
+__device__ __forceinline__ float max_abs(float m, uint64_t y) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(fabsf(lo_f(y))), "f"(fabsf(hi_f(y))));
+  return r;
+}
 
 // ---------------------------------------------------------------- row sources --
 
@@ -112,182 +128,305 @@ __device__ __forceinline__ float norm_factor(float ss, int n, float eps) {
 
 // g * u / (1 + exp(-g)): the exponential and the reciprocal are the
 // hardware's approximations (2 units each of f32 rounding), the argument's
-// rounding adds |g| units of it
-__device__ __forceinline__ float silu_mul(float g, float u) {
-  float e, s;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(g, -1.44269504f)));
-  asm("rcp.approx.f32 %0, %1;" : "=f"(s) : "f"(__fadd_rn(1.0f, e)));
-  return __fmul_rn(__fmul_rn(g, s), u);
+// rounding adds |g| units of it.  Gates below -87 give 0.
+__device__ __forceinline__ uint64_t silu_mul(uint64_t g, uint64_t u) {
+  const uint64_t x = mul2(g, both(-1.44269504f));
+  float e0, e1, s0, s1;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(lo_f(x)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(hi_f(x)));
+  const uint64_t d = add2(pack2(__float_as_uint(e0), __float_as_uint(e1)), both(1.0f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s0) : "f"(lo_f(d)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s1) : "f"(hi_f(d)));
+  return mul2(mul2(g, pack2(__float_as_uint(s0), __float_as_uint(s1))), u);
 }
 
-// N elements of T from 16 aligned bytes (N * sizeof(T) = 16) or 8, as f32
-template <typename T, int N>
-__device__ __forceinline__ void unpack(const void* p, float* v) {
-  static_assert(N * sizeof(T) == 16 || N * sizeof(T) == 8, "one load");
-  if constexpr (N * sizeof(T) == 16) {
-    // a plain load: the row may be written in place (sum_out = x)
-    const uint4 raw = *static_cast<const uint4*>(p);
-    const T* e = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-    for (int i = 0; i < N; i++) v[i] = to_f32(e[i]);
-  } else {
-    const uint2 raw = *static_cast<const uint2*>(p);
-    const T* e = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-    for (int i = 0; i < N; i++) v[i] = to_f32(e[i]);
+// two elements of T in a word (f32: in two) <-> a pair of f32
+template <typename T>
+__device__ __forceinline__ uint64_t widen(uint32_t w) {
+  if constexpr (sizeof(T) == 2) {
+    const T* e = reinterpret_cast<const T*>(&w);
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) return pack2(w << 16, w & 0xffff0000u);
+    return pack2(__float_as_uint(to_f32(e[0])), __float_as_uint(to_f32(e[1])));
   }
+  return 0;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t narrow(uint64_t v) {  // to the nearest, ties to even
+  uint32_t w;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi_f(v)), "f"(lo_f(v)));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi_f(v)), "f"(lo_f(v)));
+  return w;
+}
+// a pair rounded to T
+template <typename T>
+__device__ __forceinline__ uint64_t rounded(uint64_t v) {
+  if constexpr (sizeof(T) == 4)
+    return v;
+  else
+    return widen<T>(narrow<T>(v));
 }
 
-// A thread's part of a row: kF values.  VEC: runs of one 16-byte load (kPer
-// elements), every kPer * blockDim.x apart; else single elements, blockDim.x
-// apart, so that a warp's accesses are contiguous at any alignment.
+// A thread's part of a row: F values in pairs.  VEC: runs of one 16-byte piece
+// (kPer elements), every kPer * blockDim.x apart; else a run is one element,
+// blockDim.x apart, so that a warp's accesses are contiguous at any alignment,
+// and a pair two runs.
 template <typename T, int F, bool VEC>
 struct Part {
-  static constexpr int kPer = VEC ? 16 / (int)sizeof(T) : 1;
+  static constexpr int kPiece = 16 / (int)sizeof(T);
+  static constexpr int kPer = VEC ? kPiece : 1;
   static constexpr int kRuns = F / kPer;
   static __device__ __forceinline__ int at(int run) {
     return (run * (int)blockDim.x + (int)threadIdx.x) * kPer;
   }
-  static __device__ __forceinline__ void load(const T* row, int i, float* v) {
-    if constexpr (VEC)
-      unpack<T, kPer>(row + i, v);
-    else
-      v[0] = to_f32(row[i]);
+  // where the row starts in its buffer: at its own place within 16 bytes
+  static __device__ __forceinline__ int offset(const T* row) {
+    return VEC ? 0 : (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
   }
-  static __device__ __forceinline__ void store(T* row, int i, const float* v) {
+  // starts the copy of a row into buf (16-byte aligned, n + kPiece elements)
+  static __device__ __forceinline__ void stage(T* buf, const T* row, int n) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int run = 0; run < kRuns; run++) {
+        const int i = at(run);
+        if (i < n) cp_async16(buf + i, row + i);
+      }
+    } else {
+      const int mis = offset(row), head = min(n, mis ? kPiece - mis : 0);
+      const int pieces = (n - head) / kPiece, tail = n - head - pieces * kPiece;
+      T* dst = buf + mis;
+      for (int i = threadIdx.x; i < pieces; i += blockDim.x)
+        cp_async16(dst + head + i * kPiece, row + head + i * kPiece);
+      const int t = threadIdx.x;
+      if (t < head) dst[t] = row[t];
+      if (t >= 16 && t - 16 < tail) dst[n - 1 - (t - 16)] = row[n - 1 - (t - 16)];
+    }
+  }
+  static constexpr int kStep = VEC ? 1 : 2;         // runs handled together
+  static constexpr int kPairs = VEC ? kPer / 2 : 1;  // pairs of them
+  // the runs from `run` on -> pairs; elements behind n are `none`
+  static __device__ __forceinline__ void load(const T* row, int run, int n, uint64_t* v,
+                                              float none) {
+    const int i = at(run);
+#pragma unroll
+    for (int k = 0; k < kPairs; k++) v[k] = both(none);
+    if constexpr (VEC) {
+      if (i < n) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(row + i);
+        if constexpr (sizeof(T) == 4) {
+          v[0] = pack2(raw.x, raw.y);
+          v[1] = pack2(raw.z, raw.w);
+        } else {
+          v[0] = widen<T>(raw.x);
+          v[1] = widen<T>(raw.y);
+          v[2] = widen<T>(raw.z);
+          v[3] = widen<T>(raw.w);
+        }
+      }
+    } else {
+      const float a = i < n ? to_f32(row[i]) : none;
+      const float b = at(run + 1) < n ? to_f32(row[at(run + 1)]) : none;
+      v[0] = pack2(__float_as_uint(a), __float_as_uint(b));
+    }
+  }
+  // the norm's weights, bf16
+  static __device__ __forceinline__ void load_w(const uint16_t* w, int run, int n, uint64_t* v) {
+    const int i = at(run);
+#pragma unroll
+    for (int k = 0; k < kPairs; k++) v[k] = both(1.0f);
+    if constexpr (VEC) {
+      if (i < n) {
+        uint32_t raw[kPairs];
+        if constexpr (kPairs == 4)
+          *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(w + i);
+        else
+          *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(w + i);
+#pragma unroll
+        for (int k = 0; k < kPairs; k++) v[k] = widen<__nv_bfloat16>(raw[k]);
+      }
+    } else {
+      const float a = i < n ? bf16_to_f32(w[i]) : 1.0f;
+      const float b = at(run + 1) < n ? bf16_to_f32(w[at(run + 1)]) : 1.0f;
+      v[0] = pack2(__float_as_uint(a), __float_as_uint(b));
+    }
+  }
+  static __device__ __forceinline__ void store(T* row, int run, int n, const uint64_t* v) {
+    const int i = at(run);
     if constexpr (VEC) {
       uint4 raw;
-      T* e = reinterpret_cast<T*>(&raw);
-#pragma unroll
-      for (int k = 0; k < kPer; k++) e[k] = from_f32<T>(v[k]);
-      *reinterpret_cast<uint4*>(row + i) = raw;
+      if constexpr (sizeof(T) == 4)
+        raw = make_uint4((uint32_t)v[0], (uint32_t)(v[0] >> 32), (uint32_t)v[1],
+                         (uint32_t)(v[1] >> 32));
+      else
+        raw = make_uint4(narrow<T>(v[0]), narrow<T>(v[1]), narrow<T>(v[2]), narrow<T>(v[3]));
+      if (i < n) *reinterpret_cast<uint4*>(row + i) = raw;
     } else {
-      row[i] = from_f32<T>(v[0]);
+      if (i < n) row[i] = from_f32<T>(lo_f(v[0]));
+      if (at(run + 1) < n) row[at(run + 1)] = from_f32<T>(hi_f(v[0]));
     }
   }
   // y (F values) -> 8 bits
-  static __device__ __forceinline__ void quantise(const float* y, int n, unsigned amax_bits,
+  static __device__ __forceinline__ void quantise(const uint64_t* y, int n, unsigned amax_bits,
                                                   int8_t* q, float* scale) {
     float sc;
     const float f = quant_factor(amax_bits, &sc);
     if (threadIdx.x == 0) *scale = sc;
+    const uint64_t f2 = both(f);
 #pragma unroll
-    for (int run = 0; run < kRuns; run++) {
+    for (int run = 0; run < kRuns; run += kStep) {
       const int i = at(run);
-      if (i < n) {
-        const float* v = y + run * kPer;
-        if constexpr (!VEC) {
-          q[i] = f != 0.0f ? (int8_t)quant_byte(v[0], f) : (int8_t)0;
-        } else if constexpr (kPer == 8) {
+      const uint64_t* v = y + run / kStep * kPairs;
+      if constexpr (!VEC) {
+        const uint64_t t = f != 0.0f ? quant_pair(v[0], f2) : 0;
+        if (i < n) q[i] = (int8_t)(uint8_t)t;
+        if (at(run + 1) < n) q[at(run + 1)] = (int8_t)(uint8_t)(t >> 32);
+      } else if (i < n) {
+        if constexpr (kPer == 8)
           *reinterpret_cast<uint2*>(q + i) =
-              f != 0.0f ? make_uint2(quant4(v, f), quant4(v + 4, f)) : make_uint2(0, 0);
-        } else {
-          *reinterpret_cast<unsigned*>(q + i) = f != 0.0f ? quant4(v, f) : 0u;
-        }
+              f != 0.0f ? make_uint2(quant4(v[0], v[1], f2), quant4(v[2], v[3], f2))
+                        : make_uint2(0, 0);
+        else
+          *reinterpret_cast<unsigned*>(q + i) = f != 0.0f ? quant4(v[0], v[1], f2) : 0u;
       }
     }
   }
 };
+
+__device__ __forceinline__ void copies_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// A CTA's walk over its rows with two operands a row (the second may be
+// missing): the next row is under way while f works on this one.
+//   VEC: one buffer an operand.  A thread's pieces are its own, so it starts
+//     the next row's as soon as f has taken this row's into registers.
+//   else: two buffers, a barrier before a row is read (all threads' copies of it
+//     have landed, and all have read the buffer that is filled next).
+// f(row, a, b, next): a, b the staged row; calls next() once they are read.
+template <typename T, int F, bool VEC, typename Body>
+__device__ __forceinline__ void walk_rows(uint8_t* smem, const T* a, long lda, const T* b, long ldb,
+                                          int n, int rows, Body f) {
+  using P = Part<T, F, VEC>;
+  const int room = ((n + P::kPiece - 1) / P::kPiece + (VEC ? 0 : 1)) * P::kPiece;
+  T* buf = reinterpret_cast<T*>(smem);
+  const int step = gridDim.x;
+  int row = blockIdx.x, at = 0;
+  auto stage = [&](int r, int which) {
+    if (r < rows) {
+      T* to = buf + (long)which * 2 * room;
+      P::stage(to, a + r * lda, n);
+      if (b) P::stage(to + room, b + r * ldb, n);
+    }
+    copies_commit();
+  };
+  stage(row, 0);
+  for (; row < rows; row += step) {
+    const T* pa = a + row * lda;
+    const T* pb = b ? b + row * ldb : nullptr;
+    if constexpr (VEC) {
+      copies_wait<0>();
+      f(row, buf, buf + room, [&] { stage(row + step, 0); });
+    } else {
+      copies_wait<0>();
+      __syncthreads();
+      stage(row + step, at ^ 1);
+      const T* from = buf + (long)at * 2 * room;
+      f(row, from + P::offset(pa), from + room + (pb ? P::offset(pb) : 0), [] {});
+      at ^= 1;
+    }
+  }
+}
 
 // --------------------------------------------------------------- the kernels --
 
 template <typename T, int F, bool VEC>
 __global__ void __launch_bounds__(kMaxThr) norm_rows_kernel(NormArgs a) {
   using P = Part<T, F, VEC>;
+  extern __shared__ __align__(16) uint8_t stage_mem[];
   __shared__ float red[32];
   __shared__ unsigned redu[32];
   pdl_wait();
   pdl_launch_dependents();
-  const long row = blockIdx.x;
-  const T* x = static_cast<const T*>(a.x) + row * a.ldx;
-  const T* r = a.r ? static_cast<const T*>(a.r) + row * a.ldr : nullptr;
-  T* h = a.h ? static_cast<T*>(a.h) + row * a.ldh : nullptr;
-  float v[F];
+  walk_rows<T, F, VEC>(
+      stage_mem, static_cast<const T*>(a.x), a.ldx, static_cast<const T*>(a.r), a.ldr, a.n, a.rows,
+      [&](long row, const T* x, const T* r, auto next) {
+        uint64_t v[F / 2];
 #pragma unroll
-  for (int run = 0; run < P::kRuns; run++) {
-    const int i = P::at(run);
+        for (int run = 0; run < P::kRuns; run += P::kStep) {
+          uint64_t* vr = v + run / P::kStep * P::kPairs;
+          P::load(x, run, a.n, vr, 0.0f);
+          if (a.r) {
+            uint64_t b[P::kPairs];
+            P::load(r, run, a.n, b, 0.0f);
 #pragma unroll
-    for (int k = 0; k < P::kPer; k++) v[run * P::kPer + k] = 0.0f;
-    if (i < a.n) P::load(x, i, v + run * P::kPer);
-  }
-  if (r) {
+            for (int k = 0; k < P::kPairs; k++) vr[k] = rounded<T>(add2(vr[k], b[k]));
+          }
+        }
+        next();
+        uint64_t ss = 0;
 #pragma unroll
-    for (int run = 0; run < P::kRuns; run++) {
-      const int i = P::at(run);
-      if (i < a.n) {
-        float b[P::kPer];
-        P::load(r, i, b);
+        for (int k = 0; k < F / 2; k++) fma2(ss, v[k], v[k]);
+        if (a.h) {
+          T* h = static_cast<T*>(a.h) + row * a.ldh;
 #pragma unroll
-        for (int k = 0; k < P::kPer; k++)
-          v[run * P::kPer + k] = to_f32(from_f32<T>(__fadd_rn(v[run * P::kPer + k], b[k])));
-      }
-    }
-  }
-  float ss = 0.0f;
+          for (int run = 0; run < P::kRuns; run += P::kStep)
+            P::store(h, run, a.n, v + run / P::kStep * P::kPairs);
+        }
+        const float inv =
+            norm_factor(block_sum(__fadd_rn(lo_f(ss), hi_f(ss)), red), a.n, a.eps);
+        float m = 0.0f;
 #pragma unroll
-  for (int k = 0; k < F; k++) ss = __fmaf_rn(v[k], v[k], ss);
-  if (h) {
+        for (int run = 0; run < P::kRuns; run += P::kStep) {
+          uint64_t* vr = v + run / P::kStep * P::kPairs;
+          uint64_t w[P::kPairs];
+          if (a.w) P::load_w(a.w, run, a.n, w);
 #pragma unroll
-    for (int run = 0; run < P::kRuns; run++) {
-      const int i = P::at(run);
-      if (i < a.n) P::store(h, i, v + run * P::kPer);
-    }
-  }
-  const float inv = norm_factor(block_sum(ss, red), a.n, a.eps);
-  unsigned m = 0;
-#pragma unroll
-  for (int run = 0; run < P::kRuns; run++) {
-    const int i = P::at(run);
-    if (i < a.n) {
-      float w[P::kPer];
-#pragma unroll
-      for (int k = 0; k < P::kPer; k++) w[k] = 1.0f;
-      if (a.w) {
-        if constexpr (VEC)
-          unpack<__nv_bfloat16, P::kPer>(a.w + i, w);
-        else
-          w[0] = bf16_to_f32(a.w[i]);
-      }
-#pragma unroll
-      for (int k = 0; k < P::kPer; k++) {
-        float& y = v[run * P::kPer + k];
-        y = __fmul_rn(__fmul_rn(y, inv), w[k]);
-        m = max(m, abs_bits(y));
-      }
-    }
-  }
-  P::quantise(v, a.n, block_max(m, redu), a.q + row * a.ldq, a.scale + row);
+          for (int k = 0; k < P::kPairs; k++) {
+            vr[k] = mul2(vr[k], both(inv));
+            if (a.w) vr[k] = mul2(vr[k], w[k]);
+            m = max_abs(m, vr[k]);
+          }
+        }
+        // red and redu: the other's barrier lies between a row's reads and the
+        // next row's writes
+        P::quantise(v, a.n, block_max(abs_bits(m), redu), a.q + row * a.ldq, a.scale + row);
+      });
 }
 
 template <typename T, int F, bool VEC>
 __global__ void __launch_bounds__(kMaxThr) silu_rows_kernel(SiluArgs a) {
   using P = Part<T, F, VEC>;
-  __shared__ unsigned redu[32];
+  extern __shared__ __align__(16) uint8_t stage_mem[];
+  __shared__ unsigned redu[2][32];  // by the row's parity: one barrier a row
+  int parity = 0;
   pdl_wait();
   pdl_launch_dependents();
-  const long row = blockIdx.x;
-  const T* g = static_cast<const T*>(a.g) + row * a.ld;
-  const T* u = static_cast<const T*>(a.u) + row * a.ld;
-  float v[F];
-  unsigned m = 0;
+  walk_rows<T, F, VEC>(
+      stage_mem, static_cast<const T*>(a.g), a.ld, static_cast<const T*>(a.u), a.ld, a.n, a.rows,
+      [&](long row, const T* g, const T* u, auto next) {
+        uint64_t v[F / 2];
+        float m = 0.0f;
 #pragma unroll
-  for (int run = 0; run < P::kRuns; run++) {
-    const int i = P::at(run);
+        for (int run = 0; run < P::kRuns; run += P::kStep) {
+          uint64_t* vr = v + run / P::kStep * P::kPairs;
+          uint64_t gv[P::kPairs], uv[P::kPairs];
+          P::load(g, run, a.n, gv, 0.0f);
+          P::load(u, run, a.n, uv, 0.0f);
 #pragma unroll
-    for (int k = 0; k < P::kPer; k++) v[run * P::kPer + k] = 0.0f;
-    if (i < a.n) {
-      float gv[P::kPer], uv[P::kPer];
-      P::load(g, i, gv);
-      P::load(u, i, uv);
-#pragma unroll
-      for (int k = 0; k < P::kPer; k++) {
-        const float y = silu_mul(gv[k], uv[k]);
-        v[run * P::kPer + k] = y;
-        m = max(m, abs_bits(y));
-      }
-    }
-  }
-  P::quantise(v, a.n, block_max(m, redu), a.q + row * a.ldq, a.scale + row);
+          for (int k = 0; k < P::kPairs; k++) {
+            vr[k] = silu_mul(gv[k], uv[k]);
+            m = max_abs(m, vr[k]);
+          }
+        }
+        next();
+        P::quantise(v, a.n, block_max(abs_bits(m), redu[parity]), a.q + row * a.ldq, a.scale + row);
+        parity ^= 1;
+      });
 }
 
 // Rows of more than 32 x 1024 values: f32 in shared memory.
@@ -342,7 +481,7 @@ __global__ void __launch_bounds__(kWideThr) silu_wide_kernel(SiluArgs a) {
   const T* u = static_cast<const T*>(a.u) + row * a.ld;
   unsigned m = 0;
   for (int i = threadIdx.x; i < a.n; i += kWideThr) {
-    const float y = silu_mul(to_f32(g[i]), to_f32(u[i]));
+    const float y = lo_f(silu_mul(both(to_f32(g[i])), both(to_f32(u[i]))));
     ys[i] = y;
     m = max(m, abs_bits(y));
   }
@@ -352,12 +491,12 @@ __global__ void __launch_bounds__(kWideThr) silu_wide_kernel(SiluArgs a) {
 // ------------------------------------------------------------------- launches --
 
 template <typename Args>
-int launch(void (*kern)(Args), const Args& a, int rows, int threads, size_t smem,
+int launch(void (*kern)(Args), const Args& a, int grid, int threads, size_t smem,
            cudaStream_t st) {
   if (smem > 48 * 1024)
     EC_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(rows);
+  cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -383,36 +522,56 @@ inline bool aligned(const void* p, long ld, size_t esize, size_t to) {
   return (reinterpret_cast<uintptr_t>(p) % to) == 0 && ((size_t)ld * esize) % to == 0;
 }
 
-template <typename T>
-int norm_rows(const NormArgs& a, int rows, cudaStream_t st) {
+constexpr size_t kStageMax = 224 * 1024;  // an SM's shared memory, less the reductions'
+
+// Launches the kernel of the row's alignment and size; `wide` where a row does
+// not fit the registers, or two unaligned ones the shared memory.
+template <typename T, typename Args, typename Pick>
+int rows_launch(const Args& a, bool vec, void (*wide)(Args), Pick pick,
+                cudaStream_t st) {
   constexpr int per = 16 / (int)sizeof(T);
-  const int f = values_per_thread(rows, a.n);
-  if (a.n > f * kMaxThr) return launch(norm_wide_kernel<T>, a, rows, kWideThr, (size_t)a.n * 4, st);
+  const int f = values_per_thread(a.rows, a.n);
+  const int room = ((a.n + per - 1) / per + (vec ? 0 : 1)) * per;
+  const size_t smem = (size_t)room * sizeof(T) * 2 * (vec ? 1 : 2);
+  if (a.n > f * kMaxThr || smem > kStageMax)
+    return launch(wide, a, a.rows, kWideThr, (size_t)a.n * 4, st);
+  const int threads = threads_for(a.n, f);
+  // CTAs that an SM holds: by threads (64 registers each) and shared memory
+  int per_sm = kMaxThr / threads;
+  const int by_smem = (int)(kStageMax / (smem + 1024));
+  if (per_sm > by_smem) per_sm = by_smem;
+  if (per_sm > 16) per_sm = 16;
+  if (per_sm < 1) per_sm = 1;
+  const long at_once = 148L * per_sm;
+  return launch(pick(f, vec), a, a.rows < at_once ? a.rows : (int)at_once, threads, smem, st);
+}
+
+template <typename T>
+int norm_rows(const NormArgs& a, cudaStream_t st) {
+  constexpr int per = 16 / (int)sizeof(T);
   const bool vec = a.n % per == 0 && aligned(a.x, a.ldx, sizeof(T), 16) &&
                    (!a.r || aligned(a.r, a.ldr, sizeof(T), 16)) &&
                    (!a.h || aligned(a.h, a.ldh, sizeof(T), 16)) &&
                    (!a.w || aligned(a.w, 0, 2, 2 * per)) && aligned(a.q, a.ldq, 1, per);
-  void (*kern)(NormArgs) =
-      vec ? (f == 8 ? norm_rows_kernel<T, 8, true>
-                    : f == 16 ? norm_rows_kernel<T, 16, true> : norm_rows_kernel<T, 32, true>)
-          : (f == 8 ? norm_rows_kernel<T, 8, false>
-                    : f == 16 ? norm_rows_kernel<T, 16, false> : norm_rows_kernel<T, 32, false>);
-  return launch(kern, a, rows, threads_for(a.n, f), 0, st);
+  return rows_launch<T>(a, vec, norm_wide_kernel<T>, [](int f, bool v) {
+    return v ? (f == 8 ? norm_rows_kernel<T, 8, true>
+                       : f == 16 ? norm_rows_kernel<T, 16, true> : norm_rows_kernel<T, 32, true>)
+             : (f == 8 ? norm_rows_kernel<T, 8, false>
+                       : f == 16 ? norm_rows_kernel<T, 16, false> : norm_rows_kernel<T, 32, false>);
+  }, st);
 }
 
 template <typename T>
-int silu_rows(const SiluArgs& a, int rows, cudaStream_t st) {
+int silu_rows(const SiluArgs& a, cudaStream_t st) {
   constexpr int per = 16 / (int)sizeof(T);
-  const int f = values_per_thread(rows, a.n);
-  if (a.n > f * kMaxThr) return launch(silu_wide_kernel<T>, a, rows, kWideThr, (size_t)a.n * 4, st);
   const bool vec = a.n % per == 0 && aligned(a.g, a.ld, sizeof(T), 16) &&
                    aligned(a.u, a.ld, sizeof(T), 16) && aligned(a.q, a.ldq, 1, per);
-  void (*kern)(SiluArgs) =
-      vec ? (f == 8 ? silu_rows_kernel<T, 8, true>
-                    : f == 16 ? silu_rows_kernel<T, 16, true> : silu_rows_kernel<T, 32, true>)
-          : (f == 8 ? silu_rows_kernel<T, 8, false>
-                    : f == 16 ? silu_rows_kernel<T, 16, false> : silu_rows_kernel<T, 32, false>);
-  return launch(kern, a, rows, threads_for(a.n, f), 0, st);
+  return rows_launch<T>(a, vec, silu_wide_kernel<T>, [](int f, bool v) {
+    return v ? (f == 8 ? silu_rows_kernel<T, 8, true>
+                       : f == 16 ? silu_rows_kernel<T, 16, true> : silu_rows_kernel<T, 32, true>)
+             : (f == 8 ? silu_rows_kernel<T, 8, false>
+                       : f == 16 ? silu_rows_kernel<T, 16, false> : silu_rows_kernel<T, 32, false>);
+  }, st);
 }
 
 }  // namespace
@@ -428,10 +587,10 @@ extern "C" int ec_op_add_rmsnorm_quant(int type, const void* x, int64_t ldx, con
   if (ldx < n || ldq < n || (residual && ldr < n) || (sum_out && lds < n))
     return ec::arg_error("ec_op_add_rmsnorm_quant: a row stride is shorter than the row");
   if (n > ec::kMaxN) return ec::unsupported("ec_op_add_rmsnorm_quant: n > 57344");
-  const ec::NormArgs a{x, residual, sum_out, (long)ldx, (long)ldr, (long)lds, w, eps, n,
+  const ec::NormArgs a{x, residual, sum_out, (long)ldx, (long)ldr, (long)lds, w, eps, rows, n,
                        q, (long)ldq, scales};
   return ec::with_type(type, [&](auto t) {
-    return ec::norm_rows<decltype(t)>(a, rows, static_cast<cudaStream_t>(stream));
+    return ec::norm_rows<decltype(t)>(a, static_cast<cudaStream_t>(stream));
   });
 }
 
@@ -444,8 +603,8 @@ extern "C" int ec_op_silu_mul_quant(int type, const void* gate, const void* up, 
   if (ld < n || ldq < n)
     return ec::arg_error("ec_op_silu_mul_quant: a row stride is shorter than the row");
   if (n > ec::kMaxN) return ec::unsupported("ec_op_silu_mul_quant: n > 57344");
-  const ec::SiluArgs a{gate, up, (long)ld, n, q, (long)ldq, scales};
+  const ec::SiluArgs a{gate, up, (long)ld, rows, n, q, (long)ldq, scales};
   return ec::with_type(type, [&](auto t) {
-    return ec::silu_rows<decltype(t)>(a, rows, static_cast<cudaStream_t>(stream));
+    return ec::silu_rows<decltype(t)>(a, static_cast<cudaStream_t>(stream));
   });
 }
