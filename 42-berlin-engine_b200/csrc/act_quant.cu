@@ -11,8 +11,9 @@
 // CTAs walk over rows; the next row is copied into shared memory while this
 // one is reduced and stored, so loads stay under way through the reductions.
 // Aligned rows: every thread copies and reads back its own 16-byte pieces, and
-// needs no barrier for them.  Others: the 16-byte pieces inside the row at
-// their own alignment, the ends one by one, read back one element a lane.
+// needs no barrier for them.  Others are copied at their own alignment (the
+// ends element by element) and read back in pieces that are aligned in the
+// sum (or the first operand): two aligned reads and a shift.
 // Rows past 1024 threads' registers stay in shared memory as f32 (wide_kernel).
 #include <type_traits>
 
@@ -31,8 +32,8 @@ struct NormArgs {
   void* h;
   long ldx, ldr, ldh;
   const uint16_t* w;
-  float eps;
-  int rows, n;
+  float eps, inv_n;
+  int rows, n, buffers;
   int8_t* q;
   long ldq;
   float* scale;
@@ -42,7 +43,7 @@ struct SiluArgs {
   const void* g;
   const void* u;
   long ld;
-  int rows, n;
+  int rows, n, buffers;
   int8_t* q;
   long ldq;
   float* scale;
@@ -50,21 +51,27 @@ struct SiluArgs {
 
 // ------------------------------------------------------------ the 8-bit rule --
 
-// The row's 8-bit factor and scale from amax' bits: as unsigned integers
-// the bit patterns of |y| order like the values, infinities and NaN above
-// all finite ones, so neither is lost in the maximum.
-__device__ __forceinline__ float quant_factor(unsigned amax_bits, float* scale) {
+// 1 / x for x from 2^-110 to 2^118, within 2 units of f32 rounding: every
+// thread of a row computes it, so no exact division.
+__device__ __forceinline__ float reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// The row's 8-bit factor from amax' bits: as unsigned integers the bit
+// patterns of |y| order like the values, infinities and NaN above all finite
+// ones, so neither is lost in the maximum.  0: a row of zeros.
+__device__ __forceinline__ float quant_factor(unsigned amax_bits) {
   const float amax = __uint_as_float(amax_bits);
-  if (amax_bits >= 0x7f800000u) {
-    *scale = __uint_as_float(0x7fc00000u);
-    return 0.0f;
-  }
-  if (amax < 0x1p-100f) {
-    *scale = 1.0f;
-    return 0.0f;
-  }
-  *scale = __fdiv_rn(amax, 127.0f);
-  return __fdiv_rn(127.0f, amax);
+  const bool plain = amax_bits < 0x7f800000u && amax >= 0x1p-100f;
+  // in two powers of two, so that neither end of the range leaves f32's
+  return plain ? __fmul_rn(reciprocal(__fmul_rn(amax, 0x1p-10f)), 127.0f * 0x1p-10f) : 0.0f;
+}
+__device__ __forceinline__ float quant_scale(unsigned amax_bits) {
+  const float amax = __uint_as_float(amax_bits);
+  if (amax_bits >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
+  return amax < 0x1p-100f ? 1.0f : __fdiv_rn(amax, 127.0f);
 }
 
 // y * f rounded to the nearest integer, ties to even, in the low byte: the
@@ -97,18 +104,20 @@ __device__ __forceinline__ float max_abs(float m, uint64_t y) {
 
 // ---------------------------------------------------------------- row sources --
 
-// the statistics of a block: one barrier, then every warp joins the warps'
-// values in the same tree
-__device__ __forceinline__ float block_sum(float v, float* red) {
+// The statistics of a block: one barrier, then every warp joins the warps'
+// values in the same tree.  The sum of squares is f32 inside a 16-byte piece
+// of the row and f64 over the pieces: rounded to f32 it does not depend on how
+// many threads share the row, so a row's 8-bit values are the same in any batch.
+__device__ __forceinline__ float block_sum(double v, double* red) {
   const int lane = threadIdx.x & 31, warps = (blockDim.x + 31) >> 5;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, o));
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if (lane == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = lane < warps ? red[lane] : 0.0f;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
+  v = lane < warps ? red[lane] : 0.0;
+  for (int o = warps > 16 ? 16 : warps > 8 ? 8 : 4; o > 0; o >>= 1)
+    v += __shfl_xor_sync(0xffffffffu, v, o);
+  return __double2float_rn(__shfl_sync(0xffffffffu, v, 0));
 }
 
 __device__ __forceinline__ unsigned block_max(unsigned v, unsigned* red) {
@@ -119,11 +128,12 @@ __device__ __forceinline__ unsigned block_max(unsigned v, unsigned* red) {
   return __reduce_max_sync(0xffffffffu, lane < warps ? red[lane] : 0u);
 }
 
-// 1 / sqrt(sum / n + eps).  A sum past f32's range gives NaN, not a silent row
-// of zeros.
-__device__ __forceinline__ float norm_factor(float ss, int n, float eps) {
-  const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)n), eps)));
-  return ss == INFINITY ? __uint_as_float(0x7fc00000u) : inv;
+// 1 / sqrt(sum / n + eps), the root within 2 units.  A sum past f32's range
+// gives NaN, not a silent row of zeros.
+__device__ __forceinline__ float norm_factor(float ss, float inv_n, float eps) {
+  float r;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fmaf_rn(ss, inv_n, eps)));
+  return ss == INFINITY ? __uint_as_float(0x7fc00000u) : r;
 }
 
 // g * u / (1 + exp(-g)): the exponential and the reciprocal are the
@@ -168,126 +178,187 @@ __device__ __forceinline__ uint64_t rounded(uint64_t v) {
     return widen<T>(narrow<T>(v));
 }
 
-// A thread's part of a row: F values in pairs.  VEC: runs of one 16-byte piece
-// (kPer elements), every kPer * blockDim.x apart; else a run is one element,
-// blockDim.x apart, so that a warp's accesses are contiguous at any alignment,
-// and a pair two runs.
+// 16 bytes at any even place of shared memory: two aligned reads, moved down by
+// words and by half a word.  The place within 16 bytes is the same for all of a
+// row's pieces, so the branches are uniform.
+template <typename T>
+__device__ __forceinline__ uint4 read_shifted(const uint8_t* p) {
+  const uint32_t s = smem_u32(p) & 15u;
+  const uint4* at = reinterpret_cast<const uint4*>(p - s);
+  uint4 a = at[0];
+  if (s == 0) return a;
+  uint4 b = at[1];
+  if (s & 8) {
+    a = make_uint4(a.z, a.w, b.x, b.y);
+    b.x = b.z;
+    b.y = b.w;
+  }
+  if (s & 4) {
+    a = make_uint4(a.y, a.z, a.w, b.x);
+    b.x = b.y;
+  }
+  if (sizeof(T) == 2 && (s & 2))
+    a = make_uint4(__funnelshift_r(a.x, a.y, 16), __funnelshift_r(a.y, a.z, 16),
+                   __funnelshift_r(a.z, a.w, 16), __funnelshift_r(a.w, b.x, 16));
+  return a;
+}
+
+// A thread's part of a row: F values in pairs, in runs of one 16-byte piece
+// (kPer elements), every kPer * blockDim.x apart.  VEC: the row is whole
+// pieces.  Else its first piece starts `lead` elements before the row, and
+// what lies outside the row counts as zero.
 template <typename T, int F, bool VEC>
 struct Part {
-  static constexpr int kPiece = 16 / (int)sizeof(T);
-  static constexpr int kPer = VEC ? kPiece : 1;
+  static constexpr int kPer = 16 / (int)sizeof(T);
   static constexpr int kRuns = F / kPer;
-  static __device__ __forceinline__ int at(int run) {
-    return (run * (int)blockDim.x + (int)threadIdx.x) * kPer;
+  static constexpr int kPairs = kPer / 2;
+  static_assert(kRuns >= 1, "a piece at least");
+  int n, lead;
+
+  __device__ __forceinline__ int at(int run) const {
+    const int i = (run * (int)blockDim.x + (int)threadIdx.x) * kPer;
+    return VEC ? i : i - lead;
   }
-  // where the row starts in its buffer: at its own place within 16 bytes
-  static __device__ __forceinline__ int offset(const T* row) {
+  __device__ __forceinline__ bool inside(int i) const { return VEC || (i >= 0 && i + kPer <= n); }
+  // elements by which a row starts behind a 16-byte boundary
+  static __device__ __forceinline__ int misplaced(const T* row) {
     return VEC ? 0 : (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
   }
-  // starts the copy of a row into buf (16-byte aligned, n + kPiece elements)
-  static __device__ __forceinline__ void stage(T* buf, const T* row, int n) {
+  // bytes of a staged row: with pieces at both ends that read_shifted may touch
+  static __host__ __device__ size_t room(int n) {
+    const size_t bytes = ((size_t)n * sizeof(T) + 15) / 16 * 16;
+    return VEC ? bytes : bytes + 64;
+  }
+  // where a row's first element goes in its room
+  static __device__ __forceinline__ T* place(uint8_t* room, const T* row) {
+    return reinterpret_cast<T*>(room + (VEC ? 0 : 16)) + misplaced(row);
+  }
+  // starts the copy of a row to its place
+  __device__ __forceinline__ void stage(uint8_t* room, const T* row) const {
+    T* dst = place(room, row);
     if constexpr (VEC) {
 #pragma unroll
       for (int run = 0; run < kRuns; run++) {
         const int i = at(run);
-        if (i < n) cp_async16(buf + i, row + i);
+        if (i < n) cp_async16(dst + i, row + i);
       }
     } else {
-      const int mis = offset(row), head = min(n, mis ? kPiece - mis : 0);
-      const int pieces = (n - head) / kPiece, tail = n - head - pieces * kPiece;
-      T* dst = buf + mis;
+      const int mis = misplaced(row), head = min(n, mis ? kPer - mis : 0);
+      const int pieces = (n - head) / kPer, tail = n - head - pieces * kPer;
       for (int i = threadIdx.x; i < pieces; i += blockDim.x)
-        cp_async16(dst + head + i * kPiece, row + head + i * kPiece);
+        cp_async16(dst + head + i * kPer, row + head + i * kPer);
       const int t = threadIdx.x;
       if (t < head) dst[t] = row[t];
       if (t >= 16 && t - 16 < tail) dst[n - 1 - (t - 16)] = row[n - 1 - (t - 16)];
     }
   }
-  static constexpr int kStep = VEC ? 1 : 2;         // runs handled together
-  static constexpr int kPairs = VEC ? kPer / 2 : 1;  // pairs of them
-  // the runs from `run` on -> pairs; elements behind n are `none`
-  static __device__ __forceinline__ void load(const T* row, int run, int n, uint64_t* v,
-                                              float none) {
-    const int i = at(run);
-#pragma unroll
-    for (int k = 0; k < kPairs; k++) v[k] = both(none);
-    if constexpr (VEC) {
-      if (i < n) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(row + i);
-        if constexpr (sizeof(T) == 4) {
-          v[0] = pack2(raw.x, raw.y);
-          v[1] = pack2(raw.z, raw.w);
-        } else {
-          v[0] = widen<T>(raw.x);
-          v[1] = widen<T>(raw.y);
-          v[2] = widen<T>(raw.z);
-          v[3] = widen<T>(raw.w);
-        }
-      }
+  static __device__ __forceinline__ void spread(const uint4& raw, uint64_t* v) {
+    if constexpr (sizeof(T) == 4) {
+      v[0] = pack2(raw.x, raw.y);
+      v[1] = pack2(raw.z, raw.w);
     } else {
-      const float a = i < n ? to_f32(row[i]) : none;
-      const float b = at(run + 1) < n ? to_f32(row[at(run + 1)]) : none;
-      v[0] = pack2(__float_as_uint(a), __float_as_uint(b));
+      v[0] = widen<T>(raw.x);
+      v[1] = widen<T>(raw.y);
+      v[2] = widen<T>(raw.z);
+      v[3] = widen<T>(raw.w);
     }
   }
-  // the norm's weights, bf16
-  static __device__ __forceinline__ void load_w(const uint16_t* w, int run, int n, uint64_t* v) {
+  // the run's values of a staged row
+  __device__ __forceinline__ void load(const T* row, int run, uint64_t* v) const {
     const int i = at(run);
 #pragma unroll
-    for (int k = 0; k < kPairs; k++) v[k] = both(1.0f);
-    if constexpr (VEC) {
-      if (i < n) {
-        uint32_t raw[kPairs];
-        if constexpr (kPairs == 4)
-          *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(w + i);
-        else
-          *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(w + i);
+    for (int k = 0; k < kPairs; k++) v[k] = 0;
+    if (i >= n) return;
+    if constexpr (VEC)
+      spread(*reinterpret_cast<const uint4*>(row + i), v);
+    else
+      spread(read_shifted<T>(reinterpret_cast<const uint8_t*>(row + i)), v);
+    if (!inside(i)) clear_outside(run, v);
+  }
+  __device__ __forceinline__ void clear_outside(int run, uint64_t* v) const {
+    const int i = at(run);
 #pragma unroll
-        for (int k = 0; k < kPairs; k++) v[k] = widen<__nv_bfloat16>(raw[k]);
+    for (int k = 0; k < kPairs; k++)
+      v[k] = pack2(i + 2 * k >= 0 && i + 2 * k < n ? (uint32_t)v[k] : 0u,
+                   i + 2 * k + 1 >= 0 && i + 2 * k + 1 < n ? (uint32_t)(v[k] >> 32) : 0u);
+  }
+  // the run's weights (bf16): from memory where they lie in whole pieces, else
+  // as they were staged
+  __device__ __forceinline__ void load_w(const uint16_t* w, int run, uint64_t* v) const {
+    const int i = at(run);
+#pragma unroll
+    for (int k = 0; k < kPairs; k++) v[k] = 0;
+    if (i >= n) return;
+    uint4 raw;
+    if constexpr (VEC) {
+      if constexpr (kPairs == 4) {
+        raw = *reinterpret_cast<const uint4*>(w + i);
+      } else {
+        const uint2 two = *reinterpret_cast<const uint2*>(w + i);
+        raw = make_uint4(two.x, two.y, 0, 0);
       }
     } else {
-      const float a = i < n ? bf16_to_f32(w[i]) : 1.0f;
-      const float b = at(run + 1) < n ? bf16_to_f32(w[at(run + 1)]) : 1.0f;
-      v[0] = pack2(__float_as_uint(a), __float_as_uint(b));
+      raw = read_shifted<__nv_bfloat16>(reinterpret_cast<const uint8_t*>(w + i));
+    }
+    v[0] = widen<__nv_bfloat16>(raw.x);
+    v[1] = widen<__nv_bfloat16>(raw.y);
+    if constexpr (kPairs == 4) {
+      v[2] = widen<__nv_bfloat16>(raw.z);
+      v[3] = widen<__nv_bfloat16>(raw.w);
     }
   }
-  static __device__ __forceinline__ void store(T* row, int run, int n, const uint64_t* v) {
+  __device__ __forceinline__ void store(T* row, int run, const uint64_t* v) const {
     const int i = at(run);
-    if constexpr (VEC) {
-      uint4 raw;
-      if constexpr (sizeof(T) == 4)
-        raw = make_uint4((uint32_t)v[0], (uint32_t)(v[0] >> 32), (uint32_t)v[1],
-                         (uint32_t)(v[1] >> 32));
-      else
-        raw = make_uint4(narrow<T>(v[0]), narrow<T>(v[1]), narrow<T>(v[2]), narrow<T>(v[3]));
-      if (i < n) *reinterpret_cast<uint4*>(row + i) = raw;
+    if (i >= n) return;
+    uint32_t raw[4];
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        raw[2 * k] = (uint32_t)v[k];
+        raw[2 * k + 1] = (uint32_t)(v[k] >> 32);
+      }
     } else {
-      if (i < n) row[i] = from_f32<T>(lo_f(v[0]));
-      if (at(run + 1) < n) row[at(run + 1)] = from_f32<T>(hi_f(v[0]));
+#pragma unroll
+      for (int k = 0; k < 4; k++) raw[k] = narrow<T>(v[k]);
+    }
+    if (inside(i)) {
+      *reinterpret_cast<uint4*>(row + i) = make_uint4(raw[0], raw[1], raw[2], raw[3]);
+    } else {
+      const T* e = reinterpret_cast<const T*>(raw);
+#pragma unroll
+      for (int k = 0; k < kPer; k++)
+        if (i + k >= 0 && i + k < n) row[i + k] = e[k];
     }
   }
   // y (F values) -> 8 bits
-  static __device__ __forceinline__ void quantise(const uint64_t* y, int n, unsigned amax_bits,
-                                                  int8_t* q, float* scale) {
-    float sc;
-    const float f = quant_factor(amax_bits, &sc);
-    if (threadIdx.x == 0) *scale = sc;
+  __device__ __forceinline__ void quantise(const uint64_t* y, unsigned amax_bits, int8_t* q,
+                                           float* scale) const {
+    const float f = quant_factor(amax_bits);
+    if (threadIdx.x == 0) *scale = quant_scale(amax_bits);
     const uint64_t f2 = both(f);
+    // where the bytes of a piece can be stored together
+    const bool together = VEC || ((reinterpret_cast<uintptr_t>(q) - lead) & (kPer - 1)) == 0;
 #pragma unroll
-    for (int run = 0; run < kRuns; run += kStep) {
+    for (int run = 0; run < kRuns; run++) {
       const int i = at(run);
-      const uint64_t* v = y + run / kStep * kPairs;
-      if constexpr (!VEC) {
-        const uint64_t t = f != 0.0f ? quant_pair(v[0], f2) : 0;
-        if (i < n) q[i] = (int8_t)(uint8_t)t;
-        if (at(run + 1) < n) q[at(run + 1)] = (int8_t)(uint8_t)(t >> 32);
-      } else if (i < n) {
+      if (i >= n) continue;
+      const uint64_t* v = y + run * kPairs;
+      uint32_t b[kPer / 4];
+#pragma unroll
+      for (int k = 0; k < kPer / 4; k++)
+        b[k] = f != 0.0f ? quant4(v[2 * k], v[2 * k + 1], f2) : 0u;
+      if (together && inside(i)) {
         if constexpr (kPer == 8)
-          *reinterpret_cast<uint2*>(q + i) =
-              f != 0.0f ? make_uint2(quant4(v[0], v[1], f2), quant4(v[2], v[3], f2))
-                        : make_uint2(0, 0);
+          *reinterpret_cast<uint2*>(q + i) = make_uint2(b[0], b[1]);
         else
-          *reinterpret_cast<unsigned*>(q + i) = f != 0.0f ? quant4(v[0], v[1], f2) : 0u;
+          *reinterpret_cast<unsigned*>(q + i) = b[0];
+      } else if (inside(i)) {
+#pragma unroll
+        for (int k = 0; k < kPer; k++) q[i + k] = (int8_t)(uint8_t)(b[k / 4] >> (8 * (k & 3)));
+      } else {
+#pragma unroll
+        for (int k = 0; k < kPer; k++)
+          if (i + k >= 0 && i + k < n) q[i + k] = (int8_t)(uint8_t)(b[k / 4] >> (8 * (k & 3)));
       }
     }
   }
@@ -305,39 +376,41 @@ __device__ __forceinline__ void copies_wait() {
 // missing): the next row is under way while f works on this one.
 //   VEC: one buffer an operand.  A thread's pieces are its own, so it starts
 //     the next row's as soon as f has taken this row's into registers.
-//   else: two buffers, a barrier before a row is read (all threads' copies of it
-//     have landed, and all have read the buffer that is filled next).
+//   else: two buffers (or one, filled again after f's barriers, where two do not
+//     fit), and a barrier before a row is read: all threads' copies of it have
+//     landed, and all have read the buffer that is filled next.
 // f(row, a, b, next): a, b the staged row; calls next() once they are read.
 template <typename T, int F, bool VEC, typename Body>
 __device__ __forceinline__ void walk_rows(uint8_t* smem, const T* a, long lda, const T* b, long ldb,
-                                          int n, int rows, Body f) {
+                                          int n, int rows, int buffers, Body f) {
   using P = Part<T, F, VEC>;
-  const int room = ((n + P::kPiece - 1) / P::kPiece + (VEC ? 0 : 1)) * P::kPiece;
-  T* buf = reinterpret_cast<T*>(smem);
+  const P part{n, 0};
+  const size_t room = P::room(n);
   const int step = gridDim.x;
   int row = blockIdx.x, at = 0;
   auto stage = [&](int r, int which) {
     if (r < rows) {
-      T* to = buf + (long)which * 2 * room;
-      P::stage(to, a + r * lda, n);
-      if (b) P::stage(to + room, b + r * ldb, n);
+      part.stage(smem + which * 2 * room, a + r * lda);
+      if (b) part.stage(smem + (which * 2 + 1) * room, b + r * ldb);
     }
     copies_commit();
   };
   stage(row, 0);
   for (; row < rows; row += step) {
-    const T* pa = a + row * lda;
-    const T* pb = b ? b + row * ldb : nullptr;
+    uint8_t* from = smem + at * 2 * room;
+    const T* pa = P::place(from, a + row * lda);
+    const T* pb = b ? P::place(from + room, b + row * ldb) : nullptr;
+    copies_wait<0>();
     if constexpr (VEC) {
-      copies_wait<0>();
-      f(row, buf, buf + room, [&] { stage(row + step, 0); });
+      f(row, pa, pb, [&] { stage(row + step, 0); });
     } else {
-      copies_wait<0>();
       __syncthreads();
-      stage(row + step, at ^ 1);
-      const T* from = buf + (long)at * 2 * room;
-      f(row, from + P::offset(pa), from + room + (pb ? P::offset(pb) : 0), [] {});
-      at ^= 1;
+      if (buffers == 2) {
+        at ^= 1;
+        stage(row + step, at);
+      }
+      f(row, pa, pb, [] {});
+      if (buffers == 1) stage(row + step, 0);
     }
   }
 }
@@ -348,53 +421,73 @@ template <typename T, int F, bool VEC>
 __global__ void __launch_bounds__(kMaxThr) norm_rows_kernel(NormArgs a) {
   using P = Part<T, F, VEC>;
   extern __shared__ __align__(16) uint8_t stage_mem[];
-  __shared__ float red[32];
+  __shared__ double red[32];
   __shared__ unsigned redu[32];
   pdl_wait();
   pdl_launch_dependents();
+  uint8_t* rows_mem = stage_mem;
+  const uint16_t* w = a.w;
+  if constexpr (!VEC) {
+    // the weights too are read shifted: staged once, before any row's barrier
+    using W = Part<__nv_bfloat16, 8, false>;
+    if (a.w) {
+      const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(a.w);
+      W{a.n, 0}.stage(stage_mem, src);
+      w = reinterpret_cast<const uint16_t*>(W::place(stage_mem, src));
+      rows_mem += W::room(a.n);
+    }
+  }
   walk_rows<T, F, VEC>(
-      stage_mem, static_cast<const T*>(a.x), a.ldx, static_cast<const T*>(a.r), a.ldr, a.n, a.rows,
-      [&](long row, const T* x, const T* r, auto next) {
+      rows_mem, static_cast<const T*>(a.x), a.ldx, static_cast<const T*>(a.r), a.ldr, a.n, a.rows,
+      a.buffers, [&](long row, const T* x, const T* r, auto next) {
+        T* h = a.h ? static_cast<T*>(a.h) + row * a.ldh : nullptr;
+        const P part{a.n, P::misplaced(h ? h : static_cast<const T*>(a.x) + row * a.ldx)};
         uint64_t v[F / 2];
 #pragma unroll
-        for (int run = 0; run < P::kRuns; run += P::kStep) {
-          uint64_t* vr = v + run / P::kStep * P::kPairs;
-          P::load(x, run, a.n, vr, 0.0f);
-          if (a.r) {
+        for (int run = 0; run < P::kRuns; run++) {
+          uint64_t* vr = v + run * P::kPairs;
+          part.load(x, run, vr);
+          if (r) {
             uint64_t b[P::kPairs];
-            P::load(r, run, a.n, b, 0.0f);
+            part.load(r, run, b);
 #pragma unroll
             for (int k = 0; k < P::kPairs; k++) vr[k] = rounded<T>(add2(vr[k], b[k]));
           }
         }
         next();
-        uint64_t ss = 0;
+        double ss = 0.0;
 #pragma unroll
-        for (int k = 0; k < F / 2; k++) fma2(ss, v[k], v[k]);
-        if (a.h) {
-          T* h = static_cast<T*>(a.h) + row * a.ldh;
+        for (int run = 0; run < P::kRuns; run++) {
+          const uint64_t* vr = v + run * P::kPairs;
+          uint64_t s = mul2(vr[0], vr[0]);
 #pragma unroll
-          for (int run = 0; run < P::kRuns; run += P::kStep)
-            P::store(h, run, a.n, v + run / P::kStep * P::kPairs);
+          for (int k = 1; k < P::kPairs; k++) fma2(s, vr[k], vr[k]);
+          ss += (double)__fadd_rn(lo_f(s), hi_f(s));
         }
-        const float inv =
-            norm_factor(block_sum(__fadd_rn(lo_f(ss), hi_f(ss)), red), a.n, a.eps);
+        if (h) {
+#pragma unroll
+          for (int run = 0; run < P::kRuns; run++) part.store(h, run, v + run * P::kPairs);
+        }
+        const float inv = norm_factor(block_sum(ss, red), a.inv_n, a.eps);
         float m = 0.0f;
 #pragma unroll
-        for (int run = 0; run < P::kRuns; run += P::kStep) {
-          uint64_t* vr = v + run / P::kStep * P::kPairs;
-          uint64_t w[P::kPairs];
-          if (a.w) P::load_w(a.w, run, a.n, w);
+        for (int run = 0; run < P::kRuns; run++) {
+          uint64_t* vr = v + run * P::kPairs;
+          uint64_t wv[P::kPairs];
+          if (w) part.load_w(w, run, wv);
 #pragma unroll
           for (int k = 0; k < P::kPairs; k++) {
             vr[k] = mul2(vr[k], both(inv));
-            if (a.w) vr[k] = mul2(vr[k], w[k]);
-            m = max_abs(m, vr[k]);
+            if (w) vr[k] = mul2(vr[k], wv[k]);
           }
+          // what a piece holds outside the row: the weights there are not its
+          if (!part.inside(part.at(run))) part.clear_outside(run, vr);
+#pragma unroll
+          for (int k = 0; k < P::kPairs; k++) m = max_abs(m, vr[k]);
         }
         // red and redu: the other's barrier lies between a row's reads and the
         // next row's writes
-        P::quantise(v, a.n, block_max(abs_bits(m), redu), a.q + row * a.ldq, a.scale + row);
+        part.quantise(v, block_max(abs_bits(m), redu), a.q + row * a.ldq, a.scale + row);
       });
 }
 
@@ -408,15 +501,16 @@ __global__ void __launch_bounds__(kMaxThr) silu_rows_kernel(SiluArgs a) {
   pdl_launch_dependents();
   walk_rows<T, F, VEC>(
       stage_mem, static_cast<const T*>(a.g), a.ld, static_cast<const T*>(a.u), a.ld, a.n, a.rows,
-      [&](long row, const T* g, const T* u, auto next) {
+      a.buffers, [&](long row, const T* g, const T* u, auto next) {
+        const P part{a.n, P::misplaced(static_cast<const T*>(a.g) + row * a.ld)};
         uint64_t v[F / 2];
         float m = 0.0f;
 #pragma unroll
-        for (int run = 0; run < P::kRuns; run += P::kStep) {
-          uint64_t* vr = v + run / P::kStep * P::kPairs;
+        for (int run = 0; run < P::kRuns; run++) {
+          uint64_t* vr = v + run * P::kPairs;
           uint64_t gv[P::kPairs], uv[P::kPairs];
-          P::load(g, run, a.n, gv, 0.0f);
-          P::load(u, run, a.n, uv, 0.0f);
+          part.load(g, run, gv);
+          part.load(u, run, uv);
 #pragma unroll
           for (int k = 0; k < P::kPairs; k++) {
             vr[k] = silu_mul(gv[k], uv[k]);
@@ -424,7 +518,7 @@ __global__ void __launch_bounds__(kMaxThr) silu_rows_kernel(SiluArgs a) {
           }
         }
         next();
-        P::quantise(v, a.n, block_max(abs_bits(m), redu[parity]), a.q + row * a.ldq, a.scale + row);
+        part.quantise(v, block_max(abs_bits(m), redu[parity]), a.q + row * a.ldq, a.scale + row);
         parity ^= 1;
       });
 }
@@ -432,17 +526,16 @@ __global__ void __launch_bounds__(kMaxThr) silu_rows_kernel(SiluArgs a) {
 // Rows of more than 32 x 1024 values: f32 in shared memory.
 __device__ void quantise_wide(const float* ys, int n, unsigned amax_bits, int8_t* q,
                               float* scale) {
-  float sc;
-  const float f = quant_factor(amax_bits, &sc);
+  const float f = quant_factor(amax_bits);
   for (int i = threadIdx.x; i < n; i += kWideThr)
     q[i] = f != 0.0f ? (int8_t)quant_byte(ys[i], f) : (int8_t)0;
-  if (threadIdx.x == 0) *scale = sc;
+  if (threadIdx.x == 0) *scale = quant_scale(amax_bits);
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kWideThr) norm_wide_kernel(NormArgs a) {
   extern __shared__ __align__(16) float ys[];
-  __shared__ float red[32];
+  __shared__ double red[32];
   __shared__ unsigned redu[32];
   pdl_wait();
   pdl_launch_dependents();
@@ -450,16 +543,16 @@ __global__ void __launch_bounds__(kWideThr) norm_wide_kernel(NormArgs a) {
   const T* x = static_cast<const T*>(a.x) + row * a.ldx;
   const T* r = a.r ? static_cast<const T*>(a.r) + row * a.ldr : nullptr;
   T* h = a.h ? static_cast<T*>(a.h) + row * a.ldh : nullptr;
-  float ss = 0.0f;
+  double ss = 0.0;
   for (int i = threadIdx.x; i < a.n; i += kWideThr) {
     T v = x[i];
     if (r) v = from_f32<T>(__fadd_rn(to_f32(v), to_f32(r[i])));
     if (h) h[i] = v;
     const float f = to_f32(v);
     ys[i] = f;
-    ss = __fmaf_rn(f, f, ss);
+    ss += (double)__fmul_rn(f, f);
   }
-  const float inv = norm_factor(block_sum(ss, red), a.n, a.eps);
+  const float inv = norm_factor(block_sum(ss, red), a.inv_n, a.eps);
   unsigned m = 0;
   for (int i = threadIdx.x; i < a.n; i += kWideThr) {  // the elements it stored itself
     float y = __fmul_rn(ys[i], inv);
@@ -509,41 +602,39 @@ int launch(void (*kern)(Args), const Args& a, int grid, int threads, size_t smem
   return EC_OK;
 }
 
-// Values a thread holds: 8 while the rows are few (more threads a row hide the
-// latency), else 16 or 32.
-inline int values_per_thread(int rows, int n) {
-  int f = rows < 148 * 2 ? 8 : 16;
-  while (f < 32 && n > f * kMaxThr) f *= 2;
-  return f;
-}
-inline int threads_for(int n, int f) { return ((n + f - 1) / f + 31) / 32 * 32; }
-
 inline bool aligned(const void* p, long ld, size_t esize, size_t to) {
   return (reinterpret_cast<uintptr_t>(p) % to) == 0 && ((size_t)ld * esize) % to == 0;
 }
 
 constexpr size_t kStageMax = 224 * 1024;  // an SM's shared memory, less the reductions'
 
-// Launches the kernel of the row's alignment and size; `wide` where a row does
-// not fit the registers, or two unaligned ones the shared memory.
+// How the rows are handled: values a thread, and rows a CTA.
+struct Shape {
+  int f;
+  int rows_per_cta;  // where several CTAs share an SM
+};
+
+// Launches the kernel of the row's alignment and size; `wide` where a row fits
+// neither the registers nor the shared memory.  `extra`: shared memory for the
+// weights.
 template <typename T, typename Args, typename Pick>
-int rows_launch(const Args& a, bool vec, void (*wide)(Args), Pick pick,
+int rows_launch(Args a, bool vec, Shape s, size_t extra, void (*wide)(Args), Pick pick,
                 cudaStream_t st) {
   constexpr int per = 16 / (int)sizeof(T);
-  const int f = values_per_thread(a.rows, a.n);
-  const int room = ((a.n + per - 1) / per + (vec ? 0 : 1)) * per;
-  const size_t smem = (size_t)room * sizeof(T) * 2 * (vec ? 1 : 2);
-  if (a.n > f * kMaxThr || smem > kStageMax)
+  const int span = vec ? a.n : a.n + per - 1;  // with the lead
+  while (s.f < 32 && span > s.f * kMaxThr) s.f *= 2;
+  const size_t pair = 2 * (vec ? Part<T, 8, true>::room(a.n) : Part<T, 8, false>::room(a.n));
+  a.buffers = !vec && extra + 2 * pair <= kStageMax ? 2 : 1;
+  const size_t smem = extra + a.buffers * pair;
+  if (span > s.f * kMaxThr || smem > kStageMax)
     return launch(wide, a, a.rows, kWideThr, (size_t)a.n * 4, st);
-  const int threads = threads_for(a.n, f);
-  // CTAs that an SM holds: by threads (64 registers each) and shared memory
-  int per_sm = kMaxThr / threads;
-  const int by_smem = (int)(kStageMax / (smem + 1024));
-  if (per_sm > by_smem) per_sm = by_smem;
-  if (per_sm > 16) per_sm = 16;
-  if (per_sm < 1) per_sm = 1;
-  const long at_once = 148L * per_sm;
-  return launch(pick(f, vec), a, a.rows < at_once ? a.rows : (int)at_once, threads, smem, st);
+  const int threads = ((span + s.f - 1) / s.f + 31) / 32 * 32;
+  // CTAs that an SM holds: by threads (64 registers each) and shared memory.
+  // Alone on its SM a CTA walks all its rows; else a few, so that the SMs'
+  // different speeds even out.
+  const bool alone = kMaxThr / threads < 2 || kStageMax / (smem + 1024) < 2;
+  const int grid = alone ? (a.rows < 148 ? a.rows : 148) : (a.rows + s.rows_per_cta - 1) / s.rows_per_cta;
+  return launch(pick(s.f, vec), a, grid, threads, smem, st);
 }
 
 template <typename T>
@@ -553,7 +644,10 @@ int norm_rows(const NormArgs& a, cudaStream_t st) {
                    (!a.r || aligned(a.r, a.ldr, sizeof(T), 16)) &&
                    (!a.h || aligned(a.h, a.ldh, sizeof(T), 16)) &&
                    (!a.w || aligned(a.w, 0, 2, 2 * per)) && aligned(a.q, a.ldq, 1, per);
-  return rows_launch<T>(a, vec, norm_wide_kernel<T>, [](int f, bool v) {
+  const bool few = a.rows < 148 * 2;
+  const Shape s{few ? 8 : 16, few || sizeof(T) == 4 ? 1 : 4};
+  const size_t extra = !vec && a.w ? Part<__nv_bfloat16, 8, false>::room(a.n) : 0;
+  return rows_launch<T>(a, vec, s, extra, norm_wide_kernel<T>, [](int f, bool v) {
     return v ? (f == 8 ? norm_rows_kernel<T, 8, true>
                        : f == 16 ? norm_rows_kernel<T, 16, true> : norm_rows_kernel<T, 32, true>)
              : (f == 8 ? norm_rows_kernel<T, 8, false>
@@ -566,7 +660,9 @@ int silu_rows(const SiluArgs& a, cudaStream_t st) {
   constexpr int per = 16 / (int)sizeof(T);
   const bool vec = a.n % per == 0 && aligned(a.g, a.ld, sizeof(T), 16) &&
                    aligned(a.u, a.ld, sizeof(T), 16) && aligned(a.q, a.ldq, 1, per);
-  return rows_launch<T>(a, vec, silu_wide_kernel<T>, [](int f, bool v) {
+  const bool few = a.rows < 148 * 2;
+  const Shape s{few ? 8 : sizeof(T) == 2 && a.n >= 4096 ? 32 : 16, few || sizeof(T) == 4 ? 1 : 2};
+  return rows_launch<T>(a, vec, s, 0, silu_wide_kernel<T>, [](int f, bool v) {
     return v ? (f == 8 ? silu_rows_kernel<T, 8, true>
                        : f == 16 ? silu_rows_kernel<T, 16, true> : silu_rows_kernel<T, 32, true>)
              : (f == 8 ? silu_rows_kernel<T, 8, false>
@@ -587,7 +683,7 @@ extern "C" int ec_op_add_rmsnorm_quant(int type, const void* x, int64_t ldx, con
   if (ldx < n || ldq < n || (residual && ldr < n) || (sum_out && lds < n))
     return ec::arg_error("ec_op_add_rmsnorm_quant: a row stride is shorter than the row");
   if (n > ec::kMaxN) return ec::unsupported("ec_op_add_rmsnorm_quant: n > 57344");
-  const ec::NormArgs a{x, residual, sum_out, (long)ldx, (long)ldr, (long)lds, w, eps, rows, n,
+  const ec::NormArgs a{x, residual, sum_out, (long)ldx, (long)ldr, (long)lds, w, eps, 1.0f / (float)n, rows, n, 1,
                        q, (long)ldq, scales};
   return ec::with_type(type, [&](auto t) {
     return ec::norm_rows<decltype(t)>(a, static_cast<cudaStream_t>(stream));
@@ -603,7 +699,7 @@ extern "C" int ec_op_silu_mul_quant(int type, const void* gate, const void* up, 
   if (ld < n || ldq < n)
     return ec::arg_error("ec_op_silu_mul_quant: a row stride is shorter than the row");
   if (n > ec::kMaxN) return ec::unsupported("ec_op_silu_mul_quant: n > 57344");
-  const ec::SiluArgs a{gate, up, (long)ld, rows, n, q, (long)ldq, scales};
+  const ec::SiluArgs a{gate, up, (long)ld, rows, n, 1, q, (long)ldq, scales};
   return ec::with_type(type, [&](auto t) {
     return ec::silu_rows<decltype(t)>(a, static_cast<cudaStream_t>(stream));
   });
