@@ -178,10 +178,9 @@ __device__ __forceinline__ uint64_t rounded(uint64_t v) {
     return widen<T>(narrow<T>(v));
 }
 
-// 16 bytes at any even place of shared memory: two aligned reads, moved down by
-// words and by half a word.  The place within 16 bytes is the same for all of a
-// row's pieces, so the branches are uniform.
-template <typename T>
+// 16 bytes at any place of shared memory: two aligned reads, moved down by words
+// and by the rest.  The place within 16 bytes is the same for all of a row's
+// pieces, so the branches are uniform.
 __device__ __forceinline__ uint4 read_shifted(const uint8_t* p) {
   const uint32_t s = smem_u32(p) & 15u;
   const uint4* at = reinterpret_cast<const uint4*>(p - s);
@@ -197,9 +196,9 @@ __device__ __forceinline__ uint4 read_shifted(const uint8_t* p) {
     a = make_uint4(a.y, a.z, a.w, b.x);
     b.x = b.y;
   }
-  if (sizeof(T) == 2 && (s & 2))
-    a = make_uint4(__funnelshift_r(a.x, a.y, 16), __funnelshift_r(a.y, a.z, 16),
-                   __funnelshift_r(a.z, a.w, 16), __funnelshift_r(a.w, b.x, 16));
+  if (const uint32_t bits = (s & 3) * 8)
+    a = make_uint4(__funnelshift_r(a.x, a.y, bits), __funnelshift_r(a.y, a.z, bits),
+                   __funnelshift_r(a.z, a.w, bits), __funnelshift_r(a.w, b.x, bits));
   return a;
 }
 
@@ -233,8 +232,8 @@ struct Part {
   static __device__ __forceinline__ T* place(uint8_t* room, const T* row) {
     return reinterpret_cast<T*>(room + (VEC ? 0 : 16)) + misplaced(row);
   }
-  // starts the copy of a row to its place
-  __device__ __forceinline__ void stage(uint8_t* room, const T* row) const {
+  // starts the copy of a row to its place (the ends by warp `ends`)
+  __device__ __forceinline__ void stage(uint8_t* room, const T* row, int ends) const {
     T* dst = place(room, row);
     if constexpr (VEC) {
 #pragma unroll
@@ -247,9 +246,11 @@ struct Part {
       const int pieces = (n - head) / kPer, tail = n - head - pieces * kPer;
       for (int i = threadIdx.x; i < pieces; i += blockDim.x)
         cp_async16(dst + head + i * kPer, row + head + i * kPer);
-      const int t = threadIdx.x;
-      if (t < head) dst[t] = row[t];
-      if (t >= 16 && t - 16 < tail) dst[n - 1 - (t - 16)] = row[n - 1 - (t - 16)];
+      const int t = (int)threadIdx.x - ends % ((int)blockDim.x / 32) * 32;
+      if ((t >= 0 && t < head) || (t >= 8 && t - 8 < tail)) {
+        const int i = t < 8 ? t : n - 1 - (t - 8);
+        dst[i] = row[i];
+      }
     }
   }
   static __device__ __forceinline__ void spread(const uint4& raw, uint64_t* v) {
@@ -272,7 +273,7 @@ struct Part {
     if constexpr (VEC)
       spread(*reinterpret_cast<const uint4*>(row + i), v);
     else
-      spread(read_shifted<T>(reinterpret_cast<const uint8_t*>(row + i)), v);
+      spread(read_shifted(reinterpret_cast<const uint8_t*>(row + i)), v);
     if (!inside(i)) clear_outside(run, v);
   }
   __device__ __forceinline__ void clear_outside(int run, uint64_t* v) const {
@@ -298,7 +299,7 @@ struct Part {
         raw = make_uint4(two.x, two.y, 0, 0);
       }
     } else {
-      raw = read_shifted<__nv_bfloat16>(reinterpret_cast<const uint8_t*>(w + i));
+      raw = read_shifted(reinterpret_cast<const uint8_t*>(w + i));
     }
     v[0] = widen<__nv_bfloat16>(raw.x);
     v[1] = widen<__nv_bfloat16>(raw.y);
@@ -330,14 +331,16 @@ struct Part {
         if (i + k >= 0 && i + k < n) row[i + k] = e[k];
     }
   }
-  // y (F values) -> 8 bits
+  // y (F values) -> 8 bits.  Not VEC: the bytes pass through shared memory
+  // (bytes(n) of it), from which they are stored in whole pieces at q's own
+  // alignment.
+  static __host__ __device__ size_t bytes(int n) { return VEC ? 0 : ((size_t)n + 15) / 16 * 16 + 64; }
   __device__ __forceinline__ void quantise(const uint64_t* y, unsigned amax_bits, int8_t* q,
-                                           float* scale) const {
+                                           float* scale, uint8_t* held) const {
     const float f = quant_factor(amax_bits);
     if (threadIdx.x == 0) *scale = quant_scale(amax_bits);
     const uint64_t f2 = both(f);
-    // where the bytes of a piece can be stored together
-    const bool together = VEC || ((reinterpret_cast<uintptr_t>(q) - lead) & (kPer - 1)) == 0;
+    uint8_t* to = VEC ? reinterpret_cast<uint8_t*>(q) : held + 16 + lead;  // element 0's place
 #pragma unroll
     for (int run = 0; run < kRuns; run++) {
       const int i = at(run);
@@ -347,18 +350,24 @@ struct Part {
 #pragma unroll
       for (int k = 0; k < kPer / 4; k++)
         b[k] = f != 0.0f ? quant4(v[2 * k], v[2 * k + 1], f2) : 0u;
-      if (together && inside(i)) {
-        if constexpr (kPer == 8)
-          *reinterpret_cast<uint2*>(q + i) = make_uint2(b[0], b[1]);
-        else
-          *reinterpret_cast<unsigned*>(q + i) = b[0];
-      } else if (inside(i)) {
+      if constexpr (kPer == 8)
+        *reinterpret_cast<uint2*>(to + i) = make_uint2(b[0], b[1]);
+      else
+        *reinterpret_cast<unsigned*>(to + i) = b[0];
+    }
+    if constexpr (!VEC) {
+      __syncthreads();
+      const int mis = (int)(reinterpret_cast<uintptr_t>(q) & 15);
+      for (int i = (int)threadIdx.x * 16 - mis; i < n; i += (int)blockDim.x * 16) {
+        const uint4 raw = read_shifted(to + i);
+        if (i >= 0 && i + 16 <= n) {
+          *reinterpret_cast<uint4*>(q + i) = raw;
+        } else {
+          const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-        for (int k = 0; k < kPer; k++) q[i + k] = (int8_t)(uint8_t)(b[k / 4] >> (8 * (k & 3)));
-      } else {
-#pragma unroll
-        for (int k = 0; k < kPer; k++)
-          if (i + k >= 0 && i + k < n) q[i + k] = (int8_t)(uint8_t)(b[k / 4] >> (8 * (k & 3)));
+          for (int k = 0; k < 16; k++)
+            if (i + k >= 0 && i + k < n) q[i + k] = (int8_t)(uint8_t)(word[k / 4] >> (8 * (k & 3)));
+        }
       }
     }
   }
@@ -390,8 +399,8 @@ __device__ __forceinline__ void walk_rows(uint8_t* smem, const T* a, long lda, c
   int row = blockIdx.x, at = 0;
   auto stage = [&](int r, int which) {
     if (r < rows) {
-      part.stage(smem + which * 2 * room, a + r * lda);
-      if (b) part.stage(smem + (which * 2 + 1) * room, b + r * ldb);
+      part.stage(smem + which * 2 * room, a + r * lda, 0);
+      if (b) part.stage(smem + (which * 2 + 1) * room, b + r * ldb, 1);
     }
     copies_commit();
   };
@@ -425,15 +434,16 @@ __global__ void __launch_bounds__(kMaxThr) norm_rows_kernel(NormArgs a) {
   __shared__ unsigned redu[32];
   pdl_wait();
   pdl_launch_dependents();
-  uint8_t* rows_mem = stage_mem;
+  uint8_t* held = stage_mem;  // the row's bytes
+  uint8_t* rows_mem = stage_mem + P::bytes(a.n);
   const uint16_t* w = a.w;
   if constexpr (!VEC) {
     // the weights too are read shifted: staged once, before any row's barrier
     using W = Part<__nv_bfloat16, 8, false>;
     if (a.w) {
       const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(a.w);
-      W{a.n, 0}.stage(stage_mem, src);
-      w = reinterpret_cast<const uint16_t*>(W::place(stage_mem, src));
+      W{a.n, 0}.stage(rows_mem, src, 2);
+      w = reinterpret_cast<const uint16_t*>(W::place(rows_mem, src));
       rows_mem += W::room(a.n);
     }
   }
@@ -487,7 +497,8 @@ __global__ void __launch_bounds__(kMaxThr) norm_rows_kernel(NormArgs a) {
         }
         // red and redu: the other's barrier lies between a row's reads and the
         // next row's writes
-        part.quantise(v, block_max(abs_bits(m), redu), a.q + row * a.ldq, a.scale + row);
+        part.quantise(v, block_max(abs_bits(m), redu), a.q + row * a.ldq, a.scale + row,
+                      held);
       });
 }
 
@@ -500,7 +511,7 @@ __global__ void __launch_bounds__(kMaxThr) silu_rows_kernel(SiluArgs a) {
   pdl_wait();
   pdl_launch_dependents();
   walk_rows<T, F, VEC>(
-      stage_mem, static_cast<const T*>(a.g), a.ld, static_cast<const T*>(a.u), a.ld, a.n, a.rows,
+      stage_mem + P::bytes(a.n), static_cast<const T*>(a.g), a.ld, static_cast<const T*>(a.u), a.ld, a.n, a.rows,
       a.buffers, [&](long row, const T* g, const T* u, auto next) {
         const P part{a.n, P::misplaced(static_cast<const T*>(a.g) + row * a.ld)};
         uint64_t v[F / 2];
@@ -518,7 +529,8 @@ __global__ void __launch_bounds__(kMaxThr) silu_rows_kernel(SiluArgs a) {
           }
         }
         next();
-        part.quantise(v, block_max(abs_bits(m), redu[parity]), a.q + row * a.ldq, a.scale + row);
+        part.quantise(v, block_max(abs_bits(m), redu[parity]), a.q + row * a.ldq, a.scale + row,
+                      stage_mem);
         parity ^= 1;
       });
 }
@@ -623,6 +635,7 @@ int rows_launch(Args a, bool vec, Shape s, size_t extra, void (*wide)(Args), Pic
   constexpr int per = 16 / (int)sizeof(T);
   const int span = vec ? a.n : a.n + per - 1;  // with the lead
   while (s.f < 32 && span > s.f * kMaxThr) s.f *= 2;
+  if (!vec) extra += Part<T, 8, false>::bytes(a.n);
   const size_t pair = 2 * (vec ? Part<T, 8, true>::room(a.n) : Part<T, 8, false>::room(a.n));
   a.buffers = !vec && extra + 2 * pair <= kStageMax ? 2 : 1;
   const size_t smem = extra + a.buffers * pair;
@@ -645,7 +658,8 @@ int norm_rows(const NormArgs& a, cudaStream_t st) {
                    (!a.h || aligned(a.h, a.ldh, sizeof(T), 16)) &&
                    (!a.w || aligned(a.w, 0, 2, 2 * per)) && aligned(a.q, a.ldq, 1, per);
   const bool few = a.rows < 148 * 2;
-  const Shape s{few ? 8 : 16, few || sizeof(T) == 4 ? 1 : 4};
+  const Shape s = !vec ? Shape{16, few ? 1 : 2}
+                       : Shape{few ? 8 : 16, few || sizeof(T) == 4 ? 1 : 4};
   const size_t extra = !vec && a.w ? Part<__nv_bfloat16, 8, false>::room(a.n) : 0;
   return rows_launch<T>(a, vec, s, extra, norm_wide_kernel<T>, [](int f, bool v) {
     return v ? (f == 8 ? norm_rows_kernel<T, 8, true>
@@ -661,7 +675,9 @@ int silu_rows(const SiluArgs& a, cudaStream_t st) {
   const bool vec = a.n % per == 0 && aligned(a.g, a.ld, sizeof(T), 16) &&
                    aligned(a.u, a.ld, sizeof(T), 16) && aligned(a.q, a.ldq, 1, per);
   const bool few = a.rows < 148 * 2;
-  const Shape s{few ? 8 : sizeof(T) == 2 && a.n >= 4096 ? 32 : 16, few || sizeof(T) == 4 ? 1 : 2};
+  const Shape s = !vec ? Shape{16, few ? 1 : 2}
+                       : Shape{few ? 8 : sizeof(T) == 2 && a.n >= 4096 ? 32 : 16,
+                               few || sizeof(T) == 4 ? 1 : 2};
   return rows_launch<T>(a, vec, s, 0, silu_wide_kernel<T>, [](int f, bool v) {
     return v ? (f == 8 ? silu_rows_kernel<T, 8, true>
                        : f == 16 ? silu_rows_kernel<T, 16, true> : silu_rows_kernel<T, 32, true>)
