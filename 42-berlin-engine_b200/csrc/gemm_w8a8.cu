@@ -15,7 +15,14 @@
 // The sum is exact in int32, so neither the tiles nor the split over K change
 // a bit of the result.
 //
-// gemm_w8a8_kernel: a tile is R <= 128 channels x up to 256 tokens.  With few
+// gemm_w8a8_pair_kernel (many tokens): the two CTAs of a cluster share a tile of
+// 256 channels x Tn <= 256 tokens; each holds half of the channels and half of
+// the tokens in shared memory, and the first issues tcgen05.mma.cta_group::2
+// for both, which reads both halves: per SM half the token bytes of a 128-row
+// tile.  Loads of both CTAs complete on the first one's barriers; commits
+// release the stages of both.
+//
+// gemm_w8a8_kernel (few tokens): a tile is R <= 128 channels x up to 256 tokens.  With few
 // tokens the weights' bytes are the bound, and R is chosen so that the tiles
 // fill whole rounds of the SMs (every SM streams the same share of the
 // weights); the MMA computes its 128 rows whatever R is, which costs
@@ -139,6 +146,41 @@ __device__ __forceinline__ void st_peer(uint32_t addr, int v) {
 __device__ __forceinline__ void st_peer4(uint32_t addr, const int* v) {
   asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]),
                "r"(v[1]), "r"(v[2]), "r"(v[3])
+               : "memory");
+}
+
+// ------------------------------------------------ two CTAs, one tile --
+
+__device__ __forceinline__ void mma_i8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                            uint32_t acc) {
+  asm volatile(
+      "{ .reg .pred p; setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p; }" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+// arrives on `bar` of both CTAs once the MMAs issued so far have ended
+__device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+      "[%0], %1;" ::"r"(smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
+// into this CTA's shared memory, completing on a barrier of either CTA
+__device__ __forceinline__ void tma_2d_pair(uint32_t dst, const CUtensorMap* map, int x, int y,
+                                            uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes."
+      "cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+
+__device__ __forceinline__ void arrive_at(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
                : "memory");
 }
 
@@ -367,6 +409,173 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// Tiles in groups of kGroup channel tiles: the CTAs at work at one time share
+// both few channel tiles and few token tiles in L2.
+constexpr int kGroup = 8;
+
+__device__ __forceinline__ void tile_at(int tile, int mt, int nt, int* c, int* t) {
+  const int per = kGroup * nt, g = tile / per, in = tile - g * per;
+  const int width = min(kGroup, mt - g * kGroup);
+  *t = in / width;
+  *c = g * kGroup + in - *t * width;
+}
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    gemm_w8a8_pair_kernel(const __grid_constant__ CUtensorMap mx,
+                          const __grid_constant__ CUtensorMap mw, const W8A8Args a) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem);  // the first CTA's count
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* tfull = empty + kMaxStages;
+  uint64_t* tempty = tfull + 2;  // the first CTA's count
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(tempty + 2);
+  int* failed = reinterpret_cast<int*>(tslot + 1);
+  uint8_t* stg = smem + kHdr;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = cluster_rank();
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1, tiles = a.mt * a.nt;
+  const int half = a.Tn / 2;  // tokens of this CTA's share
+  const uint32_t wbytes = 128 * kKb, stage = wbytes + (uint32_t)half * kKb;
+
+  if (tid == 0) {
+    for (int s = 0; s < a.S; s++) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], 8);  // the epilogue warps of both
+    }
+    *failed = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tslot)), "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_arrive();
+  cluster_wait();
+  tc_fence_after();
+  pdl_launch_dependents();
+  const uint32_t tbase = *tslot;
+  bool ok = true;
+
+  if (warp == 0) {
+    // ---------------------------------------------------------- producer
+    if (lane == 0) {
+      pdl_wait();
+      int s = 0, u = 0;
+      uint32_t phase = 1;
+      for (int tile = first; tile < tiles && ok; tile += step) {
+        int ct, tt;
+        tile_at(tile, a.mt, a.nt, &ct, &tt);
+        const int c = ct * 256 + (int)rank * 128, t = tt * a.Tn + (int)rank * half;
+        for (int i = 0; i < a.chunks; i++, u++) {
+          ok = mbar_wait(&empty[s], phase, a.status);
+          if (!ok) break;
+          if (rank == 0) mbar_expect_tx(&full[s], 2 * stage);
+          const uint32_t bar = peer_addr(smem_u32(&full[s]), 0);
+          const uint32_t dst = smem_u32(stg) + s * stage;
+          tma_2d_pair(dst, &mw, i * kKb, c, bar);
+          tma_2d_pair(dst + wbytes, &mx, i * kKb, t, bar);
+          if (++s == a.S) {
+            s = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (!ok && rank == 0)  // the copies in flight land before the CTAs may end
+        for (int v = max(0, u - a.S); v < u; v++)
+          mbar_wait(&full[v % a.S], (uint32_t)((v / a.S) & 1), a.status);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // -------------------------------------------------------- MMA issuer
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = i8_idesc(256, a.Tn);
+      int n = 0, s = 0;
+      uint32_t phase = 0;
+      for (int tile = first; tile < tiles && ok; tile += step, n++) {
+        const int buf = n & 1;
+        if (n >= 2) ok = mbar_wait(&tempty[buf], (uint32_t)(((n >> 1) - 1) & 1), a.status);
+        tc_fence_after();
+        const uint32_t d = tbase + (uint32_t)(buf * 256);
+        for (int i = 0; i < a.chunks && ok; i++) {
+          ok = mbar_wait(&full[s], phase, a.status);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t src = smem_u32(stg) + s * stage;
+          const uint64_t da = sw128_desc(src), db = sw128_desc(src + wbytes);
+#pragma unroll
+          for (int j = 0; j < kKb / 32; j++)
+            mma_i8_pair(d, da + 2 * j, db + 2 * j, idesc, (i > 0 || j > 0) ? 1u : 0u);
+          mma_commit_pair(&empty[s]);
+          if (++s == a.S) {
+            s = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) {
+          st_peer(peer_addr(smem_u32(failed), 0), 1);
+          st_peer(peer_addr(smem_u32(failed), 1), 1);
+          asm volatile("fence.acq_rel.cluster;" ::: "memory");
+        }
+        mma_commit_pair(&tfull[buf]);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ----------------------------------------------------------- epilogue
+    const int q = warp & 3, r = q * 32 + lane;
+    pdl_wait();
+    int n = 0;
+    for (int tile = first; tile < tiles; tile += step, n++) {
+      int ct, tt;
+      tile_at(tile, a.mt, a.nt, &ct, &tt);
+      const int c = ct * 256 + (int)rank * 128 + r, t0 = tt * a.Tn;
+      const bool mine = c < a.m;
+      const int buf = n & 1;
+      ok = ok && mbar_wait(&tfull[buf], (uint32_t)((n >> 1) & 1), a.status) &&
+           *reinterpret_cast<volatile int*>(failed) == 0;
+      tc_fence_after();
+      const uint32_t ta = tbase + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * 256);
+      float sw = mine ? a.sw[c] : 0.0f;
+      if (!ok) sw = __uint_as_float(0x7fc00000u);
+      const int tn = min(a.Tn, a.nb - t0);
+      T* y = static_cast<T*>(a.y) + (long)t0 * a.ldy + c;
+      for (int j0 = 0; j0 < tn; j0 += 16) {
+        const float sxl = a.sx[t0 + min(j0 + (lane & 15), tn - 1)];
+        int acc[16];
+        tmem_ld16(ta + j0, acc);
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+          const float sx = __shfl_sync(0xffffffffu, sxl, j);
+          if (mine && j0 + j < tn)
+            y[(long)(j0 + j) * a.ldy] = from_f32<T>(scaled(acc[j], sx, sw));
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_at(peer_addr(smem_u32(&tempty[buf]), 0));
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  // the other CTA's arrivals and copies into this one's barriers are over
+  cluster_arrive();
+  cluster_wait();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(512)
+                 : "memory");
+  }
+}
+
 // ------------------------------------------------------------------ host --
 
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
@@ -402,7 +611,7 @@ bool byte_map(CUtensorMap* map, const void* p, long k, long rows, long ld, int b
 }
 
 struct Plan {
-  int R, Tn, mt, nt, C;
+  int R, Tn, mt, nt, C;  // R = 256: a pair's tile
   double cost;
 };
 
@@ -422,9 +631,12 @@ cudaError_t device_slots(const Slots** out) {
   static std::mutex lock;
   if (!known[dev].load(std::memory_order_acquire)) {
     std::lock_guard<std::mutex> hold(lock);
-    const void* kernels[3] = {(const void*)gemm_w8a8_kernel<float>,
+    const void* kernels[6] = {(const void*)gemm_w8a8_kernel<float>,
                               (const void*)gemm_w8a8_kernel<__nv_bfloat16>,
-                              (const void*)gemm_w8a8_kernel<__half>};
+                              (const void*)gemm_w8a8_kernel<__half>,
+                              (const void*)gemm_w8a8_pair_kernel<float>,
+                              (const void*)gemm_w8a8_pair_kernel<__nv_bfloat16>,
+                              (const void*)gemm_w8a8_pair_kernel<__half>};
     for (const void* k : kernels) {
       e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
       if (e != cudaSuccess) return e;
@@ -481,7 +693,46 @@ Plan plan_tiles(int m, int chunks, int nb, const Slots& at_once) {
       if (cost < best.cost) best = Plan{R, Tn, mt, cols, C, cost};
     }
   }
+  // pairs: 256 channels x Tn tokens
+  for (int nt = nt0; nt <= nt0 * 4 && (nt == nt0 || nb >= 64 * nt); nt++) {
+    const int Tn = ceil_div(ceil_div(nb, nt), 32) * 32;
+    const int cols = ceil_div(nb, Tn), mt = ceil_div(m, 256);
+    const int slots = at_once.clusters[2];
+    if (slots < 1) break;
+    const double per_sm = (double)ceil_div((long)mt * cols, slots) * chunks;
+    const double load = per_sm * (128 + Tn / 2) * kKb / 50.0;
+    const double mma = per_sm * 2.0 * Tn;
+    const double cost = (load > mma ? load : mma) + 1000.0;
+    if (cost < best.cost) best = Plan{256, Tn, mt, cols, 2, cost};
+  }
   return best;
+}
+
+template <typename T>
+int launch_pair(const int8_t* x, long ldx, const int8_t* w, long ldw, int k, W8A8Args a, int slots,
+                cudaStream_t st) {
+  const int stage = (128 + a.Tn / 2) * kKb;
+  a.S = (kSmemMax - kHdr) / stage;
+  if (a.S > kMaxStages) a.S = kMaxStages;
+  CUtensorMap mx, mw;
+  if (!byte_map(&mx, x, k, a.nb, ldx, a.Tn / 2) || !byte_map(&mw, w, k, a.m, ldw, 128)) {
+    ec_set_last_error("ec_op_gemm_w8a8: tensor map refused");
+    return EC_ERR_CUDA;
+  }
+  const int tiles = a.mt * a.nt;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * (tiles < slots ? tiles : slots));
+  cfg.blockDim = dim3(kThreads);
+  const size_t smem = kHdr + (size_t)a.S * stage;
+  cfg.dynamicSmemBytes = smem > 120 * 1024 ? smem : 120 * 1024;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  EC_CUDA_TRY(cudaLaunchKernelEx(&cfg, gemm_w8a8_pair_kernel<T>, mx, mw, a));
+  return EC_OK;
 }
 
 template <typename T>
@@ -501,6 +752,7 @@ int launch(const int8_t* x, long ldx, const int8_t* w, long ldw, int k, W8A8Args
   a.mt = p.mt;
   a.nt = p.nt;
   a.C = p.C;
+  if (p.R == 256) return launch_pair<T>(x, ldx, w, ldw, k, a, slots->clusters[2], st);
   a.xrows = a.nb < a.Tn ? a.nb : a.Tn;
   const int block = (a.Tn + ((a.R + 7) & ~7)) * kKb;
   const int share = ceil_div(a.chunks, a.C);
