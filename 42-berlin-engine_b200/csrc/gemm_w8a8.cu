@@ -47,6 +47,7 @@ constexpr int kMaxStages = 24;
 constexpr int kHdr = 1024;
 constexpr int kSmemMax = 227 * 1024;
 constexpr int kMaxCluster = 8;
+constexpr int kAhead = 8;      // blocks of weights that a CTA brings to L2 before it may start
 
 struct W8A8Args {
   const float* sx;
@@ -60,6 +61,7 @@ struct W8A8Args {
   int xrows;    // token rows of one box: min(Tn, nb)
   int ks, S;    // blocks of K per stage, stages
   int C;        // CTAs that share a tile's K
+  int exchange; // bytes of shared memory for their partial sums
   int* status;
 };
 
@@ -120,6 +122,18 @@ __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int
       "{%2, %3}], [%4];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
       : "memory");
+}
+
+// Ahead of the copies: the tensor map, and a box into L2.  L2 is where all
+// writers meet, so a box may be prefetched before the kernel that writes it has
+// ended; only the copy itself has to wait.
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+__device__ __forceinline__ void prefetch_2d(const CUtensorMap* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y)
+               : "memory");
 }
 
 __device__ __forceinline__ void cluster_arrive() {
@@ -201,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* tempty = tfull + 2;
   uint32_t* tslot = reinterpret_cast<uint32_t*>(tempty + 2);
   int* failed = reinterpret_cast<int*>(tslot + 1);
-  uint8_t* stg = smem + kHdr;
+  uint8_t* stg = smem + kHdr + a.exchange;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int C = a.C, rank = C > 1 ? (int)cluster_rank() : 0;
   const int first = blockIdx.x / C, step = gridDim.x / C, tiles = a.mt * a.nt;
@@ -234,6 +248,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (C > 1) cluster_arrive();  // waited for before the first store into a peer
   pdl_launch_dependents();
   const uint32_t tbase = *tslot;
   bool ok = true;
@@ -241,6 +256,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 0) {
     // ---------------------------------------------------------- producer
     if (lane == 0) {
+      prefetch_map(&mw);
+      prefetch_map(&mx);
+      for (int b = c0; b < min(c1, c0 + kAhead); b++)
+        prefetch_2d(&mw, b * kKb, first / a.nt * a.R);
       pdl_wait();
       int u = 0, s = 0;
       uint32_t phase = 1;  // a fresh barrier's previous phase counts as complete
@@ -317,11 +336,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int c = tile / a.nt * a.R + r, t0 = tile % a.nt * a.Tn;
       const bool mine = r < a.R && c < a.m;
       const int buf = n & 1;
+      float sw = mine ? a.sw[c] : 0.0f;
       ok = ok && mbar_wait(&tfull[buf], (uint32_t)((n >> 1) & 1), a.status) &&
            *reinterpret_cast<volatile int*>(failed) == 0;
       tc_fence_after();
       const uint32_t ta = tbase + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * (tcols >> 1));
-      float sw = mine ? a.sw[c] : 0.0f;
       if (!ok) sw = __uint_as_float(0x7fc00000u);
       const int tn = min(a.Tn, a.nb - t0);
       T* y = static_cast<T*>(a.y) + (long)t0 * a.ldy + c;
@@ -342,25 +361,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   if (C > 1) {
-    // One tile per cluster.  The stages become the exchange buffer
-    // [CTA of the cluster][its token columns / 4][128 channels][4] once every
-    // CTA's MMAs have read them.
+    // One tile per cluster: every CTA sends each other its partial sums of the
+    // columns that the other finishes, into its exchange buffer [CTA of the
+    // cluster][token columns / 4][128 channels][4].
     const int wc = ((a.Tn + C - 1) / C + 3) & ~3;  // token columns each CTA finishes
     const int q = warp & 3, r = q * 32 + lane;
     const int c = first / a.nt * a.R + r, t0 = first % a.nt * a.Tn;
+    const bool mine = warp >= 2 && r < a.R && c < a.m;
+    float sw = 0.0f;
+    cluster_wait();  // every CTA of the cluster runs
     if (warp >= 2) {
       pdl_wait();
+      if (mine) sw = a.sw[c];
       ok = mbar_wait(&tfull[0], 0, a.status);
       tc_fence_after();
-    }
-    __syncwarp();
-    cluster_arrive();
-    cluster_wait();
-    if (warp >= 2) {
       ok = ok && *reinterpret_cast<volatile int*>(failed) == 0;
       if (!ok && lane == 0)
         for (int p = 0; p < C; p++) st_peer(peer_addr(smem_u32(failed), p), 1);
-      const uint32_t at = smem_u32(stg) + (uint32_t)(rank * wc * 512 + r * 16);
+      const uint32_t at = smem_u32(smem + kHdr) + (uint32_t)(rank * wc * 512 + r * 16);
       const uint32_t ta = tbase + ((uint32_t)(q * 32) << 16);
       for (int j0 = 0; j0 < a.Tn; j0 += 16) {
         int acc[16];
@@ -376,11 +394,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     cluster_arrive();
     cluster_wait();
-    if (warp >= 2 && r < a.R && c < a.m) {
+    if (mine) {
       const int tn = min(min(a.Tn, a.nb - t0), (rank + 1) * wc) - rank * wc;
-      const int4* part = reinterpret_cast<const int4*>(stg) + r;
-      const float sw =
-          *reinterpret_cast<volatile int*>(failed) ? __uint_as_float(0x7fc00000u) : a.sw[c];
+      const int4* part = reinterpret_cast<const int4*>(smem + kHdr) + r;
+      if (*reinterpret_cast<volatile int*>(failed)) sw = __uint_as_float(0x7fc00000u);
       const int tt = t0 + rank * wc;
       T* y = static_cast<T*>(a.y) + (long)tt * a.ldy + c;
       for (int j = 0; j < tn; j += 4) {
@@ -468,6 +485,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (warp == 0) {
     // ---------------------------------------------------------- producer
     if (lane == 0) {
+      prefetch_map(&mw);
+      prefetch_map(&mx);
+      if (first < tiles) {
+        int ct, tt;
+        tile_at(first, a.mt, a.nt, &ct, &tt);
+        for (int i = 0; i < min(a.chunks, kAhead); i++)
+          prefetch_2d(&mw, i * kKb, ct * 256 + (int)rank * 128);
+      }
       pdl_wait();
       int s = 0, u = 0;
       uint32_t phase = 1;
@@ -540,11 +565,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int c = ct * 256 + (int)rank * 128 + r, t0 = tt * a.Tn;
       const bool mine = c < a.m;
       const int buf = n & 1;
+      float sw = mine ? a.sw[c] : 0.0f;
       ok = ok && mbar_wait(&tfull[buf], (uint32_t)((n >> 1) & 1), a.status) &&
            *reinterpret_cast<volatile int*>(failed) == 0;
       tc_fence_after();
       const uint32_t ta = tbase + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * 256);
-      float sw = mine ? a.sw[c] : 0.0f;
       if (!ok) sw = __uint_as_float(0x7fc00000u);
       const int tn = min(a.Tn, a.nb - t0);
       T* y = static_cast<T*>(a.y) + (long)t0 * a.ldy + c;
@@ -610,11 +635,6 @@ bool byte_map(CUtensorMap* map, const void* p, long k, long rows, long ld, int b
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-struct Plan {
-  int R, Tn, mt, nt, C;  // R = 256: a pair's tile
-  double cost;
-};
-
 // What a device runs at once: SMs, and clusters of each size.  Clusters live
 // inside a GPC, so e.g. 33 clusters of 4 fit on 148 SMs, not 37.
 struct Slots {
@@ -663,49 +683,85 @@ cudaError_t device_slots(const Slots** out) {
   return cudaSuccess;
 }
 
+struct Plan {
+  int R, Tn, C, ks;  // R = 256: a pair's tile
+  float cost;
+};
+
 inline int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 
-// The tile for m x k weights and nb tokens on n_sm SMs: the cheapest of the
-// token splits and cluster sizes under the model below (cycles).
+// Cycles of a plan, up to what all plans have in common: per block of K the
+// slowest of the copies into an SM, the MMAs (whose 128 or 256 rows cost 40-50
+// cycles however few tokens there are) and the issue of a stage, then the
+// epilogue and the join of a split K.  The constants are fitted to the times
+// of all plans of 88 shapes (1-7378 tokens, 65-128256 channels, k 64-27584):
+// the plan chosen by this model is within 1% of the best one's time in the
+// mean, 10% at most.
+float plan_cost(const Plan& p, int m, int chunks, int nb, const Slots& at_once) {
+  const long cols = ceil_div(nb, p.Tn);
+  if (p.R == 256) {
+    const int rounds = ceil_div(ceil_div(m, 256) * cols, at_once.clusters[2]);
+    const float copy = (128 + p.Tn / 2) * kKb / 53.0f;
+    const float mma = 4.0f * fmaxf(41.0f, 0.5f * p.Tn);
+    return rounds * (chunks * fmaxf(fmaxf(copy, mma), 250.0f) + 2.2f * p.Tn);
+  }
+  const int rounds = ceil_div(ceil_div(m, p.R) * cols, at_once.clusters[p.C]);
+  const int share = ceil_div(chunks, p.C);
+  const float copy = (p.R + p.Tn) * kKb / 70.0f;
+  const float mma = 4.0f * fmaxf(50.0f, 0.5f * p.Tn);
+  return rounds * (share * fmaxf(copy, mma) + ceil_div(share, p.ks) * 254.0f + 14.0f * p.Tn) +
+         (p.ks < share ? p.ks : share) * mma * 0.41f + (p.C > 1 ? 400.0f + 24.0f * p.Tn : 0.0f);
+}
+
 Plan plan_tiles(int m, int chunks, int nb, const Slots& at_once) {
-  Plan best{0, 0, 0, 0, 0, 1e300};
-  const int nt0 = ceil_div(nb, 256);
-  for (int nt = nt0; nt <= nt0 * 4 && (nt == nt0 || nb >= 64 * nt); nt *= 2) {
-    const int Tn = ceil_div(ceil_div(nb, nt), 16) * 16;
-    const int cols = ceil_div(nb, Tn);
-    for (int C = 1; C <= kMaxCluster; C++) {
-      if (C > chunks) break;
+  Plan best{0, 0, 0, 0, 1e30f};
+  auto offer = [&](Plan p) {
+    p.cost = plan_cost(p, m, chunks, nb, at_once);
+    if (p.cost < best.cost) best = p;
+  };
+  // pairs: 256 channels x Tn tokens
+  if (at_once.clusters[2] > 0)
+    for (int nt = ceil_div(nb, 256), i = 0; i < 6; nt++, i++)
+      offer(Plan{256, ceil_div(ceil_div(nb, nt), 32) * 32, 2, 1, 0});
+  // single CTAs, or clusters that split K
+  const int splits[5] = {ceil_div(nb, 256), 2 * ceil_div(nb, 256), ceil_div(nb, 128),
+                         ceil_div(nb, 64), ceil_div(nb, 32)};
+  for (int i = 0; i < 5; i++) {
+    const int Tn = ceil_div(ceil_div(nb, splits[i]), 16) * 16, cols = ceil_div(nb, Tn);
+    if ((i > 0 && splits[i] == splits[i - 1]) || (cols > 16 && Tn < 128)) continue;
+    for (int C = 1; C <= kMaxCluster && C <= chunks && (C == 1 || Tn <= 128); C++) {
       const int slots = at_once.clusters[C];
       if (slots < 1) continue;
-      int rounds = ceil_div((long)ceil_div(m, 128) * cols, slots);
-      if (C > 1 && rounds > 1) break;
-      // the most tiles those rounds hold, then the rows each needs
-      int mt = (int)((long)rounds * slots / cols);
-      int R = ceil_div(m, mt);
-      if (R > 128) R = 128;
-      R = R < 8 ? (m < 8 ? m : 8) : R;
-      mt = ceil_div(m, R);
-      const double per_sm = (double)rounds * ceil_div(chunks, C);  // blocks of K per SM
-      const double load = per_sm * (R + Tn) * kKb / 34.0;          // bytes a cycle into an SM
-      const double mma = per_sm * (Tn < 32 ? 64.0 : 2.0 * Tn);
-      const double join = C > 1 ? 1500.0 + 20.0 * Tn : 0.0;
-      const double cost = (load > mma ? load : mma) + join;
-      if (cost < best.cost) best = Plan{R, Tn, mt, cols, C, cost};
+      const int q = ceil_div((long)ceil_div(m, 128) * cols, slots);
+      if (C > 1 && q > 1) break;
+      for (int more = 0; more < (C == 1 && q < 4 ? 2 : 1); more++) {
+        // the most tiles that these rounds hold, then the channels each needs
+        const int mt = (int)((long)(q + more) * slots / cols);
+        int R = ceil_div(m, mt);
+        R = R > 128 ? 128 : R < 8 ? (m < 8 ? m : 8) : R;
+        const int block = (Tn + (R + 7) / 8 * 8) * kKb, share = ceil_div(chunks, C);
+        for (int ks = 1; ks <= 8 && ks <= share && block * ks <= 90000; ks *= 2) {
+          if (block * ks < 6000 && ks < 8 && 2 * ks <= share) continue;
+          offer(Plan{R, Tn, C, ks, 0});
+        }
+      }
     }
   }
-  // pairs: 256 channels x Tn tokens
-  for (int nt = nt0; nt <= nt0 * 4 && (nt == nt0 || nb >= 64 * nt); nt++) {
-    const int Tn = ceil_div(ceil_div(nb, nt), 32) * 32;
-    const int cols = ceil_div(nb, Tn), mt = ceil_div(m, 256);
-    const int slots = at_once.clusters[2];
-    if (slots < 1) break;
-    const double per_sm = (double)ceil_div((long)mt * cols, slots) * chunks;
-    const double load = per_sm * (128 + Tn / 2) * kKb / 50.0;
-    const double mma = per_sm * 2.0 * Tn;
-    const double cost = (load > mma ? load : mma) + 1000.0;
-    if (cost < best.cost) best = Plan{256, Tn, mt, cols, 2, cost};
-  }
   return best;
+}
+
+// The plan of a shape, kept by the calling thread (a plan costs microseconds)
+Plan plan_of(int m, int chunks, int nb, const Slots& at_once) {
+  struct Kept {
+    int m, chunks, nb;
+    const Slots* slots;
+    Plan plan;
+  };
+  static thread_local Kept kept[64];
+  Kept& k = kept[((unsigned)m * 31u + (unsigned)chunks * 17u + (unsigned)nb) % 64];
+  if (k.m != m || k.chunks != chunks || k.nb != nb || k.slots != &at_once)
+    k = Kept{m, chunks, nb, &at_once, plan_tiles(m, chunks, nb, at_once)};
+  return k.plan;
 }
 
 template <typename T>
@@ -746,23 +802,23 @@ int launch(const int8_t* x, long ldx, const int8_t* w, long ldw, int k, W8A8Args
   EC_CUDA_TRY(device_slots(&slots));
   const int n_sm = slots->clusters[1];
   a.chunks = ceil_div(k, kKb);
-  const Plan p = plan_tiles(a.m, a.chunks, a.nb, *slots);
+  const Plan p = plan_of(a.m, a.chunks, a.nb, *slots);
   a.R = p.R;
   a.Tn = p.Tn;
-  a.mt = p.mt;
-  a.nt = p.nt;
   a.C = p.C;
+  a.mt = ceil_div(a.m, a.R);
+  a.nt = ceil_div(a.nb, a.Tn);
   if (p.R == 256) return launch_pair<T>(x, ldx, w, ldw, k, a, slots->clusters[2], st);
   a.xrows = a.nb < a.Tn ? a.nb : a.Tn;
   const int block = (a.Tn + ((a.R + 7) & ~7)) * kKb;
-  const int share = ceil_div(a.chunks, a.C);
-  a.ks = 1;
-  while (a.ks < 8 && block * a.ks * 2 <= 40960 && a.ks * 2 <= share) a.ks *= 2;
+  a.ks = p.ks;
   // the last block's MMA reads 128 rows from its weights on
   const int slack = 128 * kKb;
-  a.S = (kSmemMax - kHdr - slack) / (block * a.ks);
+  const int finish = ((a.Tn + a.C - 1) / a.C + 3) & ~3;  // columns a CTA finishes
+  a.exchange = a.C > 1 ? (a.C * finish * 512 + 1023) & ~1023 : 0;
+  a.S = (kSmemMax - kHdr - slack - a.exchange) / (block * a.ks);
   if (a.S > kMaxStages) a.S = kMaxStages;
-  const size_t smem = kHdr + (size_t)a.S * block * a.ks + slack;
+  const size_t smem = kHdr + a.exchange + (size_t)a.S * block * a.ks + slack;
   CUtensorMap mx, mw;
   if (!byte_map(&mx, x, k, a.nb, ldx, a.xrows) || !byte_map(&mw, w, k, a.m, ldw, a.R)) {
     ec_set_last_error("ec_op_gemm_w8a8: tensor map refused");
