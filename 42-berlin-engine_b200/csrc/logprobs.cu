@@ -223,16 +223,37 @@ struct Warp {
                                        float c2) {
     const float cm = max_of(v);
     if (!(cm <= st.m)) rescale(st, max_nan(cm, st.m), c2);
+    // (l - m) in units of log 2, its power, and their product.  A logit of
+    // -inf makes the product NaN: such chunks, and those with values that are
+    // not the row's, are added with these far enough below for it to be 0.
     const uint64_t m2 = pair_of(-st.m, -st.m), c22 = pair_of(c2, c2);
+    uint64_t s = st.s, w = st.w;
+    bool plain = __all_sync(0xffffffffu, valid == (1u << kChunk) - 1u);
+    if (plain) {
 #pragma unroll
-    for (int j = 0; j < kChunk; j += 2) {
-      // (l - m) in units of log 2; -inf and undefined ones far enough below
-      const uint64_t x = mul2(add2(pair_of(v[j], v[j + 1]), m2), c22);
-      const float d0 = fmaxf(lo_f(x), kFar), d1 = fmaxf(hi_f(x), kFar);
-      const uint64_t e = pair_of(exp2_of(d0), exp2_of(d1));
-      st.s = add2(st.s, e);
-      fma2(st.w, e, pair_of(d0, d1));
+      for (int j = 0; j < kChunk; j += 2) {
+        const uint64_t x = mul2(add2(pair_of(v[j], v[j + 1]), m2), c22);
+        const uint64_t e = pair_of(exp2_of(lo_f(x)), exp2_of(hi_f(x)));
+        s = add2(s, e);
+        fma2(w, e, x);
+      }
+      const float sum = __fadd_rn(lo_f(w), hi_f(w));
+      plain = sum == sum;
     }
+    if (!plain) {
+      s = st.s;
+      w = st.w;
+#pragma unroll
+      for (int j = 0; j < kChunk; j += 2) {
+        const uint64_t x = mul2(add2(pair_of(v[j], v[j + 1]), m2), c22);
+        const float d0 = fmaxf(lo_f(x), kFar), d1 = fmaxf(hi_f(x), kFar);
+        const uint64_t e = pair_of(exp2_of(d0), exp2_of(d1));
+        s = add2(s, e);
+        fma2(w, e, pair_of(d0, d1));
+      }
+    }
+    st.s = s;
+    st.w = w;
     if (top && __any_sync(0xffffffffu, !(cm <= thr))) {
       unsigned mine = 0;  // the lane's values that can enter
 #pragma unroll
@@ -338,10 +359,15 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
   T* ring = reinterpret_cast<T*>(ring_mem + (size_t)warp * D * kChunkBytes<T>) + lane * kPer;
   constexpr int kSlot = kChunkBytes<T> / (int)sizeof(T);
   auto fetch = [&](int slot, int b) {
+    T* to = ring + slot * kSlot;
+    const T* from = body + (long)(b + lane) * kPer;
+    if (b + 32 * kLoads <= v1) {
 #pragma unroll
-    for (int u = 0; u < kLoads; u++) {
-      const int i = b + u * 32 + lane;
-      if (i < v1) cp_async16(ring + slot * kSlot + u * 32 * kPer, body + (long)i * kPer);
+      for (int u = 0; u < kLoads; u++) cp_async16(to + u * 32 * kPer, from + u * 32 * kPer);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kLoads; u++)
+        if (b + u * 32 + lane < v1) cp_async16(to + u * 32 * kPer, from + u * 32 * kPer);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -349,15 +375,22 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
   for (int d = 0; d < D; d++) fetch(d, first + d * step);
   // a chunk's values, -inf where the row has none; which are the row's
   auto read = [&](float* v, const T* kept, int b) {
-    unsigned valid = 0;
+    unsigned valid = (1u << kChunk) - 1u;
 #pragma unroll
     for (int u = 0; u < kLoads; u++) {
       const uint4 raw = *reinterpret_cast<const uint4*>(kept + u * 32 * kPer);
       const T* e = reinterpret_cast<const T*>(&raw);
-      const bool in = b + u * 32 + lane < v1;
-      if (in) valid |= ((1u << kPer) - 1u) << (u * kPer);
 #pragma unroll
-      for (int k = 0; k < kPer; k++) v[u * kPer + k] = in ? to_f32(e[k]) : -INFINITY;
+      for (int k = 0; k < kPer; k++) v[u * kPer + k] = to_f32(e[k]);
+    }
+    if (b + 32 * kLoads > v1) {
+#pragma unroll
+      for (int u = 0; u < kLoads; u++) {
+        if (b + u * 32 + lane < v1) continue;
+        valid &= ~(((1u << kPer) - 1u) << (u * kPer));
+#pragma unroll
+        for (int k = 0; k < kPer; k++) v[u * kPer + k] = -INFINITY;
+      }
     }
     return valid;
   };
