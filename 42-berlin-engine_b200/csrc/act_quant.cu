@@ -696,6 +696,10 @@ extern "C" int ec_op_add_rmsnorm_quant(int type, const void* x, int64_t ldx, con
   if (!ec::known_type(type)) return ec::arg_error("ec_op_add_rmsnorm_quant: unknown type");
   if (!x || !q || !scales || rows <= 0 || n <= 0 || !(eps >= 0.0f))
     return ec::arg_error("ec_op_add_rmsnorm_quant: null pointer, empty shape or negative eps");
+  if (!ec::on_elements(type, x) || !ec::on_elements(type, residual) ||
+      !ec::on_elements(type, sum_out) || (reinterpret_cast<uintptr_t>(w) & 1) ||
+      (reinterpret_cast<uintptr_t>(scales) & 3))
+    return ec::arg_error("ec_op_add_rmsnorm_quant: a pointer is not aligned to its element");
   if (ldx < n || ldq < n || (residual && ldr < n) || (sum_out && lds < n))
     return ec::arg_error("ec_op_add_rmsnorm_quant: a row stride is shorter than the row");
   if (n > ec::kMaxN) return ec::unsupported("ec_op_add_rmsnorm_quant: n > 57344");
@@ -712,6 +716,9 @@ extern "C" int ec_op_silu_mul_quant(int type, const void* gate, const void* up, 
   if (!ec::known_type(type)) return ec::arg_error("ec_op_silu_mul_quant: unknown type");
   if (!gate || !up || !q || !scales || rows <= 0 || n <= 0)
     return ec::arg_error("ec_op_silu_mul_quant: null pointer or empty shape");
+  if (!ec::on_elements(type, gate) || !ec::on_elements(type, up) ||
+      (reinterpret_cast<uintptr_t>(scales) & 3))
+    return ec::arg_error("ec_op_silu_mul_quant: a pointer is not aligned to its element");
   if (ld < n || ldq < n)
     return ec::arg_error("ec_op_silu_mul_quant: a row stride is shorter than the row");
   if (n > ec::kMaxN) return ec::unsupported("ec_op_silu_mul_quant: n > 57344");

@@ -859,6 +859,10 @@ extern "C" int ec_op_gemm_w8a8(const int8_t* x, int64_t ldx, const float* x_scal
   if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | (uintptr_t)ldx |
        (uintptr_t)ldw) & 15)
     return ec::arg_error("ec_op_gemm_w8a8: x, w, ldx and ldw must be multiples of 16 bytes");
+  if (!ec::on_elements(type, y) ||
+      ((reinterpret_cast<uintptr_t>(x_scale) | reinterpret_cast<uintptr_t>(w_scale) |
+        reinterpret_cast<uintptr_t>(status)) & 3))
+    return ec::arg_error("ec_op_gemm_w8a8: a pointer is not aligned to its element");
   if (k > ec::kMaxK) return ec::unsupported("ec_op_gemm_w8a8: k > 131071");
   ec::W8A8Args a{};
   a.sx = x_scale;

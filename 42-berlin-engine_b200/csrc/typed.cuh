@@ -42,7 +42,10 @@ int with_type(int type, F f) {
 inline bool known_type(int type) {
   return type == EC_T_F32 || type == EC_T_BF16 || type == EC_T_F16;
 }
-inline size_t type_size(int type) { return type == EC_T_F32 ? 4 : 2; }
+// whether p (or NULL) is aligned to the type's element
+inline bool on_elements(int type, const void* p) {
+  return (reinterpret_cast<uintptr_t>(p) & (type == EC_T_F32 ? 3 : 1)) == 0;
+}
 
 inline int arg_error(const char* msg) {
   ec_set_last_error(msg);

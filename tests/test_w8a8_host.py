@@ -36,6 +36,12 @@ def test_norm_arguments(eng, changes):
     refused(eng, eng.lib().ec_op_add_rmsnorm_quant, NORM, changes, eng.EC_ERR_ARG)
 
 
+@pytest.mark.parametrize("changes", [
+    {1: P + 2}, {3: P + 1}, {5: P + 3}, {7: P + 1}, {13: P + 2}, {0: 1, 1: P + 1}, {0: 2, 5: P + 1}])
+def test_norm_element_alignment(eng, changes):
+    refused(eng, eng.lib().ec_op_add_rmsnorm_quant, NORM, changes, eng.EC_ERR_ARG)
+
+
 def test_norm_width(eng):
     n = 57345
     refused(eng, eng.lib().ec_op_add_rmsnorm_quant, NORM,
@@ -46,7 +52,8 @@ SILU = [0, P, P, 64, 2, 64, P, 64, P, None]
 
 
 @pytest.mark.parametrize("changes", [
-    {0: 3}, {1: None}, {2: None}, {3: 63}, {4: 0}, {5: 0}, {6: None}, {7: 63}, {8: None}])
+    {0: 3}, {1: None}, {2: None}, {3: 63}, {4: 0}, {5: 0}, {6: None}, {7: 63}, {8: None},
+    {1: P + 2}, {2: P + 1}, {0: 1, 2: P + 1}, {8: P + 1}])
 def test_silu_arguments(eng, changes):
     refused(eng, eng.lib().ec_op_silu_mul_quant, SILU, changes, eng.EC_ERR_ARG)
 
@@ -62,7 +69,8 @@ GEMM = [P, 64, P, P, 64, P, 0, P, 32, 32, 64, 2, None, None]
 
 @pytest.mark.parametrize("changes", [
     {0: None}, {2: None}, {3: None}, {5: None}, {7: None}, {6: 3}, {9: 0}, {10: 0}, {11: 0},
-    {1: 48}, {4: 48}, {8: 31}, {1: 72}, {4: 72}, {0: P + 8}, {3: P + 1}])
+    {1: 48}, {4: 48}, {8: 31}, {1: 72}, {4: 72}, {0: P + 8}, {3: P + 1},
+    {7: P + 2}, {6: 1, 7: P + 1}, {2: P + 2}, {5: P + 1}, {12: P + 2}])
 def test_gemm_arguments(eng, changes):
     refused(eng, eng.lib().ec_op_gemm_w8a8, GEMM, changes, eng.EC_ERR_ARG)
 
@@ -78,7 +86,8 @@ LOGP = [0, P, 64, 64, 2, P, 1.0, 4, P, P, P, P, None]
 
 @pytest.mark.parametrize("changes", [
     {0: 3}, {1: None}, {2: 63}, {3: 0}, {4: 0}, {5: None}, {8: None}, {6: 0.0}, {6: -1.0},
-    {6: float("nan")}, {6: float("inf")}, {6: 1e-38}, {7: -1}, {7: 65}, {10: None}, {11: None}])
+    {6: float("nan")}, {6: float("inf")}, {6: 1e-38}, {7: -1}, {7: 65}, {10: None}, {11: None},
+    {1: P + 2}, {0: 2, 1: P + 1}, {5: P + 2}, {8: P + 1}, {9: P + 2}, {10: P + 2}, {11: P + 2}])
 def test_logprob_arguments(eng, changes):
     refused(eng, eng.lib().ec_op_token_logprobs, LOGP, changes, eng.EC_ERR_ARG)
 
