@@ -28,7 +28,7 @@
 // weights); the MMA computes its 128 rows whatever R is, which costs
 // nothing there.  With C > 1 a cluster of C CTAs splits K: the partial
 // accumulators meet in distributed shared memory, each CTA finishing a part of
-// the token columns.  Warp 0 streams, warp 1 issues the MMAs, warps 2-5 drain
+// the token columns.  Warp 0 streams, warp 1 issues the MMAs, warps 2-9 drain
 // TMEM; two TMEM buffers let a tile's epilogue run under the next one's MMAs.
 #include <atomic>
 #include <mutex>
@@ -42,7 +42,8 @@ namespace {
 
 constexpr int kMaxK = 131071;  // 128 * 128 * k < 2^31
 constexpr int kKb = 128;       // K bytes of one TMA box: one 128-byte swizzle row
-constexpr int kThreads = 192;
+constexpr int kEpi = 8;        // epilogue warps: two for each quarter of TMEM's lanes
+constexpr int kThreads = 64 + 32 * kEpi;
 constexpr int kMaxStages = 24;
 constexpr int kHdr = 1024;
 constexpr int kSmemMax = 227 * 1024;
@@ -202,6 +203,35 @@ __device__ __forceinline__ float scaled(int acc, float sx, float sw) {
   return __fmul_rn(__fmul_rn((float)acc, sx), sw);
 }
 
+// An epilogue warp's columns of a tile of tn tokens: the first or the second
+// half of them, in blocks of 16.
+__device__ __forceinline__ void own_columns(int warp, int Tn, int tn, int* j0, int* j1) {
+  const int half = (Tn / 16 + 1) / 2 * 16;
+  *j0 = warp < 6 ? 0 : half;
+  *j1 = min(tn, warp < 6 ? half : Tn);
+}
+
+// Columns [j0, j1) of a tile -> y: this lane's channel (where `mine`), y and sx
+// at the tile's first token.  The next block's scales are on their way while
+// one is stored.
+template <typename T>
+__device__ __forceinline__ void store_columns(uint32_t ta, int j0, int j1, T* y, long ldy,
+                                              const float* sx, float sw, bool mine, int lane) {
+  float next = j0 < j1 ? sx[min(j0 + (lane & 15), j1 - 1)] : 0.0f;
+  y += (long)j0 * ldy;
+  for (; j0 < j1; j0 += 16) {
+    const float sxl = next;
+    int acc[16];
+    tmem_ld16(ta + j0, acc);
+    if (j0 + 16 < j1) next = sx[min(j0 + 16 + (lane & 15), j1 - 1)];
+#pragma unroll
+    for (int j = 0; j < 16; j++, y += ldy) {
+      const float s = __shfl_sync(0xffffffffu, sxl, j);
+      if (mine && j0 + j < j1) *y = from_f32<T>(scaled(acc[j], s, sw));
+    }
+  }
+}
+
 // ---------------------------------------------------------------- kernel --
 
 template <typename T>
@@ -234,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 2; i++) {
       mbar_init(&tfull[i], 1);
-      mbar_init(&tempty[i], 4);
+      mbar_init(&tempty[i], kEpi);
     }
     *failed = 0;
     fence_mbar_init();
@@ -344,17 +374,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) sw = __uint_as_float(0x7fc00000u);
       const int tn = min(a.Tn, a.nb - t0);
       T* y = static_cast<T*>(a.y) + (long)t0 * a.ldy + c;
-      for (int j0 = 0; j0 < tn; j0 += 16) {
-        const float sxl = a.sx[t0 + min(j0 + (lane & 15), tn - 1)];
-        int acc[16];
-        tmem_ld16(ta + j0, acc);
-#pragma unroll
-        for (int j = 0; j < 16; j++) {
-          const float sx = __shfl_sync(0xffffffffu, sxl, j);
-          if (mine && j0 + j < tn)
-            y[(long)(j0 + j) * a.ldy] = from_f32<T>(scaled(acc[j], sx, sw));
-        }
-      }
+      int j0, j1;
+      own_columns(warp, a.Tn, tn, &j0, &j1);
+      store_columns(ta, j0, j1, y, a.ldy, a.sx + t0, sw, mine, lane);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&tempty[buf]);
@@ -380,7 +402,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int p = 0; p < C; p++) st_peer(peer_addr(smem_u32(failed), p), 1);
       const uint32_t at = smem_u32(smem + kHdr) + (uint32_t)(rank * wc * 512 + r * 16);
       const uint32_t ta = tbase + ((uint32_t)(q * 32) << 16);
-      for (int j0 = 0; j0 < a.Tn; j0 += 16) {
+      int j0, j1;
+      own_columns(warp, a.Tn, a.Tn, &j0, &j1);
+      for (; j0 < j1; j0 += 16) {
         int acc[16];
         tmem_ld16(ta + j0, acc);
 #pragma unroll
@@ -400,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (*reinterpret_cast<volatile int*>(failed)) sw = __uint_as_float(0x7fc00000u);
       const int tt = t0 + rank * wc;
       T* y = static_cast<T*>(a.y) + (long)tt * a.ldy + c;
-      for (int j = 0; j < tn; j += 4) {
+      for (int j = warp < 6 ? 0 : 4; j < tn; j += 8) {
         int4 acc = part[j * 32];
         for (int p = 1; p < C; p++) {
           const int4 v = part[(p * wc + j) * 32];
@@ -462,7 +486,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 2; i++) {
       mbar_init(&tfull[i], 1);
-      mbar_init(&tempty[i], 8);  // the epilogue warps of both
+      mbar_init(&tempty[i], 2 * kEpi);  // the epilogue warps of both
     }
     *failed = 0;
     fence_mbar_init();
@@ -573,17 +597,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (!ok) sw = __uint_as_float(0x7fc00000u);
       const int tn = min(a.Tn, a.nb - t0);
       T* y = static_cast<T*>(a.y) + (long)t0 * a.ldy + c;
-      for (int j0 = 0; j0 < tn; j0 += 16) {
-        const float sxl = a.sx[t0 + min(j0 + (lane & 15), tn - 1)];
-        int acc[16];
-        tmem_ld16(ta + j0, acc);
-#pragma unroll
-        for (int j = 0; j < 16; j++) {
-          const float sx = __shfl_sync(0xffffffffu, sxl, j);
-          if (mine && j0 + j < tn)
-            y[(long)(j0 + j) * a.ldy] = from_f32<T>(scaled(acc[j], sx, sw));
-        }
-      }
+      int j0, j1;
+      own_columns(warp, a.Tn, tn, &j0, &j1);
+      store_columns(ta, j0, j1, y, a.ldy, a.sx + t0, sw, mine, lane);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_at(peer_addr(smem_u32(&tempty[buf]), 0));
