@@ -45,7 +45,8 @@ constexpr int kKb = 128;       // K bytes of one TMA box: one 128-byte swizzle r
 constexpr int kEpi = 8;        // epilogue warps: two for each quarter of TMEM's lanes
 constexpr int kThreads = 64 + 32 * kEpi;
 constexpr int kMaxStages = 24;
-constexpr int kHdr = 1024;
+constexpr int kHdr = 1024;     // barriers; from kScales on, the scales of up to 128 tokens
+constexpr int kScales = 512;
 constexpr int kSmemMax = 227 * 1024;
 constexpr int kMaxCluster = 8;
 constexpr int kAhead = 8;      // blocks of weights that a CTA brings to L2 before it may start
@@ -175,12 +176,13 @@ __device__ __forceinline__ void mma_i8_pair(uint32_t d, uint64_t a, uint64_t b, 
       : "memory");
 }
 
-// arrives on `bar` of both CTAs once the MMAs issued so far have ended
-__device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
+// arrives on `bar` of both CTAs (ranks lead, lead + 1) once the MMAs issued so
+// far have ended
+__device__ __forceinline__ void mma_commit_pair(uint64_t* bar, uint32_t lead) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
       "[%0], %1;" ::"r"(smem_u32(bar)),
-      "h"((uint16_t)3)
+      "h"((uint16_t)(3u << lead))
       : "memory");
 }
 
@@ -231,6 +233,51 @@ __device__ __forceinline__ void store_columns(uint32_t ta, int j0, int j1, T* y,
     }
   }
 }
+
+// The join of a K split over C CTAs (ranks offset, offset + stride, ... of the
+// cluster; this one is number `me`): each finishes wc of the tile's columns.
+// An exchange buffer is [CTA][column / 4][128 channels][4].
+__device__ __forceinline__ void send_columns(uint32_t exchange, uint32_t ta, int warp, int r,
+                                             int Tn, int wc, int me, int stride, int offset) {
+  const uint32_t at = exchange + (uint32_t)(me * wc * 512 + r * 16);
+  int j0, j1;
+  own_columns(warp, Tn, Tn, &j0, &j1);
+  for (; j0 < j1; j0 += 16) {
+    int acc[16];
+    tmem_ld16(ta + j0, acc);
+#pragma unroll
+    for (int j = 0; j < 16; j += 4) {
+      const int owner = (j0 + j) / wc, col = (j0 + j) - owner * wc;
+      st_peer4(peer_addr(at, owner * stride + offset) + col * 512, acc + j);
+    }
+  }
+}
+
+// Its columns' sums -> y (this CTA's first column and this lane's channel), tn
+// of them within the tokens; sxs: their scales in shared memory.
+template <typename T>
+__device__ __forceinline__ void finish_columns(const uint8_t* exchange, int C, int wc, int warp,
+                                               int r, int tn, T* y, long ldy, const float* sxs,
+                                               float sw) {
+  const int4* part = reinterpret_cast<const int4*>(exchange) + r;
+  for (int j = warp < 6 ? 0 : 4; j < tn; j += 8) {
+    int4 acc = part[j * 32];
+    for (int p = 1; p < C; p++) {
+      const int4 v = part[(p * wc + j) * 32];
+      acc.x += v.x;
+      acc.y += v.y;
+      acc.z += v.z;
+      acc.w += v.w;
+    }
+    const int sum[4] = {acc.x, acc.y, acc.z, acc.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (j + i < tn) y[(long)(j + i) * ldy] = from_f32<T>(scaled(sum[i], sxs[j + i], sw));
+  }
+}
+
+// columns that each of C CTAs finishes
+__host__ __device__ inline int join_width(int Tn, int C) { return ((Tn + C - 1) / C + 3) & ~3; }
 
 // ---------------------------------------------------------------- kernel --
 
@@ -386,59 +433,32 @@ __global__ void __launch_bounds__(kThreads, 1)
     // One tile per cluster: every CTA sends each other its partial sums of the
     // columns that the other finishes, into its exchange buffer [CTA of the
     // cluster][token columns / 4][128 channels][4].
-    const int wc = ((a.Tn + C - 1) / C + 3) & ~3;  // token columns each CTA finishes
-    const int q = warp & 3, r = q * 32 + lane;
-    const int c = first / a.nt * a.R + r, t0 = first % a.nt * a.Tn;
+    const int wc = join_width(a.Tn, C), q = warp & 3, r = q * 32 + lane;
+    const int c = first / a.nt * a.R + r, t0 = first % a.nt * a.Tn, tt = t0 + rank * wc;
     const bool mine = warp >= 2 && r < a.R && c < a.m;
+    float* sxs = reinterpret_cast<float*>(smem + kScales);
     float sw = 0.0f;
     cluster_wait();  // every CTA of the cluster runs
     if (warp >= 2) {
       pdl_wait();
       if (mine) sw = a.sw[c];
+      if (tid - 64 < wc && tt + tid - 64 < a.nb) sxs[tid - 64] = a.sx[tt + tid - 64];
       ok = mbar_wait(&tfull[0], 0, a.status);
       tc_fence_after();
       ok = ok && *reinterpret_cast<volatile int*>(failed) == 0;
       if (!ok && lane == 0)
         for (int p = 0; p < C; p++) st_peer(peer_addr(smem_u32(failed), p), 1);
-      const uint32_t at = smem_u32(smem + kHdr) + (uint32_t)(rank * wc * 512 + r * 16);
-      const uint32_t ta = tbase + ((uint32_t)(q * 32) << 16);
-      int j0, j1;
-      own_columns(warp, a.Tn, a.Tn, &j0, &j1);
-      for (; j0 < j1; j0 += 16) {
-        int acc[16];
-        tmem_ld16(ta + j0, acc);
-#pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-          const int owner = (j0 + j) / wc, col = (j0 + j) - owner * wc;
-          st_peer4(peer_addr(at, owner) + col * 512, acc + j);
-        }
-      }
+      send_columns(smem_u32(smem + kHdr), tbase + ((uint32_t)(q * 32) << 16), warp, r, a.Tn, wc,
+                   rank, 1, 0);
       tc_fence_before();
     }
     __syncwarp();
     cluster_arrive();
     cluster_wait();
     if (mine) {
-      const int tn = min(min(a.Tn, a.nb - t0), (rank + 1) * wc) - rank * wc;
-      const int4* part = reinterpret_cast<const int4*>(smem + kHdr) + r;
       if (*reinterpret_cast<volatile int*>(failed)) sw = __uint_as_float(0x7fc00000u);
-      const int tt = t0 + rank * wc;
-      T* y = static_cast<T*>(a.y) + (long)tt * a.ldy + c;
-      for (int j = warp < 6 ? 0 : 4; j < tn; j += 8) {
-        int4 acc = part[j * 32];
-        for (int p = 1; p < C; p++) {
-          const int4 v = part[(p * wc + j) * 32];
-          acc.x += v.x;
-          acc.y += v.y;
-          acc.z += v.z;
-          acc.w += v.w;
-        }
-        const int sum[4] = {acc.x, acc.y, acc.z, acc.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-          if (j + i < tn)
-            y[(long)(j + i) * a.ldy] = from_f32<T>(scaled(sum[i], a.sx[tt + j + i], sw));
-      }
+      finish_columns(smem + kHdr, C, wc, warp, r, min(min(a.Tn, a.nb - t0) - rank * wc, wc),
+                     static_cast<T*>(a.y) + (long)tt * a.ldy + c, a.ldy, sxs, sw);
     }
   }
   tc_fence_before();
@@ -462,7 +482,7 @@ __device__ __forceinline__ void tile_at(int tile, int mt, int nt, int* c, int* t
 }
 
 template <typename T>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, 1)
     gemm_w8a8_pair_kernel(const __grid_constant__ CUtensorMap mx,
                           const __grid_constant__ CUtensorMap mw, const W8A8Args a) {
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -474,8 +494,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   int* failed = reinterpret_cast<int*>(tslot + 1);
   uint8_t* stg = smem + kHdr;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t rank = cluster_rank();
-  const int first = blockIdx.x >> 1, step = gridDim.x >> 1, tiles = a.mt * a.nt;
+  const int C = a.C;  // pairs that share a tile's K
+  const uint32_t crank = cluster_rank(), rank = crank & 1, lead = crank & ~1u;
+  const int me = (int)(crank >> 1);
+  const int first = blockIdx.x / (2 * C), step = gridDim.x / (2 * C), tiles = a.mt * a.nt;
+  const int c0 = (int)((long)me * a.chunks / C), c1 = (int)((long)(me + 1) * a.chunks / C);
   const int half = a.Tn / 2;  // tokens of this CTA's share
   const uint32_t wbytes = 128 * kKb, stage = wbytes + (uint32_t)half * kKb;
 
@@ -514,7 +537,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (first < tiles) {
         int ct, tt;
         tile_at(first, a.mt, a.nt, &ct, &tt);
-        for (int i = 0; i < min(a.chunks, kAhead); i++)
+        for (int i = c0; i < min(c1, c0 + kAhead); i++)
           prefetch_2d(&mw, i * kKb, ct * 256 + (int)rank * 128);
       }
       pdl_wait();
@@ -524,11 +547,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         int ct, tt;
         tile_at(tile, a.mt, a.nt, &ct, &tt);
         const int c = ct * 256 + (int)rank * 128, t = tt * a.Tn + (int)rank * half;
-        for (int i = 0; i < a.chunks; i++, u++) {
+        for (int i = c0; i < c1; i++, u++) {
           ok = mbar_wait(&empty[s], phase, a.status);
           if (!ok) break;
           if (rank == 0) mbar_expect_tx(&full[s], 2 * stage);
-          const uint32_t bar = peer_addr(smem_u32(&full[s]), 0);
+          const uint32_t bar = peer_addr(smem_u32(&full[s]), lead);
           const uint32_t dst = smem_u32(stg) + s * stage;
           tma_2d_pair(dst, &mw, i * kKb, c, bar);
           tma_2d_pair(dst + wbytes, &mx, i * kKb, t, bar);
@@ -554,7 +577,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (n >= 2) ok = mbar_wait(&tempty[buf], (uint32_t)(((n >> 1) - 1) & 1), a.status);
         tc_fence_after();
         const uint32_t d = tbase + (uint32_t)(buf * 256);
-        for (int i = 0; i < a.chunks && ok; i++) {
+        for (int i = c0; i < c1 && ok; i++) {
           ok = mbar_wait(&full[s], phase, a.status);
           if (!ok) break;
           tc_fence_after();
@@ -562,23 +585,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const uint64_t da = sw128_desc(src), db = sw128_desc(src + wbytes);
 #pragma unroll
           for (int j = 0; j < kKb / 32; j++)
-            mma_i8_pair(d, da + 2 * j, db + 2 * j, idesc, (i > 0 || j > 0) ? 1u : 0u);
-          mma_commit_pair(&empty[s]);
+            mma_i8_pair(d, da + 2 * j, db + 2 * j, idesc, (i > c0 || j > 0) ? 1u : 0u);
+          mma_commit_pair(&empty[s], lead);
           if (++s == a.S) {
             s = 0;
             phase ^= 1;
           }
         }
         if (!ok) {
-          st_peer(peer_addr(smem_u32(failed), 0), 1);
-          st_peer(peer_addr(smem_u32(failed), 1), 1);
+          for (int p = 0; p < 2 * C; p++) st_peer(peer_addr(smem_u32(failed), p), 1);
           asm volatile("fence.acq_rel.cluster;" ::: "memory");
         }
-        mma_commit_pair(&tfull[buf]);
+        mma_commit_pair(&tfull[buf], lead);
       }
     }
     __syncwarp();
-  } else {
+  } else if (C == 1) {
     // ----------------------------------------------------------- epilogue
     const int q = warp & 3, r = q * 32 + lane;
     pdl_wait();
@@ -602,7 +624,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       store_columns(ta, j0, j1, y, a.ldy, a.sx + t0, sw, mine, lane);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) arrive_at(peer_addr(smem_u32(&tempty[buf]), 0));
+      if (lane == 0) arrive_at(peer_addr(smem_u32(&tempty[buf]), lead));
+    }
+  }
+  if (C > 1) {
+    // One tile per cluster.  The stages become the exchange buffer once all
+    // MMAs of the cluster have read them.
+    int ct, tt0;
+    tile_at(first, a.mt, a.nt, &ct, &tt0);
+    const int wc = join_width(a.Tn, C), q = warp & 3, r = q * 32 + lane;
+    const int c = ct * 256 + (int)rank * 128 + r, t0 = tt0 * a.Tn, tt = t0 + me * wc;
+    const bool mine = warp >= 2 && c < a.m;
+    float* sxs = reinterpret_cast<float*>(smem + kScales);
+    float sw = 0.0f;
+    if (warp >= 2) {
+      pdl_wait();
+      if (mine) sw = a.sw[c];
+      if (tid - 64 < wc && tt + tid - 64 < a.nb) sxs[tid - 64] = a.sx[tt + tid - 64];
+      ok = mbar_wait(&tfull[0], 0, a.status);
+      tc_fence_after();
+      if (!ok && lane == 0)
+        for (int p = 0; p < 2 * C; p++) st_peer(peer_addr(smem_u32(failed), p), 1);
+    }
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    if (warp >= 2) {
+      send_columns(smem_u32(stg), tbase + ((uint32_t)(q * 32) << 16), warp, r, a.Tn, wc, me, 2,
+                   (int)rank);
+      tc_fence_before();
+    }
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    if (mine) {
+      if (*reinterpret_cast<volatile int*>(failed)) sw = __uint_as_float(0x7fc00000u);
+      finish_columns(stg, C, wc, warp, r, min(min(a.Tn, a.nb - t0) - me * wc, wc),
+                     static_cast<T*>(a.y) + (long)tt * a.ldy + c, a.ldy, sxs, sw);
     }
   }
   tc_fence_before();
@@ -700,7 +758,7 @@ cudaError_t device_slots(const Slots** out) {
 }
 
 struct Plan {
-  int R, Tn, C, ks;  // R = 256: a pair's tile
+  int R, Tn, C, ks;  // R = 256: a pair's tile, K split over C pairs; else over C CTAs
   float cost;
 };
 
@@ -716,10 +774,11 @@ inline int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 float plan_cost(const Plan& p, int m, int chunks, int nb, const Slots& at_once) {
   const long cols = ceil_div(nb, p.Tn);
   if (p.R == 256) {
-    const int rounds = ceil_div(ceil_div(m, 256) * cols, at_once.clusters[2]);
+    const int rounds = ceil_div(ceil_div(m, 256) * cols, at_once.clusters[2 * p.C]);
     const float copy = (128 + p.Tn / 2) * kKb / 53.0f;
     const float mma = 4.0f * fmaxf(41.0f, 0.5f * p.Tn);
-    return rounds * (chunks * fmaxf(fmaxf(copy, mma), 250.0f) + 2.2f * p.Tn);
+    return rounds * (ceil_div(chunks, p.C) * fmaxf(fmaxf(copy, mma), 250.0f) + 2.2f * p.Tn) +
+           (p.C > 1 ? 1500.0f + 24.0f * p.Tn : 0.0f);
   }
   const int rounds = ceil_div(ceil_div(m, p.R) * cols, at_once.clusters[p.C]);
   const int share = ceil_div(chunks, p.C);
@@ -736,9 +795,13 @@ Plan plan_tiles(int m, int chunks, int nb, const Slots& at_once) {
     if (p.cost < best.cost) best = p;
   };
   // pairs: 256 channels x Tn tokens
-  if (at_once.clusters[2] > 0)
-    for (int nt = ceil_div(nb, 256), i = 0; i < 6; nt++, i++)
-      offer(Plan{256, ceil_div(ceil_div(nb, nt), 32) * 32, 2, 1, 0});
+  for (int nt = ceil_div(nb, 256), i = 0; i < 6; nt++, i++) {
+    const int Tn = ceil_div(ceil_div(nb, nt), 32) * 32;
+    const long tiles = (long)ceil_div(m, 256) * ceil_div(nb, Tn);
+    for (int C = 1; C <= 4 && C <= chunks; C++)
+      if (at_once.clusters[2 * C] > 0 && (C == 1 || tiles <= at_once.clusters[2 * C]))
+        offer(Plan{256, Tn, C, 1, 0});
+  }
   // single CTAs, or clusters that split K
   const int splits[5] = {ceil_div(nb, 256), 2 * ceil_div(nb, 256), ceil_div(nb, 128),
                          ceil_div(nb, 64), ceil_div(nb, 32)};
@@ -793,16 +856,19 @@ int launch_pair(const int8_t* x, long ldx, const int8_t* w, long ldw, int k, W8A
   }
   const int tiles = a.mt * a.nt;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2 * (tiles < slots ? tiles : slots));
+  cfg.gridDim = dim3(2 * a.C * (a.C > 1 || tiles < slots ? tiles : slots));
   cfg.blockDim = dim3(kThreads);
   const size_t smem = kHdr + (size_t)a.S * stage;
   cfg.dynamicSmemBytes = smem > 120 * 1024 ? smem : 120 * 1024;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)(2 * a.C);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   EC_CUDA_TRY(cudaLaunchKernelEx(&cfg, gemm_w8a8_pair_kernel<T>, mx, mw, a));
   return EC_OK;
 }
@@ -830,8 +896,7 @@ int launch(const int8_t* x, long ldx, const int8_t* w, long ldw, int k, W8A8Args
   a.ks = p.ks;
   // the last block's MMA reads 128 rows from its weights on
   const int slack = 128 * kKb;
-  const int finish = ((a.Tn + a.C - 1) / a.C + 3) & ~3;  // columns a CTA finishes
-  a.exchange = a.C > 1 ? (a.C * finish * 512 + 1023) & ~1023 : 0;
+  a.exchange = a.C > 1 ? (a.C * join_width(a.Tn, a.C) * 512 + 1023) & ~1023 : 0;
   a.S = (kSmemMax - kHdr - slack - a.exchange) / (block * a.ks);
   if (a.S > kMaxStages) a.S = kMaxStages;
   const size_t smem = kHdr + a.exchange + (size_t)a.S * block * a.ks + slack;

@@ -82,7 +82,8 @@ SHAPES = [  # tokens, channels, k
     (65, 257, 4095), (80, 300, 300), (127, 129, 2048), (128, 256, 256), (129, 1000, 640),
     (200, 4096, 512), (255, 255, 255), (256, 256, 4096), (257, 513, 1025), (384, 2000, 384),
     (512, 512, 512), (517, 5003, 1433), (700, 128, 8192), (1000, 1000, 100), (1024, 6144, 256),
-    (2048, 4096, 512), (2049, 700, 129), (5000, 64, 64), (1, 1, 131071), (300, 1, 70), (1, 128256, 512)]
+    (2048, 4096, 512), (2049, 700, 129), (5000, 64, 64), (1, 1, 131071), (513, 200, 131071),
+    (256, 1000, 20000), (160, 512, 30000), (1066, 256, 11648), (90, 1300, 17217), (225, 3000, 9001), (300, 1, 70), (1, 128256, 512)]
 
 
 @pytest.mark.parametrize("kind", TYPES)
