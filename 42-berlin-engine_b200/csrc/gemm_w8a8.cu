@@ -28,7 +28,7 @@
 // weights); the MMA computes its 128 rows whatever R is, which costs
 // nothing there.  With C > 1 a cluster of C CTAs splits K: the partial
 // accumulators meet in distributed shared memory, each CTA finishing a part of
-// the token columns.  Warp 0 streams, warp 1 issues the MMAs, warps 2-9 drain
+// the token columns.  Warp 0 streams, warp 1 issues the MMAs, the others drain
 // TMEM; two TMEM buffers let a tile's epilogue run under the next one's MMAs.
 #include <atomic>
 #include <mutex>
@@ -42,7 +42,7 @@ namespace {
 
 constexpr int kMaxK = 131071;  // 128 * 128 * k < 2^31
 constexpr int kKb = 128;       // K bytes of one TMA box: one 128-byte swizzle row
-constexpr int kEpi = 8;        // epilogue warps: two for each quarter of TMEM's lanes
+constexpr int kEpi = 16;       // epilogue warps: four for each quarter of TMEM's lanes
 constexpr int kThreads = 64 + 32 * kEpi;
 constexpr int kMaxStages = 24;
 constexpr int kHdr = 1024;     // barriers; from kScales on, the scales of up to 128 tokens
@@ -106,7 +106,11 @@ __device__ __forceinline__ void tc_fence_before() {
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 }
 
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, int* r) {
+__device__ __forceinline__ void tmem_wait() {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+// 16 columns of this warp's lanes; the registers hold them after tmem_wait
+__device__ __forceinline__ void tmem_start16(uint32_t taddr, int* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
       "%11, %12, %13, %14, %15}, [%16];"
@@ -114,7 +118,10 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, int* r) {
         "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
         "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, int* r) {
+  tmem_start16(taddr, r);
+  tmem_wait();
 }
 
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y,
@@ -196,8 +203,11 @@ __device__ __forceinline__ void tma_2d_pair(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
+// An arrival that hands over TMEM columns only (after tcgen05.wait::ld and
+// tcgen05.fence::before_thread_sync): a releasing one would first wait for
+// the tile's stores to y.
 __device__ __forceinline__ void arrive_at(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
                : "memory");
 }
 
@@ -205,32 +215,64 @@ __device__ __forceinline__ float scaled(int acc, float sx, float sw) {
   return __fmul_rn(__fmul_rn((float)acc, sx), sw);
 }
 
-// An epilogue warp's columns of a tile of tn tokens: the first or the second
-// half of them, in blocks of 16.
+// An epilogue warp's columns of a tile of tn tokens: its share of them, in
+// blocks of 16.
 __device__ __forceinline__ void own_columns(int warp, int Tn, int tn, int* j0, int* j1) {
-  const int half = (Tn / 16 + 1) / 2 * 16;
-  *j0 = warp < 6 ? 0 : half;
-  *j1 = min(tn, warp < 6 ? half : Tn);
+  constexpr int kParts = kEpi / 4;
+  const int part = (warp - 2) / 4, blocks = Tn / 16;
+  *j0 = blocks * part / kParts * 16;
+  *j1 = min(tn, blocks * (part + 1) / kParts * 16);
+}
+
+// the scales of columns j .. j + 15 (those below j1), one a lane
+__device__ __forceinline__ float block_scales(const float* sx, int j, int j1, int lane) {
+  return j < j1 ? sx[min(j + (lane & 15), j1 - 1)] : 0.0f;
+}
+
+// A block of 16 columns (the first `count` of them) -> y
+template <typename T>
+__device__ __forceinline__ void store_block(const int* acc, int count, T*& y, long ldy, float sxl,
+                                            float sw, bool mine) {
+  const uint64_t sw2 = pack2(__float_as_uint(sw), __float_as_uint(sw));
+#pragma unroll
+  for (int j = 0; j < 16; j += 2) {
+    const float s0 = __shfl_sync(0xffffffffu, sxl, j), s1 = __shfl_sync(0xffffffffu, sxl, j + 1);
+    const uint64_t v =
+        mul2(mul2(pack2(__float_as_uint((float)acc[j]), __float_as_uint((float)acc[j + 1])),
+                  pack2(__float_as_uint(s0), __float_as_uint(s1))), sw2);
+    if (mine && j < count) *y = from_f32<T>(lo_f(v));
+    y += ldy;
+    if (mine && j + 1 < count) *y = from_f32<T>(hi_f(v));
+    y += ldy;
+  }
 }
 
 // Columns [j0, j1) of a tile -> y: this lane's channel (where `mine`), y and sx
-// at the tile's first token.  The next block's scales are on their way while
-// one is stored.
+// at the tile's first token, `scales` block_scales of j0.  While a block is
+// scaled and stored the next one's sums and scales are on their way.
 template <typename T>
 __device__ __forceinline__ void store_columns(uint32_t ta, int j0, int j1, T* y, long ldy,
-                                              const float* sx, float sw, bool mine, int lane) {
-  float next = j0 < j1 ? sx[min(j0 + (lane & 15), j1 - 1)] : 0.0f;
+                                              const float* sx, float scales, float sw, bool mine,
+                                              int lane) {
+  if (j0 >= j1) return;
   y += (long)j0 * ldy;
-  for (; j0 < j1; j0 += 16) {
-    const float sxl = next;
-    int acc[16];
-    tmem_ld16(ta + j0, acc);
-    if (j0 + 16 < j1) next = sx[min(j0 + 16 + (lane & 15), j1 - 1)];
-#pragma unroll
-    for (int j = 0; j < 16; j++, y += ldy) {
-      const float s = __shfl_sync(0xffffffffu, sxl, j);
-      if (mine && j0 + j < j1) *y = from_f32<T>(scaled(acc[j], s, sw));
-    }
+  int even[16], odd[16];
+  tmem_start16(ta + j0, even);
+  while (true) {
+    tmem_wait();
+    float sxl = scales;
+    scales = block_scales(sx, j0 + 16, j1, lane);
+    if (j0 + 16 < j1) tmem_start16(ta + j0 + 16, odd);
+    store_block(even, j1 - j0, y, ldy, sxl, sw, mine);
+    j0 += 16;
+    if (j0 >= j1) break;
+    tmem_wait();
+    sxl = scales;
+    scales = block_scales(sx, j0 + 16, j1, lane);
+    if (j0 + 16 < j1) tmem_start16(ta + j0 + 16, even);
+    store_block(odd, j1 - j0, y, ldy, sxl, sw, mine);
+    j0 += 16;
+    if (j0 >= j1) break;
   }
 }
 
@@ -260,7 +302,7 @@ __device__ __forceinline__ void finish_columns(const uint8_t* exchange, int C, i
                                                int r, int tn, T* y, long ldy, const float* sxs,
                                                float sw) {
   const int4* part = reinterpret_cast<const int4*>(exchange) + r;
-  for (int j = warp < 6 ? 0 : 4; j < tn; j += 8) {
+  for (int j = (warp - 2) / 4 * 4; j < tn; j += kEpi) {
     int4 acc = part[j * 32];
     for (int p = 1; p < C; p++) {
       const int4 v = part[(p * wc + j) * 32];
@@ -413,20 +455,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int c = tile / a.nt * a.R + r, t0 = tile % a.nt * a.Tn;
       const bool mine = r < a.R && c < a.m;
       const int buf = n & 1;
+      const int tn = min(a.Tn, a.nb - t0);
+      int j0, j1;
+      own_columns(warp, a.Tn, tn, &j0, &j1);
       float sw = mine ? a.sw[c] : 0.0f;
+      const float scales = block_scales(a.sx + t0, j0, j1, lane);
       ok = ok && mbar_wait(&tfull[buf], (uint32_t)((n >> 1) & 1), a.status) &&
            *reinterpret_cast<volatile int*>(failed) == 0;
       tc_fence_after();
       const uint32_t ta = tbase + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * (tcols >> 1));
       if (!ok) sw = __uint_as_float(0x7fc00000u);
-      const int tn = min(a.Tn, a.nb - t0);
       T* y = static_cast<T*>(a.y) + (long)t0 * a.ldy + c;
-      int j0, j1;
-      own_columns(warp, a.Tn, tn, &j0, &j1);
-      store_columns(ta, j0, j1, y, a.ldy, a.sx + t0, sw, mine, lane);
+      store_columns(ta, j0, j1, y, a.ldy, a.sx + t0, scales, sw, mine, lane);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&tempty[buf]);
+      if (lane == 0) arrive_at(smem_u32(&tempty[buf]));
     }
   }
   if (C > 1) {
@@ -611,17 +654,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int c = ct * 256 + (int)rank * 128 + r, t0 = tt * a.Tn;
       const bool mine = c < a.m;
       const int buf = n & 1;
+      const int tn = min(a.Tn, a.nb - t0);
+      int j0, j1;
+      own_columns(warp, a.Tn, tn, &j0, &j1);
       float sw = mine ? a.sw[c] : 0.0f;
+      const float scales = block_scales(a.sx + t0, j0, j1, lane);
       ok = ok && mbar_wait(&tfull[buf], (uint32_t)((n >> 1) & 1), a.status) &&
            *reinterpret_cast<volatile int*>(failed) == 0;
       tc_fence_after();
       const uint32_t ta = tbase + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * 256);
       if (!ok) sw = __uint_as_float(0x7fc00000u);
-      const int tn = min(a.Tn, a.nb - t0);
       T* y = static_cast<T*>(a.y) + (long)t0 * a.ldy + c;
-      int j0, j1;
-      own_columns(warp, a.Tn, tn, &j0, &j1);
-      store_columns(ta, j0, j1, y, a.ldy, a.sx + t0, sw, mine, lane);
+      store_columns(ta, j0, j1, y, a.ldy, a.sx + t0, scales, sw, mine, lane);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_at(peer_addr(smem_u32(&tempty[buf]), lead));
@@ -817,6 +861,8 @@ Plan plan_tiles(int m, int chunks, int nb, const Slots& at_once) {
         // the most tiles that these rounds hold, then the channels each needs
         const int mt = (int)((long)(q + more) * slots / cols);
         int R = ceil_div(m, mt);
+        // whole 32-byte sectors of y, once they count
+        if (nb >= 32) R = (R + 15) / 16 * 16;
         R = R > 128 ? 128 : R < 8 ? (m < 8 ? m : 8) : R;
         const int block = (Tn + (R + 7) / 8 * 8) * kKb, share = ceil_div(chunks, C);
         for (int ks = 1; ks <= 8 && ks <= share && block * ks <= 90000; ks *= 2) {
