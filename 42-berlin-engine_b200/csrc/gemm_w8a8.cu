@@ -813,23 +813,23 @@ inline int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 // cycles however few tokens there are) and the issue of a stage, then the
 // epilogue and the join of a split K.  The constants are fitted to the times
 // of all plans of 88 shapes (1-7378 tokens, 65-128256 channels, k 64-27584):
-// the plan chosen by this model is within 1% of the best one's time in the
-// mean, 10% at most.
+// the plan chosen by this model is within 1.4% of the best one's time in the
+// mean, 20% at most (a call of 3.4 us).
 float plan_cost(const Plan& p, int m, int chunks, int nb, const Slots& at_once) {
   const long cols = ceil_div(nb, p.Tn);
+  const int share = ceil_div(chunks, p.C);
   if (p.R == 256) {
     const int rounds = ceil_div(ceil_div(m, 256) * cols, at_once.clusters[2 * p.C]);
-    const float copy = (128 + p.Tn / 2) * kKb / 53.0f;
+    const float copy = (128 + p.Tn / 2) * kKb / 67.0f;
     const float mma = 4.0f * fmaxf(41.0f, 0.5f * p.Tn);
-    return rounds * (ceil_div(chunks, p.C) * fmaxf(fmaxf(copy, mma), 250.0f) + 2.2f * p.Tn) +
-           (p.C > 1 ? 1500.0f + 24.0f * p.Tn : 0.0f);
+    return 1280.0f + rounds * (share * fmaxf(fmaxf(copy, mma), 173.0f) + 16.0f * p.Tn + 196.0f) +
+           (p.C > 1 ? 2290.0f + 35.0f * p.Tn : 0.0f);
   }
   const int rounds = ceil_div(ceil_div(m, p.R) * cols, at_once.clusters[p.C]);
-  const int share = ceil_div(chunks, p.C);
-  const float copy = (p.R + p.Tn) * kKb / 70.0f;
-  const float mma = 4.0f * fmaxf(50.0f, 0.5f * p.Tn);
-  return rounds * (share * fmaxf(copy, mma) + ceil_div(share, p.ks) * 254.0f + 14.0f * p.Tn) +
-         (p.ks < share ? p.ks : share) * mma * 0.41f + (p.C > 1 ? 400.0f + 24.0f * p.Tn : 0.0f);
+  const float copy = (p.R + p.Tn) * kKb / 64.0f;
+  const float mma = 4.0f * fmaxf(52.0f, 0.5f * p.Tn);
+  return rounds * (share * fmaxf(copy, mma) + ceil_div(share, p.ks) * 175.0f + 9.2f * p.Tn + 223.0f) +
+         (p.ks < share ? p.ks : share) * mma * 0.2f + (p.C > 1 ? 876.0f + 40.0f * p.Tn : 0.0f);
 }
 
 Plan plan_tiles(int m, int chunks, int nb, const Slots& at_once) {
