@@ -107,7 +107,8 @@ __device__ __forceinline__ float max_abs(float m, uint64_t y) {
 // The statistics of a block: one barrier, then every warp joins the warps'
 // values in the same tree.  The sum of squares is f32 inside a 16-byte piece
 // of the row and f64 over the pieces: rounded to f32 it does not depend on how
-// many threads share the row, so a row's 8-bit values are the same in any batch.
+// many threads share the row, so the 8-bit values of a row of whole pieces are the
+// same in any batch.
 __device__ __forceinline__ float block_sum(double v, double* red) {
   const int lane = threadIdx.x & 31, warps = (blockDim.x + 31) >> 5;
 #pragma unroll
@@ -132,7 +133,7 @@ __device__ __forceinline__ unsigned block_max(unsigned v, unsigned* red) {
 // gives NaN, not a silent row of zeros.
 __device__ __forceinline__ float norm_factor(float ss, float inv_n, float eps) {
   float r;
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fmaf_rn(ss, inv_n, eps)));
+  asm("rsqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(__fmaf_rn(ss, inv_n, eps)));
   return ss == INFINITY ? __uint_as_float(0x7fc00000u) : r;
 }
 
@@ -396,8 +397,9 @@ __device__ __forceinline__ void walk_rows(uint8_t* smem, const T* a, long lda, c
   const P part{n, 0};
   const size_t room = P::room(n);
   const int step = gridDim.x;
-  int row = blockIdx.x, at = 0;
-  auto stage = [&](int r, int which) {
+  long row = blockIdx.x;
+  int at = 0;
+  auto stage = [&](long r, int which) {
     if (r < rows) {
       part.stage(smem + which * 2 * room, a + r * lda, 0);
       if (b) part.stage(smem + (which * 2 + 1) * room, b + r * ldb, 1);
@@ -646,7 +648,8 @@ int rows_launch(Args a, bool vec, Shape s, size_t extra, void (*wide)(Args), Pic
   // Alone on its SM a CTA walks all its rows; else a few, so that the SMs'
   // different speeds even out.
   const bool alone = kMaxThr / threads < 2 || kStageMax / (smem + 1024) < 2;
-  const int grid = alone ? (a.rows < 148 ? a.rows : 148) : (a.rows + s.rows_per_cta - 1) / s.rows_per_cta;
+  const int grid = alone ? (a.rows < 148 ? a.rows : 148)
+                         : (a.rows + s.rows_per_cta - 1) / s.rows_per_cta;
   return launch(pick(s.f, vec), a, grid, threads, smem, st);
 }
 
@@ -702,7 +705,8 @@ extern "C" int ec_op_add_rmsnorm_quant(int type, const void* x, int64_t ldx, con
     return ec::arg_error("ec_op_add_rmsnorm_quant: a pointer is not aligned to its element");
   if (ldx < n || ldq < n || (residual && ldr < n) || (sum_out && lds < n))
     return ec::arg_error("ec_op_add_rmsnorm_quant: a row stride is shorter than the row");
-  if (n > ec::kMaxN) return ec::unsupported("ec_op_add_rmsnorm_quant: n > 57344");
+  if (n > ec::kMaxN || rows > ec::kMaxRows)
+    return ec::unsupported("ec_op_add_rmsnorm_quant: n > 57344 or rows > 2^30");
   const ec::NormArgs a{x, residual, sum_out, (long)ldx, (long)ldr, (long)lds, w, eps, 1.0f / (float)n, rows, n, 1,
                        q, (long)ldq, scales};
   return ec::with_type(type, [&](auto t) {
@@ -721,7 +725,8 @@ extern "C" int ec_op_silu_mul_quant(int type, const void* gate, const void* up, 
     return ec::arg_error("ec_op_silu_mul_quant: a pointer is not aligned to its element");
   if (ld < n || ldq < n)
     return ec::arg_error("ec_op_silu_mul_quant: a row stride is shorter than the row");
-  if (n > ec::kMaxN) return ec::unsupported("ec_op_silu_mul_quant: n > 57344");
+  if (n > ec::kMaxN || rows > ec::kMaxRows)
+    return ec::unsupported("ec_op_silu_mul_quant: n > 57344 or rows > 2^30");
   const ec::SiluArgs a{gate, up, (long)ld, rows, n, 1, q, (long)ldq, scales};
   return ec::with_type(type, [&](auto t) {
     return ec::silu_rows<decltype(t)>(a, static_cast<cudaStream_t>(stream));

@@ -990,7 +990,8 @@ extern "C" int ec_op_gemm_w8a8(const int8_t* x, int64_t ldx, const float* x_scal
       ((reinterpret_cast<uintptr_t>(x_scale) | reinterpret_cast<uintptr_t>(w_scale) |
         reinterpret_cast<uintptr_t>(status)) & 3))
     return ec::arg_error("ec_op_gemm_w8a8: a pointer is not aligned to its element");
-  if (k > ec::kMaxK) return ec::unsupported("ec_op_gemm_w8a8: k > 131071");
+  if (k > ec::kMaxK || m > ec::kMaxRows || nb > ec::kMaxRows)
+    return ec::unsupported("ec_op_gemm_w8a8: k > 131071, or m or nb > 2^30");
   ec::W8A8Args a{};
   a.sx = x_scale;
   a.sw = w_scale;

@@ -571,7 +571,8 @@ extern "C" int ec_op_token_logprobs(int type, const void* logits, int64_t ld, in
   if (!tokens != !logprob || top_k < 0 || top_k > n || (top_k > 0 && (!top_ids || !top_logprobs)))
     return ec::arg_error("ec_op_token_logprobs: tokens and logprob go together; top_k 0..n with "
                          "both outputs");
-  if (top_k > ec::kMaxTop) return ec::unsupported("ec_op_token_logprobs: top_k > 32");
+  if (top_k > ec::kMaxTop || n > ec::kMaxRows || rows > ec::kMaxRows)
+    return ec::unsupported("ec_op_token_logprobs: top_k > 32, or n or rows > 2^30");
   const ec::LogprobArgs a{logits, (long)ld, n, tokens, 1.0f / temperature, top_k, 1, logprob,
                           entropy, top_ids, top_logprobs};
   return ec::with_type(type, [&](auto t) {

@@ -39,6 +39,9 @@ int with_type(int type, F f) {
   }
 }
 
+// Most rows, channels or logits of a call: indices a tile past them stay ints.
+constexpr int kMaxRows = 1 << 30;
+
 inline bool known_type(int type) {
   return type == EC_T_F32 || type == EC_T_BF16 || type == EC_T_F16;
 }

@@ -387,8 +387,9 @@ int		ec_op_sample_temperature(const float *logits, int n, int rows,
 /* allocation, no workspace, nothing kept between calls: calls on different  */
 /* streams and captured graphs share nothing.  Row strides (ld*) count       */
 /* elements and may exceed the row; elements behind a row's end are neither  */
-/* read nor written.  Results do not depend on scheduling: equal inputs give */
-/* equal bits.                                                               */
+/* read nor written.  Pointers are aligned to their elements (else           */
+/* EC_ERR_ARG); rows, m and nb are at most 2^30 (else EC_ERR_UNSUPPORTED).   */
+/* Results do not depend on scheduling: equal inputs give equal bits.        */
 /*                                                                           */
 /* The 8-bit rule of a row y (ec_set_weight_bf16's rounding):                */
 /*   scale = amax / 127, q = y * (127 / amax) to the nearest integer, ties   */
@@ -444,7 +445,8 @@ int		ec_op_gemm_w8a8(const int8_t *x, int64_t ldx, const float *x_scale,
 ** A logit of -inf has probability 0 and adds nothing to the entropy; a row
 ** of nothing else has log probabilities -inf and entropy 0.  A NaN or +inf
 ** makes the row's log probabilities and entropy NaN; NaN orders below -inf
-** among the top_k.  No allocation. */
+** among the top_k.  Pointers are aligned to their elements; n and rows are
+** at most 2^30.  No allocation, nothing kept between calls. */
 int		ec_op_token_logprobs(int type, const void *logits, int64_t ld, int n,
 			int rows, const int *tokens, float temperature, int top_k,
 			float *logprob, float *entropy, int *top_ids, float *top_logprobs,

@@ -113,7 +113,8 @@ def inputs(torch, kind, rows, n, seed=0):
 
 SHAPES = [(1, 1), (3, 2), (1, 7), (5, 31), (2, 64), (7, 257), (4, 1000), (3, 1024), (2, 2047),
           (2, 4096), (9, 4100), (3, 5003), (2, 8192), (2, 14336), (1, 16385), (2, 28672),
-          (1, 57343), (1, 57344), (301, 512)]
+          (1, 57343), (1, 57344), (301, 512), (2, 20001),
+          (3, 24007), (2, 27999), (150, 9001), (2, 32761), (2, 32768), (2, 32776), (700, 130)]
 
 
 @pytest.mark.parametrize("kind", TYPES)

@@ -123,6 +123,18 @@ def test_strides_and_alignment(eng, torch, kind, offset, pad):
         check(l, [0, n - 1, n // 2], 1.0, 7, got, n)
 
 
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("offset", range(8))
+def test_short_rows_at_any_alignment(eng, torch, kind, offset):
+    """Rows that end before, at or just behind their first whole 16 bytes."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    for n in (1, 2, 3, 5, 8, 9, 13, 17):
+        l = (torch.randn(9, n, generator=g, device="cuda") * 3).to(dtype(torch, kind))
+        tokens = [k % n for k in range(9)]
+        got = run(eng, torch, kind, l, tokens, 1.0, n, n + offset % 3, offset)
+        check(l, tokens, 1.0, n, got, n)
+
+
 @pytest.mark.parametrize("n", [50, 5000, 128256])
 def test_ties_go_to_the_lowest_index(eng, torch, n):
     l = torch.zeros(4, n, device="cuda")

@@ -46,6 +46,7 @@ def test_norm_width(eng):
     n = 57345
     refused(eng, eng.lib().ec_op_add_rmsnorm_quant, NORM,
             {2: n, 4: n, 6: n, 10: n, 12: n}, eng.EC_ERR_UNSUPPORTED)
+    refused(eng, eng.lib().ec_op_add_rmsnorm_quant, NORM, {9: 2 ** 30 + 1}, eng.EC_ERR_UNSUPPORTED)
 
 
 SILU = [0, P, P, 64, 2, 64, P, 64, P, None]
@@ -61,6 +62,7 @@ def test_silu_arguments(eng, changes):
 def test_silu_width(eng):
     n = 57345
     refused(eng, eng.lib().ec_op_silu_mul_quant, SILU, {3: n, 5: n, 7: n}, eng.EC_ERR_UNSUPPORTED)
+    refused(eng, eng.lib().ec_op_silu_mul_quant, SILU, {4: 2 ** 30 + 1}, eng.EC_ERR_UNSUPPORTED)
 
 
 # x ldx sx w ldw sw type y ldy m k nb status stream
@@ -76,8 +78,10 @@ def test_gemm_arguments(eng, changes):
 
 
 def test_gemm_length(eng):
-    refused(eng, eng.lib().ec_op_gemm_w8a8, GEMM, {1: 131072, 4: 131072, 10: 131072},
-            eng.EC_ERR_UNSUPPORTED)
+    fn, big = eng.lib().ec_op_gemm_w8a8, 2 ** 30 + 1
+    refused(eng, fn, GEMM, {1: 131072, 4: 131072, 10: 131072}, eng.EC_ERR_UNSUPPORTED)
+    refused(eng, fn, GEMM, {11: big}, eng.EC_ERR_UNSUPPORTED)
+    refused(eng, fn, GEMM, {9: big, 8: big}, eng.EC_ERR_UNSUPPORTED)
 
 
 # type logits ld n rows tokens temperature top_k logprob entropy ids tlp stream
@@ -93,5 +97,8 @@ def test_logprob_arguments(eng, changes):
 
 
 def test_logprob_top(eng):
-    refused(eng, eng.lib().ec_op_token_logprobs, LOGP, {7: 33}, eng.EC_ERR_UNSUPPORTED)
+    fn, big = eng.lib().ec_op_token_logprobs, 2 ** 30 + 1
+    refused(eng, fn, LOGP, {7: 33}, eng.EC_ERR_UNSUPPORTED)
+    refused(eng, fn, LOGP, {4: big}, eng.EC_ERR_UNSUPPORTED)
+    refused(eng, fn, LOGP, {2: big, 3: big}, eng.EC_ERR_UNSUPPORTED)
     assert C.sizeof(C.c_int64) == 8
