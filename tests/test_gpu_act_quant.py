@@ -264,6 +264,37 @@ def test_silu_rows_without_a_finite_scale(eng, torch):
         assert sc[4].isfinite() and q[4].abs().max() == 127
 
 
+@pytest.mark.parametrize("n", [1000, 1003])
+def test_offsets_past_32_bits(eng, torch, n):
+    """Row strides that put the third row past 2^31 elements."""
+    far = 2 ** 30 + 8
+    x, r, w = inputs(torch, "bf16", 3, n, 5)
+    buf = torch.empty(2 * far + n, dtype=torch.bfloat16, device="cuda")
+    q = torch.zeros(2 * far + n, dtype=torch.int8, device="cuda")
+    sc = torch.zeros(3, device="cuda")
+    rows = lambda b: torch.stack([b[t * far:t * far + n] for t in range(3)])  # noqa: E731
+    for t in range(3):
+        buf[t * far:t * far + n] = x[t]
+    eng.check(eng.lib().ec_op_add_rmsnorm_quant(
+        1, buf.data_ptr(), far, r.data_ptr(), n, buf.data_ptr(), far, w.data_ptr(), 1e-5, 3, n,
+        q.data_ptr(), far, sc.data_ptr(), None))  # the sum in x's place
+    torch.cuda.synchronize()
+    h = (x.float() + r.float()).to(torch.bfloat16)
+    assert torch.equal(rows(buf), h)
+    check_rows(norm64(h, w, 1e-5), norm_rel(n), rows(q).cpu().numpy().astype(np.float64),
+               sc.double().cpu().numpy())
+    for t in range(3):
+        buf[t * far:t * far + n] = x[t]
+    up = torch.empty_like(buf)
+    for t in range(3):
+        up[t * far:t * far + n] = r[t]
+    eng.check(eng.lib().ec_op_silu_mul_quant(1, buf.data_ptr(), up.data_ptr(), far, 3, n,
+                                             q.data_ptr(), far, sc.data_ptr(), None))
+    torch.cuda.synchronize()
+    check_rows(silu64(x, r), silu_rel(x), rows(q).cpu().numpy().astype(np.float64),
+               sc.double().cpu().numpy())
+
+
 def test_equal_calls_give_equal_bits(eng, torch):
     x, r, w = inputs(torch, "bf16", 600, 4096, 3)
     one = run_norm(eng, torch, "bf16", x, r, w, 1e-5)

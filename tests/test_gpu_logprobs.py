@@ -208,6 +208,15 @@ def test_peaked_and_far_logits(eng, torch):
     assert np.all(np.abs(got[1] - en) < 8 * U)
 
 
+@pytest.mark.parametrize("n", [1000, 40001])
+def test_offsets_past_32_bits(eng, torch, n):
+    """A row stride that puts the third row past 2^31 elements."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    l = (torch.randn(3, n, generator=g, device="cuda") * 3).to(torch.bfloat16)
+    got = run(eng, torch, "bf16", l, [0, 1, n - 1], 1.0, 9, 2 ** 30 + 3)
+    check(l, [0, 1, n - 1], 1.0, 9, got, n)
+
+
 def test_equal_calls_give_equal_bits(eng, torch):
     l = torch.randn(64, 50000, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
     a = run(eng, torch, "f32", l, list(range(64)), 0.9, 16)

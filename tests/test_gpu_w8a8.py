@@ -163,6 +163,30 @@ def test_two_streams_at_once(eng, torch):
         check(torch, "f32", y, exact(torch, x, w, sx, sw, k))
 
 
+def test_offsets_past_32_bits(eng, torch):
+    """Row strides that put the last rows of x, w and y past 2^31 elements."""
+    k, far = 300, 2 ** 31 + 16
+    x, w = int8_rows(torch, 2, k, 304, 1), int8_rows(torch, 2, k, 304, 2)
+    sx, sw = scales(torch, 3, 40, 3)
+    fx, fw = (torch.empty(far + 304, dtype=torch.int8, device="cuda") for _ in range(2))
+    for f, v in ((fx, x), (fw, w)):
+        f[:k], f[far:far + k] = v[0, :k], v[1, :k]
+    y = torch.zeros(2, 2, device="cuda")
+    eng.check(eng.lib().ec_op_gemm_w8a8(fx.data_ptr(), far, sx.data_ptr(), fw.data_ptr(), far,
+                                        sw.data_ptr(), 0, y.data_ptr(), 2, 2, k, 2, None, None))
+    torch.cuda.synchronize()
+    check(torch, "f32", y, exact(torch, x, w, sx[:2], sw[:2], k))
+    del fx, fw
+    x, w = int8_rows(torch, 3, k, 304, 1), int8_rows(torch, 40, k, 304, 2)
+    ldy = 2 ** 30 + 3
+    y = torch.empty(2 * ldy + 40, dtype=torch.bfloat16, device="cuda")
+    eng.check(eng.lib().ec_op_gemm_w8a8(x.data_ptr(), 304, sx.data_ptr(), w.data_ptr(), 304,
+                                        sw.data_ptr(), 1, y.data_ptr(), ldy, 40, k, 3, None, None))
+    torch.cuda.synchronize()
+    got = torch.stack([y[t * ldy:t * ldy + 40] for t in range(3)])
+    check(torch, "bf16", got, exact(torch, x, w, sx, sw, k))
+
+
 # ------------------------------------------------------------------ runs --
 
 
