@@ -51,22 +51,12 @@ struct SiluArgs {
 
 // ------------------------------------------------------------ the 8-bit rule --
 
-// 1 / x for x from 2^-110 to 2^118, within 2 units of f32 rounding: every
-// thread of a row computes it, so no exact division.
-__device__ __forceinline__ float reciprocal(float x) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
 // The row's 8-bit factor from amax' bits: as unsigned integers the bit
 // patterns of |y| order like the values, infinities and NaN above all finite
 // ones, so neither is lost in the maximum.  0: a row of zeros.
 __device__ __forceinline__ float quant_factor(unsigned amax_bits) {
   const float amax = __uint_as_float(amax_bits);
-  const bool plain = amax_bits < 0x7f800000u && amax >= 0x1p-100f;
-  // in two powers of two, so that neither end of the range leaves f32's
-  return plain ? __fmul_rn(reciprocal(__fmul_rn(amax, 0x1p-10f)), 127.0f * 0x1p-10f) : 0.0f;
+  return amax_bits < 0x7f800000u && amax >= 0x1p-100f ? __fdiv_rn(127.0f, amax) : 0.0f;
 }
 __device__ __forceinline__ float quant_scale(unsigned amax_bits) {
   const float amax = __uint_as_float(amax_bits);
@@ -74,19 +64,19 @@ __device__ __forceinline__ float quant_scale(unsigned amax_bits) {
   return amax < 0x1p-100f ? 1.0f : __fdiv_rn(amax, 127.0f);
 }
 
-// y * f rounded to the nearest integer, ties to even, in the low byte: the
-// one rounding of the sum with 1.5 * 2^23, whose unit is 1 (|y * f| <= 127
-// and a rounding of it).  f = 0 marks a row of zeros, whatever y holds.
+// y * f, rounded to f32 and then to the nearest integer, ties to even, in the
+// low byte: the one rounding of the sum with 1.5 * 2^23, whose unit is 1
+// (|y * f| <= 127 and a rounding of it).  The product is rounded first, not
+// fused: 16-bit rows often hold exact halves, which the product's rounding
+// restores.  f = 0 marks a row of zeros, whatever y holds.
 __device__ __forceinline__ unsigned quant_byte(float y, float f) {
-  return __float_as_uint(__fmaf_rn(y, f, 12582912.0f)) & 0xffu;
+  return __float_as_uint(__fadd_rn(__fmul_rn(y, f), 12582912.0f)) & 0xffu;
 }
 __device__ __forceinline__ uint64_t both(float v) {
   return pack2(__float_as_uint(v), __float_as_uint(v));
 }
 __device__ __forceinline__ uint64_t quant_pair(uint64_t y, uint64_t f) {
-  uint64_t t = both(12582912.0f);
-  fma2(t, y, f);
-  return t;
+  return add2(mul2(y, f), both(12582912.0f));
 }
 __device__ __forceinline__ unsigned quant4(uint64_t y01, uint64_t y23, uint64_t f) {
   const uint64_t a = quant_pair(y01, f), b = quant_pair(y23, f);
@@ -133,7 +123,7 @@ __device__ __forceinline__ unsigned block_max(unsigned v, unsigned* red) {
 // gives NaN, not a silent row of zeros.
 __device__ __forceinline__ float norm_factor(float ss, float inv_n, float eps) {
   float r;
-  asm("rsqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(__fmaf_rn(ss, inv_n, eps)));
+  asm("rsqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(__fadd_rn(__fmul_rn(ss, inv_n), eps)));
   return ss == INFINITY ? __uint_as_float(0x7fc00000u) : r;
 }
 
