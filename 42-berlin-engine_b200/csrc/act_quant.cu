@@ -15,6 +15,11 @@
 // ends element by element) and read back in pieces that are aligned in the
 // sum (or the first operand): two aligned reads and a shift.
 // Rows past 1024 threads' registers stay in shared memory as f32 (wide_kernel).
+//
+// One B200, inputs from HBM: residual + norm of 8192x8192 f32 132 us (6.6 TB/s,
+// the copy peak), bf16 80 us (5.9 TB/s, 72% of the issue slots); SwiGLU of
+// 4096x28672 bf16 97 us (6.0 TB/s); one row of 4096 2.3 us, two barriers and a
+// memory round trip over an empty launch.
 #include <type_traits>
 
 #include "typed.cuh"
@@ -618,6 +623,21 @@ struct Shape {
   int rows_per_cta;  // where several CTAs share an SM
 };
 
+// Few rows: 8 values a thread, more threads hide a row's latency (us, norm,
+// 64x8192 bf16: 3.3 with 8, 3.6 with 16, 4.9 with 32).  Many: 16 of f32 (8192x8192:
+// 132; 184 with 8, 149 with 32) and 32 of 16-bit rows (80; 155, 98), fewer
+// reductions a value, 16 of short ones; 16-bit rows two a CTA (SwiGLU 8192x1024:
+// 9.2; 9.8 with one).  Unaligned rows carry more a thread besides: 16, two a CTA
+// (4000x5003 bf16 norm: 55; 112 with 8, 57 with 32; 59 with one).
+template <typename T>
+Shape shape_of(int rows, int n, bool vec) {
+  const bool few = rows < 148 * 2;
+  if (!vec) return Shape{16, few ? 1 : 2};
+  if (few) return Shape{8, 1};
+  if (sizeof(T) == 4) return Shape{16, 1};
+  return Shape{n >= 4096 ? 32 : 16, 2};
+}
+
 // Launches the kernel of the row's alignment and size; `wide` where a row fits
 // neither the registers nor the shared memory.  `extra`: shared memory for the
 // weights.
@@ -635,8 +655,10 @@ int rows_launch(Args a, bool vec, Shape s, size_t extra, void (*wide)(Args), Pic
     return launch(wide, a, a.rows, kWideThr, (size_t)a.n * 4, st);
   const int threads = ((span + s.f - 1) / s.f + 31) / 32 * 32;
   // CTAs that an SM holds: by threads (64 registers each) and shared memory.
-  // Alone on its SM a CTA walks all its rows; else a few, so that the SMs'
-  // different speeds even out.
+  // Alone on its SM a CTA walks all its rows, the next one's copies under this
+  // one's reductions (4096x28672 bf16 SwiGLU: 95 us; 125 with one row a CTA).
+  // Several on an SM cover one another, and rows handed out as CTAs end even
+  // out the SMs' different speeds (8192x8192 f32 norm: 132; 163 walking).
   const bool alone = kMaxThr / threads < 2 || kStageMax / (smem + 1024) < 2;
   const int grid = alone ? (a.rows < 148 ? a.rows : 148)
                          : (a.rows + s.rows_per_cta - 1) / s.rows_per_cta;
@@ -650,9 +672,7 @@ int norm_rows(const NormArgs& a, cudaStream_t st) {
                    (!a.r || aligned(a.r, a.ldr, sizeof(T), 16)) &&
                    (!a.h || aligned(a.h, a.ldh, sizeof(T), 16)) &&
                    (!a.w || aligned(a.w, 0, 2, 2 * per)) && aligned(a.q, a.ldq, 1, per);
-  const bool few = a.rows < 148 * 2;
-  const Shape s = !vec ? Shape{16, few ? 1 : 2}
-                       : Shape{few ? 8 : 16, few || sizeof(T) == 4 ? 1 : 4};
+  const Shape s = shape_of<T>(a.rows, a.n, vec);
   const size_t extra = !vec && a.w ? Part<__nv_bfloat16, 8, false>::room(a.n) : 0;
   return rows_launch<T>(a, vec, s, extra, norm_wide_kernel<T>, [](int f, bool v) {
     return v ? (f == 8 ? norm_rows_kernel<T, 8, true>
@@ -667,10 +687,7 @@ int silu_rows(const SiluArgs& a, cudaStream_t st) {
   constexpr int per = 16 / (int)sizeof(T);
   const bool vec = a.n % per == 0 && aligned(a.g, a.ld, sizeof(T), 16) &&
                    aligned(a.u, a.ld, sizeof(T), 16) && aligned(a.q, a.ldq, 1, per);
-  const bool few = a.rows < 148 * 2;
-  const Shape s = !vec ? Shape{16, few ? 1 : 2}
-                       : Shape{few ? 8 : sizeof(T) == 2 && a.n >= 4096 ? 32 : 16,
-                               few || sizeof(T) == 4 ? 1 : 2};
+  const Shape s = shape_of<T>(a.rows, a.n, vec);
   return rows_launch<T>(a, vec, s, 0, silu_wide_kernel<T>, [](int f, bool v) {
     return v ? (f == 8 ? silu_rows_kernel<T, 8, true>
                        : f == 16 ? silu_rows_kernel<T, 16, true> : silu_rows_kernel<T, 32, true>)

@@ -19,16 +19,22 @@
 // 256 channels x Tn <= 256 tokens; each holds half of the channels and half of
 // the tokens in shared memory, and the first issues tcgen05.mma.cta_group::2
 // for both, which reads both halves: per SM half the token bytes of a 128-row
-// tile.  Loads of both CTAs complete on the first one's barriers; commits
-// release the stages of both.
+// tile (8192x28672x4096: 598 us; 773 with one CTA a tile).  Loads of both CTAs
+// complete on the first one's barriers; commits release the stages of both.
+// The tensor cores bound it: 3.2-3.4 POP/s, and 2.75 where the power limit
+// holds the clock at 1.2 GHz.
 //
-// gemm_w8a8_kernel (few tokens): a tile is R <= 128 channels x up to 256 tokens.  With few
-// tokens the weights' bytes are the bound, and R is chosen so that the tiles
-// fill whole rounds of the SMs (every SM streams the same share of the
-// weights); the MMA computes its 128 rows whatever R is, which costs
-// nothing there.  With C > 1 a cluster of C CTAs splits K: the partial
-// accumulators meet in distributed shared memory, each CTA finishing a part of
-// the token columns.  Warp 0 streams, warp 1 issues the MMAs, the others drain
+// gemm_w8a8_kernel (few tokens): a tile is R <= 128 channels x up to 256 tokens.
+// The weights' bytes are the bound (1x128256x4096: 5.8-6.2 TB/s), and R is
+// chosen so that the tiles fill whole rounds of the SMs (every SM streams the
+// same share of the weights).  The MMA computes its 128 rows whatever R is, in
+// 66 cycles with few tokens; below 50 rows a tile that would bound it, and K is
+// split instead (1x4096x14336: 14 us with 125 rows over 4 CTAs, 24 with 28 rows
+// alone).
+//
+// Both can split K over a cluster (256x4096x14336: 23 us over 2 pairs, 31
+// without): the partial accumulators meet in distributed shared memory, each
+// CTA finishing a part of the token columns.  Warp 0 streams, warp 1 issues the MMAs, the others drain
 // TMEM; two TMEM buffers let a tile's epilogue run under the next one's MMAs.
 #include <atomic>
 #include <mutex>

@@ -12,6 +12,11 @@
 // entry and of the value that the block's warps together already hold top_k
 // times.  On rows in random order few chunks do.
 //
+// One B200, rows from HBM: 2048x128256 f32 with 20 alternatives 181 us (5.8
+// TB/s), without 168 us; bf16 172 and 117 us (issue: 16 and 10 instructions a
+// value); one row with 5 alternatives 9.3 us, of which 4 are the dependent steps
+// of thresholds, entries and list merges.
+//
 // A row is split over a cluster of CTAs while the rows alone do not fill the
 // SMs; the statistics and lists meet in a fixed order through (distributed)
 // shared memory, so equal inputs give equal bits.
