@@ -107,6 +107,14 @@ __device__ __noinline__ u64 merge_keys(u64 list, u64 x, int lane) {
 
 // the rank-th largest (from 0) of the lanes' values
 __device__ __forceinline__ unsigned nth_largest(unsigned x, int rank, int lane) {
+  if (rank < 4) {  // the same by taking the largest away
+    unsigned m = __reduce_max_sync(0xffffffffu, x);
+    for (; rank > 0; rank--) {
+      if (lane == __ffs(__ballot_sync(0xffffffffu, x == m)) - 1) x = 0;
+      m = __reduce_max_sync(0xffffffffu, x);
+    }
+    return m;
+  }
 #pragma unroll
   for (int k = 2; k <= 32; k <<= 1) {
 #pragma unroll
@@ -196,6 +204,7 @@ __device__ __forceinline__ float max_of(const float* v) {
 
 struct Warp {
   Running st;
+  bool barred; // a chunk had logits of -inf
   u64 key;     // the list
   float thr;   // only values above it can enter; NaN: any can
   int lane, warp, warps, top, share;
@@ -233,7 +242,7 @@ struct Warp {
     // not the row's, are added with these far enough below for it to be 0.
     const uint64_t m2 = pair_of(-st.m, -st.m), c22 = pair_of(c2, c2);
     uint64_t s = st.s, w = st.w;
-    bool plain = __all_sync(0xffffffffu, valid == (1u << kChunk) - 1u);
+    bool plain = !barred && __all_sync(0xffffffffu, valid == (1u << kChunk) - 1u);
     if (plain) {
 #pragma unroll
       for (int j = 0; j < kChunk; j += 2) {
@@ -244,6 +253,7 @@ struct Warp {
       }
       const float sum = __fadd_rn(lo_f(w), hi_f(w));
       plain = sum == sum;
+      barred = __any_sync(0xffffffffu, !plain);  // likely further on too
     }
     if (!plain) {
       s = st.s;
@@ -400,15 +410,22 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
     return valid;
   };
   // the warps with a chunk, and the first threshold: the share-th largest of
-  // each one's lane maxima
+  // each one's lane maxima over the chunks under way
   w.warps = max(1, min(warps, (v1 - v0 + 32 * kLoads - 1) / (32 * kLoads)));
   w.share = (a.top + w.warps - 1) / w.warps;
   if (a.top) {
     if (warp < w.warps) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
-      float v[kChunk];
-      read(v, ring, first);
-      const unsigned o = nth_largest(order_of(max_of(v)), w.share - 1, lane);
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      float m = -INFINITY;
+#pragma unroll
+      for (int d = 0; d < D; d++) {
+        if (first + d * step < v1) {
+          float v[kChunk];
+          read(v, ring + d * kSlot, first + d * step);
+          m = max_nan(m, max_of(v));
+        }
+      }
+      const unsigned o = nth_largest(order_of(m), w.share - 1, lane);
       if (lane == 0) held[warp] = o;
     }
     __syncthreads();
