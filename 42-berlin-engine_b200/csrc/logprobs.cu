@@ -14,8 +14,9 @@
 //
 // One B200, rows from HBM: 2048x128256 f32 with 20 alternatives 181 us (5.8
 // TB/s), without 168 us; bf16 172 and 117 us (issue: 16 and 10 instructions a
-// value); one row with 5 alternatives 9.3 us, of which 4 are the dependent steps
-// of thresholds, entries and list merges.
+// value); one row with 5 alternatives 8.4 us, of which 4 are the dependent steps
+// of thresholds, entries and list merges; 300x32003 bf16, nine tenths of it -inf,
+// with 8 alternatives 18.7 us.
 //
 // A row is split over a cluster of CTAs while the rows alone do not fill the
 // SMs; the statistics and lists meet in a fixed order through (distributed)
@@ -320,8 +321,8 @@ __device__ __forceinline__ float peer_f32(uint32_t addr, int rank) {
   return v;
 }
 
-// Bytes of a chunk of 32 lanes, and chunks that a warp has under way: 8 KB of it,
-// so that some 200 KB are in flight on an SM whatever its warps work at.
+// Bytes of a chunk of 32 lanes, and chunks that a warp has under way: 6 KB, so
+// that 32 warps keep 192 KB in flight on an SM whatever they work at.
 template <typename T>
 constexpr int kChunkBytes = 32 * kChunk * (int)sizeof(T);
 template <typename T>
@@ -388,6 +389,13 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
   };
 #pragma unroll
   for (int d = 0; d < D; d++) fetch(d, first + d * step);
+  // the given token's logit, asked for now and used at the end
+  int token = -1;
+  float token_l = 0.0f;
+  if (a.logprob && rank == 0 && threadIdx.x == 0) {
+    token = a.tokens[row];
+    if (token >= 0 && token < a.n) token_l = to_f32(l[token]);
+  }
   // a chunk's values, -inf where the row has none; which are the row's
   auto read = [&](float* v, const T* kept, int b) {
     unsigned valid = (1u << kChunk) - 1u;
@@ -519,10 +527,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
     if (a.entropy)
       a.entropy[row] = lost ? nan : none ? 0.0f
                        : __fsub_rn(logs, __fmul_rn(__fdiv_rn(st.w, st.s), 0.693147181f));
-    if (a.logprob) {
-      const int t = a.tokens[row];
-      a.logprob[row] = t == -1 ? 0.0f : t >= 0 && t < a.n ? logprob(to_f32(l[t])) : nan;
-    }
+    if (a.logprob)
+      a.logprob[row] = token == -1 ? 0.0f : token >= 0 && token < a.n ? logprob(token_l) : nan;
   }
   if (lane < a.top) {
     a.ids[row * a.top + lane] = (int)~(unsigned)w.key;
@@ -540,8 +546,10 @@ inline int cluster_for(int rows, int n) {
 
 // Warps of a CTA: 16 while there are few rows, so that a row ends early; with
 // many rows fewer, so that more rows are on an SM at once and one's joins pass
-// under another's chunks (4096x32000 with 20 alternatives: 117 us with 4 warps,
-// 136 with 8, 189 with 16; 2048x128256: 189, 181, 206).
+// under another's chunks.  f32 with 20 alternatives, us with 4 / 8 / 16 warps:
+// 200x32000 - / 15.9 / 15.8; 300x32003 22.0 / 22.6 / 22.7; 600x32000 32 / 30 /
+// 37; 4096x32000 116 / 129 / 173; 296x128256 50 / 38 / 36; 2048x128256 186 / 176
+// / 203.
 inline int warps_for(int rows, int n, int cl) {
   const int most = cl > 1 || rows < 256 ? 16 : n > 65536 ? 8 : 4;
   const int chunks = (n / cl + 32 * kChunk - 1) / (32 * kChunk);
