@@ -208,6 +208,21 @@ def test_peaked_and_far_logits(eng, torch):
     assert np.all(np.abs(got[1] - en) < 8 * U)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [3, 1000, 70001])
+def test_ends_of_the_temperature(eng, torch, kind, n):
+    """2^-100: all but the largest token are some 1e30 below it, finite in f32.
+    2^100: every power is 1, the sum n."""
+    l = torch.randperm(n, generator=torch.Generator(device="cuda").manual_seed(n), device="cuda")
+    l = (l.float() / n - 0.5).to(torch.float32 if kind == "f32" else torch.bfloat16)
+    top = int(l.argmax())
+    l[top] = 2.0
+    l = l.repeat(2, 1)
+    for temperature in (2.0 ** -100, 2.0 ** 100):
+        tokens = [top, (top + 1) % n]
+        check(l, tokens, temperature, 3, run(eng, torch, kind, l, tokens, temperature, 3), n)
+
+
 @pytest.mark.parametrize("n", [1000, 40001])
 def test_offsets_past_32_bits(eng, torch, n):
     """A row stride that puts the third row past 2^31 elements."""

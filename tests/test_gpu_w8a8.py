@@ -5,6 +5,10 @@ Tolerance of the product: the int32 sum is exact; its conversion to f32 and
 the two scalings are three roundings of 2^-24 of the result, and the rounding
 to the output's type is half a step of it.
 """
+import subprocess
+import sys
+from pathlib import Path
+
 import numpy as np
 import pytest
 
@@ -327,3 +331,36 @@ def test_block_captured_and_replayed(eng, torch):
         torch.cuda.synchronize()
         for b, want in zip(blocks, eager):
             assert all(torch.equal(p, q) for p, q in zip(b.results(), want[k]))
+
+
+FIRST_CAPTURED = """
+import sys
+sys.path.insert(0, "tests")
+import torch
+from conftest import load_pkg_module
+import test_gpu_w8a8 as t
+eng = load_pkg_module("engine")
+eng.lib()
+b = t.Block(torch, 40, 512, 1408, 4096, seed=1)
+s = torch.cuda.Stream()
+s.wait_stream(torch.cuda.current_stream())
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=s):
+    b.call(eng, torch.cuda.current_stream().cuda_stream)
+g.replay()
+torch.cuda.synchronize()
+captured = b.results()
+b.call(eng, None)
+torch.cuda.synchronize()
+assert all(torch.equal(p, q) for p, q in zip(captured, b.results()))
+print("equal")
+"""
+
+
+def test_first_calls_captured():
+    """A process whose first calls are captured ones: what a call sets up once
+    a device does not disturb the capture."""
+    root = Path(__file__).resolve().parents[1]
+    done = subprocess.run([sys.executable, "-c", FIRST_CAPTURED], cwd=root, capture_output=True,
+                          text=True, timeout=300)
+    assert done.returncode == 0 and done.stdout.strip().endswith("equal"), done.stderr[-2000:]
