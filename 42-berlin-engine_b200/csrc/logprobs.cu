@@ -9,14 +9,15 @@
 // exponents in base 2, e = 2^((l - m) log2(e) / T)), and every warp the sorted
 // top_k of what it has seen, one entry a lane.  A warp looks for entries only
 // in chunks whose maximum passes its threshold: the larger of its own last
-// entry and of the value that the block's warps together already hold top_k
-// times.  On rows in random order few chunks do.
+// entry and of the top_k-th of 32 values that the block's warps have seen.  On
+// rows in random order few chunks do (2048x128256: a quarter with 20
+// alternatives, a tenth with 5).
 //
-// One B200, rows from HBM: 2048x128256 f32 with 20 alternatives 181 us (5.8
-// TB/s), without 168 us; bf16 172 and 117 us (issue: 16 and 10 instructions a
-// value); one row with 5 alternatives 8.4 us, of which 4 are the dependent steps
-// of thresholds, entries and list merges; 300x32003 bf16, nine tenths of it -inf,
-// with 8 alternatives 18.7 us.
+// One B200, rows from HBM: 2048x128256 f32 with 20 alternatives 177-187 us
+// (5.6-5.9 TB/s), without 165-180; bf16 170 and 120 (issue: 16 and 10
+// instructions a value); one row with 5 alternatives 8.4 us, of which 4 are the
+// dependent steps of thresholds, entries and list merges; 300x32003 bf16, nine
+// tenths of it -inf, with 8 alternatives 18.9 us.
 //
 // A row is split over a cluster of CTAs while the rows alone do not fill the
 // SMs; the statistics and lists meet in a fixed order through (distributed)
@@ -106,26 +107,18 @@ __device__ __noinline__ u64 merge_keys(u64 list, u64 x, int lane) {
   return merge_lists(list, x, lane);
 }
 
-// the rank-th largest (from 0) of the lanes' values
-__device__ __forceinline__ unsigned nth_largest(unsigned x, int rank, int lane) {
-  if (rank < 4) {  // the same by taking the largest away
-    unsigned m = __reduce_max_sync(0xffffffffu, x);
-    for (; rank > 0; rank--) {
-      if (lane == __ffs(__ballot_sync(0xffffffffu, x == m)) - 1) x = 0;
-      m = __reduce_max_sync(0xffffffffu, x);
-    }
-    return m;
-  }
+// the lanes' values, descending
+__device__ __forceinline__ unsigned descending(unsigned x, int lane) {
 #pragma unroll
   for (int k = 2; k <= 32; k <<= 1) {
 #pragma unroll
     for (int s = k >> 1; s > 0; s >>= 1) {
       const unsigned o = __shfl_xor_sync(0xffffffffu, x, s);
       const bool up = (lane & k) == 0 || k == 32;
-      x = ((lane & s) == 0) == up ? min(x, o) : max(x, o);
+      x = ((lane & s) == 0) == up ? max(x, o) : min(x, o);
     }
   }
-  return __shfl_sync(0xffffffffu, x, 31 - rank);
+  return x;
 }
 
 // ------------------------------------------------------- the statistics --
@@ -208,25 +201,55 @@ struct Warp {
   bool barred; // a chunk had logits of -inf
   u64 key;     // the list
   float thr;   // only values above it can enter; NaN: any can
-  int lane, warp, warps, top, share;
-  unsigned* held;  // [warps]: order of each warp's share-th entry
+  int lane, warps, top, share, slots;
+  unsigned* held;  // [warp][slots]: orders of values that the warps have seen
+  unsigned* own;   // this warp's
 
-  // `share` = ceil(top / warps) values of every warp are top values at least,
-  // so the smallest of the warps' share-th values bounds the row's last entry
-  // from below (values equal to it may still enter, by their index).
+  // A bound of the row's last entry from below (values equal to it may still
+  // enter, by their index).  A slot only ever grows, up to its warp's value of
+  // that rank, so a mix of slots read at different times gives a smaller
+  // bound, never a wrong one.
+  //   slots > 1: each warp's largest ones, 32 in all (0: none yet); the top-th
+  //     largest of them, that is the largest that top of the 32 reach.
+  //   slots = 1: each warp's share-th, share = ceil(top / warps); the smallest
+  //     of them: less to do, and no worse while there are few warps.
   __device__ __forceinline__ unsigned all_hold() {
-    volatile unsigned* h = held;
-    return __reduce_min_sync(0xffffffffu, lane < warps ? h[lane] : 0xffffffffu);
+    const unsigned x = *reinterpret_cast<volatile unsigned*>(held + lane);
+    if (slots == 1) return __reduce_min_sync(0xffffffffu, lane < warps ? x : 0xffffffffu);
+    int reach = 0;
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      unsigned a, b, c, d;
+      asm volatile("ld.volatile.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(smem_u32(held + j)));
+      reach += (a >= x) + (b >= x) + (c >= x) + (d >= x);
+    }
+    return __reduce_max_sync(0xffffffffu, reach >= top ? x : 0u);
+  }
+  // The first values: the largest of the lanes'.
+  __device__ __forceinline__ void hold_first(unsigned x) {
+    const int count = slots > 1 ? slots : share;
+    if (count > 4) {  // slots = 1
+      x = __shfl_sync(0xffffffffu, descending(x, lane), share - 1);
+      if (lane == 0) own[0] = x;
+      return;
+    }
+    for (int i = 0; i < count; i++) {
+      const unsigned m = __reduce_max_sync(0xffffffffu, x);
+      if (lane == 0) own[slots > 1 ? i : 0] = m;
+      if (lane == __ffs(__ballot_sync(0xffffffffu, x == m)) - 1) x = 0;
+    }
   }
   // The threshold after the list has changed.  All values to come have larger
   // indices than the list's, so one equal to its last does not enter.
   __device__ __forceinline__ void update() {
-    const unsigned own = (unsigned)(__shfl_sync(0xffffffffu, key, top - 1) >> 32);
-    const unsigned mine = (unsigned)(__shfl_sync(0xffffffffu, key, share - 1) >> 32);
-    volatile unsigned* h = held;
-    if (lane == 0 && warp < warps && mine > h[warp]) h[warp] = mine;
+    const unsigned mine = (unsigned)(key >> 32);
+    const unsigned last = __shfl_sync(0xffffffffu, mine, top - 1);
+    volatile unsigned* h = own;
+    const int at = slots > 1 ? lane : lane - (share - 1);
+    if (at >= 0 && at < slots && mine > h[at]) h[at] = mine;
     __syncwarp();
-    thr = fmaxf(fmaxf(thr, just_below(all_hold())), own > 1u ? value_of(own) : just_below(0u));
+    thr = fmaxf(fmaxf(thr, just_below(all_hold())), last > 1u ? value_of(last) : just_below(0u));
   }
 
   // A chunk: kChunk values a lane, the j-th also at `kept` (this lane's, run
@@ -339,13 +362,13 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
   constexpr int D = ring_depth<T>();
   extern __shared__ __align__(16) uint8_t ring_mem[];  // [warp][D][kLoads][32 lanes][16]
   __shared__ T ends[32 * kPer];  // warp 0's: the values outside whole pieces
-  __shared__ unsigned held[kMaxWarps];
+  __shared__ __align__(16) unsigned held[32];
   __shared__ Stat stats[kMaxWarps];
   __shared__ u64 lists[kMaxWarps][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int rank = blockIdx.x % a.cl;
   const long row = blockIdx.x / a.cl;
-  if (threadIdx.x < kMaxWarps) held[threadIdx.x] = 0;
+  if (threadIdx.x < 32) held[threadIdx.x] = 0;
   __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
@@ -355,9 +378,14 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
   w.st = Running{-INFINITY, 0ull, 0ull};
   w.thr = __uint_as_float(0x7fc00000u);
   w.lane = lane;
-  w.warp = warp;
   w.top = a.top;
+  // one / 32 values in all, us: 256x128256 bf16, 16 warps, 5 alternatives 32.5 /
+  // 29.1, 20 35.4 / 33.2, 24 35.2 / 34.5, 32 35.3 / 40.3; 2048x128256 bf16, 8
+  // warps, 5 154.6 / 146.4, 20 171.9 / 170.0, 24 171.1 / 177.5; 4096x32000 f32, 4
+  // warps, 20 116 / 124
+  w.slots = warps >= 8 && a.top <= 20 ? 32 / warps : 1;
   w.held = held;
+  w.own = held + warp * w.slots;
 
   // [0, head) and [head + nv * kPer, n) lie outside whole 16-byte pieces
   const int mis = (int)((reinterpret_cast<uintptr_t>(l) & 15) / sizeof(T));
@@ -417,13 +445,13 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
     }
     return valid;
   };
-  // the warps with a chunk, and the first threshold: the share-th largest of
-  // each one's lane maxima over the chunks under way
+  // the warps with a chunk, and the first threshold, from the lane maxima over
+  // the chunks under way
   w.warps = max(1, min(warps, (v1 - v0 + 32 * kLoads - 1) / (32 * kLoads)));
   w.share = (a.top + w.warps - 1) / w.warps;
   if (a.top) {
-    if (warp < w.warps) {
-      asm volatile("cp.async.wait_all;" ::: "memory");
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (first < v1) {
       float m = -INFINITY;
 #pragma unroll
       for (int d = 0; d < D; d++) {
@@ -433,8 +461,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
           m = max_nan(m, max_of(v));
         }
       }
-      const unsigned o = nth_largest(order_of(m), w.share - 1, lane);
-      if (lane == 0) held[warp] = o;
+      w.hold_first(order_of(m));
     }
     __syncthreads();
     w.thr = just_below(w.all_hold());
@@ -544,14 +571,21 @@ inline int cluster_for(int rows, int n) {
   return cl;
 }
 
-// Warps of a CTA: 16 while there are few rows, so that a row ends early; with
-// many rows fewer, so that more rows are on an SM at once and one's joins pass
-// under another's chunks.  f32 with 20 alternatives, us with 4 / 8 / 16 warps:
-// 200x32000 - / 15.9 / 15.8; 300x32003 22.0 / 22.6 / 22.7; 600x32000 32 / 30 /
-// 37; 4096x32000 116 / 129 / 173; 296x128256 50 / 38 / 36; 2048x128256 186 / 176
-// / 203.
+// Warps of a CTA.  With few rows 16, so that a row ends early; with more, and
+// with shorter rows, fewer: more rows are on an SM at once and one's joins pass
+// under another's chunks.  With four rows an SM 8, of which an SM holds just
+// four CTAs: CTAs of 4 gather on some SMs.  us with 4 / 8 / 16 warps:
+//   8 alternatives, bf16: 148x32000 16.7 / 12.3 / 10.5; 296x8000 9.0 / 7.9 / 8.5;
+//   296x32000 18.3 / 15.0 / 14.6; 400x32000 20.2 / 20.7 / 21.3; 592x32000 29.0 /
+//   22.1 / 26.1; 1000x32000 31.6 / 34.9 / 43.3; 444x128256 48.6 / 45.3 / 44.2;
+//   1000x128256 80.7 / 82.4 / 91.5.  20, f32: 2048x128256 203 / 187 / 199;
+//   4096x32000 116 / 133 / 177.
 inline int warps_for(int rows, int n, int cl) {
-  const int most = cl > 1 || rows < 256 ? 16 : n > 65536 ? 8 : 4;
+  const int per_sm = (int)(((long)rows + 147) / 148);
+  const int most = cl > 1 || per_sm == 1 ? 16
+                   : per_sm == 2         ? (n > 16384 ? 16 : 8)
+                   : n > 65536           ? (per_sm == 3 ? 16 : 8)
+                                         : (per_sm == 4 ? 8 : 4);
   const int chunks = (n / cl + 32 * kChunk - 1) / (32 * kChunk);
   int warps = 1;
   while (warps < most && warps < chunks) warps *= 2;
