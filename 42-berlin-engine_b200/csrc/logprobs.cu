@@ -43,7 +43,8 @@ struct LogprobArgs {
   const int* tokens;
   float inv_t;
   int top;
-  int cl;  // CTAs of a row
+  int cl;     // CTAs of a row
+  int depth;  // chunks that a warp's ring holds
   float* logprob;
   float* entropy;
   int* ids;
@@ -164,8 +165,8 @@ __device__ __forceinline__ Stat warp_join(Stat a, float c2) {
   return a;
 }
 
-// A lane's running statistics: the sums in two halves (paired f32
-// arithmetic), joined at the end.
+// Running statistics: the warp's maximum, a lane's sums under it in two halves
+// (paired f32 arithmetic), joined at the end.
 struct Running {
   float m;
   uint64_t s, w;
@@ -184,6 +185,12 @@ __device__ __forceinline__ void rescale(Running& a, float m, float c2) {
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// the largest of the lanes' values (NaN if any is)
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
 // the maximum of kChunk values (NaN if any is)
@@ -254,19 +261,19 @@ struct Warp {
 
   // A chunk: kChunk values a lane, the j-th also at `kept` (this lane's, run
   // j / kPer of 512 bytes a warp) and at index i0 + (j / kPer) * 32 * kPer +
-  // j % kPer; bit j of `valid`: it is one of the row's, else it is -inf.  All
-  // indices lie behind those of earlier chunks.
+  // j % kPer; bit j of `valid`: it is one of the row's, else it is -inf (whole:
+  // all are).  All indices lie behind those of earlier chunks.
   template <typename T, int kPer>
   __device__ __forceinline__ void take(const float* v, const T* kept, int i0, unsigned valid,
-                                       float c2) {
-    const float cm = max_of(v);
+                                       bool whole, float c2) {
+    const float cm = warp_max(max_of(v));
     if (!(cm <= st.m)) rescale(st, max_nan(cm, st.m), c2);
     // (l - m) in units of log 2, its power, and their product.  A logit of
     // -inf makes the product NaN: such chunks, and those with values that are
     // not the row's, are added with these far enough below for it to be 0.
     const uint64_t m2 = pair_of(-st.m, -st.m), c22 = pair_of(c2, c2);
     uint64_t s = st.s, w = st.w;
-    bool plain = !barred && __all_sync(0xffffffffu, valid == (1u << kChunk) - 1u);
+    bool plain = whole && !barred;
     if (plain) {
 #pragma unroll
       for (int j = 0; j < kChunk; j += 2) {
@@ -293,12 +300,12 @@ struct Warp {
     }
     st.s = s;
     st.w = w;
-    if (top && __any_sync(0xffffffffu, !(cm <= thr))) {
+    if (top && !(cm <= thr)) {
       unsigned mine = 0;  // the lane's values that can enter
 #pragma unroll
       for (int j = 0; j < kChunk; j++)
         if (!(v[j] <= thr)) mine |= 1u << j;
-      mine &= valid;
+      if (!whole) mine &= valid;
       // one of each lane's at a time, as long as any can
 #pragma unroll 1
       while (true) {
@@ -353,6 +360,11 @@ __host__ __device__ constexpr int ring_depth() {
   return 6144 / kChunkBytes<T>;
 }
 
+// 16 bytes into shared memory, past L1
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
 // ------------------------------------------------------------------ kernel --
 
 template <typename T>
@@ -360,12 +372,16 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
   constexpr int kPer = 16 / (int)sizeof(T);    // values of one 16-byte copy
   constexpr int kLoads = kChunk / kPer;
   constexpr int D = ring_depth<T>();
-  extern __shared__ __align__(16) uint8_t ring_mem[];  // [warp][D][kLoads][32 lanes][16]
+  extern __shared__ __align__(16) uint8_t ring_mem[];  // [warp][depth][kLoads][32 lanes][16]
   __shared__ T ends[32 * kPer];  // warp 0's: the values outside whole pieces
   __shared__ __align__(16) unsigned held[32];
   __shared__ Stat stats[kMaxWarps];
-  __shared__ u64 lists[kMaxWarps][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  __shared__ int given;
+  __shared__ float given_l;
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  // by a shuffle, from which the compiler knows that all lanes have the same: its
+  // branches need no reconvergence (a sixth of the instructions)
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
   const int rank = blockIdx.x % a.cl;
   const long row = blockIdx.x / a.cl;
   if (threadIdx.x < 32) held[threadIdx.x] = 0;
@@ -400,33 +416,27 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
   const bool back = rank == a.cl - 1 && warp == 0 && head + nv * kPer < a.n;
   // Every lane copies its own pieces D chunks ahead and reads back only what it
   // copied itself, so its own wait is all the synchronisation.
-  T* ring = reinterpret_cast<T*>(ring_mem + (size_t)warp * D * kChunkBytes<T>) + lane * kPer;
+  uint8_t* const own_mem = ring_mem + warp * a.depth * kChunkBytes<T>;
+  T* ring = reinterpret_cast<T*>(own_mem) + lane * kPer;
   constexpr int kSlot = kChunkBytes<T> / (int)sizeof(T);
-  auto fetch = [&](int slot, int b) {
-    T* to = ring + slot * kSlot;
-    const T* from = body + (long)(b + lane) * kPer;
+  const uint32_t ring_at = smem_u32(ring);
+  auto fetch = [&](uint32_t at, const T* from, int b) {
     if (b + 32 * kLoads <= v1) {
 #pragma unroll
-      for (int u = 0; u < kLoads; u++) cp_async16(to + u * 32 * kPer, from + u * 32 * kPer);
+      for (int u = 0; u < kLoads; u++) copy16(at + u * 512, from + u * 32 * kPer);
     } else {
 #pragma unroll
       for (int u = 0; u < kLoads; u++)
-        if (b + u * 32 + lane < v1) cp_async16(to + u * 32 * kPer, from + u * 32 * kPer);
+        if (b + u * 32 + lane < v1) copy16(at + u * 512, from + u * 32 * kPer);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  const T* next = body + (long)(first + lane) * kPer;  // this lane's of the next chunk to copy
 #pragma unroll
-  for (int d = 0; d < D; d++) fetch(d, first + d * step);
+  for (int d = 0; d < D; d++, next += (long)step * kPer)
+    fetch(ring_at + d * kChunkBytes<T>, next, first + d * step);
   // the given token's logit, asked for now and used at the end
-  int token = -1;
-  float token_l = 0.0f;
-  if (a.logprob && rank == 0 && threadIdx.x == 0) {
-    token = a.tokens[row];
-    if (token >= 0 && token < a.n) token_l = to_f32(l[token]);
-  }
-  // a chunk's values, -inf where the row has none; which are the row's
-  auto read = [&](float* v, const T* kept, int b) {
-    unsigned valid = (1u << kChunk) - 1u;
+  auto read = [&](float* v, const T* kept) {
 #pragma unroll
     for (int u = 0; u < kLoads; u++) {
       const uint4 raw = *reinterpret_cast<const uint4*>(kept + u * 32 * kPer);
@@ -434,16 +444,19 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
 #pragma unroll
       for (int k = 0; k < kPer; k++) v[u * kPer + k] = to_f32(e[k]);
     }
-    if (b + 32 * kLoads > v1) {
+  };
+  // the lane's values of chunk b that are the row's
+  auto pieces = [&](int b) {
+    unsigned valid = 0;
 #pragma unroll
-      for (int u = 0; u < kLoads; u++) {
-        if (b + u * 32 + lane < v1) continue;
-        valid &= ~(((1u << kPer) - 1u) << (u * kPer));
-#pragma unroll
-        for (int k = 0; k < kPer; k++) v[u * kPer + k] = -INFINITY;
-      }
-    }
+    for (int u = 0; u < kLoads; u++)
+      if (b + u * 32 + lane < v1) valid |= ((1u << kPer) - 1u) << (u * kPer);
     return valid;
+  };
+  auto clear = [&](float* v, unsigned valid) {
+#pragma unroll
+    for (int j = 0; j < kChunk; j++)
+      if (!(valid >> j & 1)) v[j] = -INFINITY;
   };
   // the warps with a chunk, and the first threshold, from the lane maxima over
   // the chunks under way
@@ -457,7 +470,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
       for (int d = 0; d < D; d++) {
         if (first + d * step < v1) {
           float v[kChunk];
-          read(v, ring + d * kSlot, first + d * step);
+          const int b = first + d * step;
+          read(v, ring + d * kSlot);
+          if (b + 32 * kLoads > v1) clear(v, pieces(b));
           m = max_nan(m, max_of(v));
         }
       }
@@ -470,31 +485,40 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
 #pragma unroll 1
   for (int b = front ? first - step : first; b < v1 || (back && b < v1 + step); b += step) {
     float v[kChunk];
-    unsigned valid;
-    int i0;
-    T* kept = ring + slot * kSlot;
-    const bool whole = b >= first && b < v1;
-    if (whole) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
-      i0 = head + (b + lane) * kPer;
-      valid = read(v, kept, b);
-    } else {
-      const int from = b < first ? 0 : head + nv * kPer, to = b < first ? head : a.n;
-      kept = ends + lane * kPer;
-      i0 = from + lane;
-      valid = i0 < to ? 1u : 0u;
-#pragma unroll
-      for (int j = 0; j < kChunk; j++) v[j] = -INFINITY;
-      if (valid) {
-        kept[0] = l[i0];
-        v[0] = to_f32(kept[0]);
+    const T* kept = ring + slot * kSlot;
+    int i0 = head + (b + lane) * kPer;
+    asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
+    read(v, kept);
+    unsigned valid = 0;
+    const bool whole = b >= first && b + 32 * kLoads <= v1;
+    if (!whole) {
+      if (b >= first && b < v1) {
+        valid = pieces(b);
+      } else {  // an end: a value a lane, of which the copies have nothing
+        const int from = b < first ? 0 : head + nv * kPer, to = b < first ? head : a.n;
+        i0 = from + lane;
+        T* own = ends + lane * kPer;
+        if (i0 < to) {
+          valid = 1u;
+          own[0] = l[i0];
+          v[0] = to_f32(own[0]);
+        }
+        kept = own;
       }
+      clear(v, valid);
     }
-    w.take<T, kPer>(v, kept, i0, valid, c2);
-    if (whole) {
-      fetch(slot, b + D * step);
+    w.take<T, kPer>(v, kept, i0, valid, whole, c2);
+    if (b >= first) {
+      fetch(ring_at + slot * kChunkBytes<T>, next, b + D * step);
+      next += (long)step * kPer;
       slot = slot == D - 1 ? 0 : slot + 1;
     }
+  }
+  // the given token and its logit, by the warp that ends first
+  if (a.logprob && rank == 0 && warp == warps - 1 && lane == 0) {
+    const int t = a.tokens[row];
+    given = t;
+    if (t >= 0 && t < a.n) given_l = to_f32(l[t]);
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 
@@ -502,13 +526,18 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
   Stat st = warp_join(Stat{w.st.m, __fadd_rn(lo_f(w.st.s), hi_f(w.st.s)),
                            __fadd_rn(lo_f(w.st.w), hi_f(w.st.w))}, c2);
   if (lane == 0) stats[warp] = st;
-  lists[warp][lane] = w.key;
+  // its list, where its chunks were (all lanes' copies and reads are over)
+  __syncwarp();
+  auto list_of = [&](int i) {
+    return reinterpret_cast<u64*>(ring_mem + i * a.depth * kChunkBytes<T>);
+  };
+  list_of(warp)[lane] = w.key;
   __syncthreads();
   auto merge_tree = [&](int count) {
     for (int s = 1; s < count; s <<= 1) {
       if (warp % (2 * s) == 0 && warp + s < count) {
-        w.key = merge_lists(w.key, lists[warp + s][31 - lane], lane);
-        lists[warp][lane] = w.key;
+        w.key = merge_lists(w.key, list_of(warp + s)[31 - lane], lane);
+        list_of(warp)[lane] = w.key;
       }
       __syncthreads();
     }
@@ -528,7 +557,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
     if (rank == 0) {
       if (a.top && warp < a.cl) {
         w.key = peer_u64(smem_u32(&block_list[lane]), warp);
-        lists[warp][lane] = w.key;
+        list_of(warp)[lane] = w.key;
       }
       if (warp == 0) {
         Stat p{-INFINITY, 0.0f, 0.0f};
@@ -555,7 +584,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
       a.entropy[row] = lost ? nan : none ? 0.0f
                        : __fsub_rn(logs, __fmul_rn(__fdiv_rn(st.w, st.s), 0.693147181f));
     if (a.logprob)
-      a.logprob[row] = token == -1 ? 0.0f : token >= 0 && token < a.n ? logprob(token_l) : nan;
+      a.logprob[row] = given == -1 ? 0.0f : given >= 0 && given < a.n ? logprob(given_l) : nan;
   }
   if (lane < a.top) {
     a.ids[row * a.top + lane] = (int)~(unsigned)w.key;
@@ -599,7 +628,11 @@ int launch_logprobs(LogprobArgs a, int rows, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)rows * a.cl);
   cfg.blockDim = dim3(warps * 32);
-  cfg.dynamicSmemBytes = (size_t)warps * ring_depth<T>() * kChunkBytes<T>;
+  // a warp's chunks, and one more that the ends' pass over it looks at
+  const int chunks = (a.n / a.cl + 32 * kChunk) / (32 * kChunk);
+  const int each = (chunks + warps - 1) / warps + 1;
+  a.depth = each < ring_depth<T>() ? each : ring_depth<T>();
+  cfg.dynamicSmemBytes = (size_t)warps * a.depth * kChunkBytes<T>;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -637,7 +670,7 @@ extern "C" int ec_op_token_logprobs(int type, const void* logits, int64_t ld, in
                          "both outputs");
   if (top_k > ec::kMaxTop || n > ec::kMaxRows || rows > ec::kMaxRows)
     return ec::unsupported("ec_op_token_logprobs: top_k > 32, or n or rows > 2^30");
-  const ec::LogprobArgs a{logits, (long)ld, n, tokens, 1.0f / temperature, top_k, 1, logprob,
+  const ec::LogprobArgs a{logits, (long)ld, n, tokens, 1.0f / temperature, top_k, 1, 1, logprob,
                           entropy, top_ids, top_logprobs};
   return ec::with_type(type, [&](auto t) {
     return ec::launch_logprobs<decltype(t)>(a, rows, static_cast<cudaStream_t>(stream));
