@@ -13,11 +13,11 @@
 // rows in random order few chunks do (2048x128256: a quarter with 20
 // alternatives, a tenth with 5).
 //
-// One B200, rows from HBM: 2048x128256 f32 with 20 alternatives 177-187 us
-// (5.6-5.9 TB/s), without 165-180; bf16 170 and 120 (issue: 16 and 10
-// instructions a value); one row with 5 alternatives 8.4 us, of which 4 are the
-// dependent steps of thresholds, entries and list merges; 300x32003 bf16, nine
-// tenths of it -inf, with 8 alternatives 18.9 us.
+// One B200, rows from HBM: 2048x128256 f32 with 20 alternatives 162 us (6.5
+// TB/s, the copy peak), bf16 138 and without 99 (issue: 14 and 9 instructions a
+// value); one row with 5 alternatives 7.6 us, of which 3 are the dependent steps
+// of thresholds, entries and list merges; 300x32003 bf16, nine tenths of it -inf,
+// with 8 alternatives 16.4 us.
 //
 // A row is split over a cluster of CTAs while the rows alone do not fill the
 // SMs; the statistics and lists meet in a fixed order through (distributed)
@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
   __shared__ float given_l;
   const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   // by a shuffle, from which the compiler knows that all lanes have the same: its
-  // branches need no reconvergence (a sixth of the instructions)
+  // branches need no reconvergence (7% of the instructions)
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
   const int rank = blockIdx.x % a.cl;
   const long row = blockIdx.x / a.cl;
@@ -395,11 +395,10 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) token_logprobs_kernel(Logpr
   w.thr = __uint_as_float(0x7fc00000u);
   w.lane = lane;
   w.top = a.top;
-  // one / 32 values in all, us: 256x128256 bf16, 16 warps, 5 alternatives 32.5 /
-  // 29.1, 20 35.4 / 33.2, 24 35.2 / 34.5, 32 35.3 / 40.3; 2048x128256 bf16, 8
-  // warps, 5 154.6 / 146.4, 20 171.9 / 170.0, 24 171.1 / 177.5; 4096x32000 f32, 4
-  // warps, 20 116 / 124
-  w.slots = warps >= 8 && a.top <= 20 ? 32 / warps : 1;
+  // one / 32 values in all, us: 16 warps, 200x128256 bf16, 5 alternatives 27.2 /
+  // 24.1, 20 29.6 / 28.0, 32 29.7 / 34.7; 8 warps, 592x32000 f32, 5 19.6 / 18.7, 20
+  // 22.3 / 23.0; 4 warps, 4096x32000 f32, 5 86.6 / 86.9, 20 97 / 106
+  w.slots = warps >= 8 && a.top <= (warps == 16 ? 20 : 12) ? 32 / warps : 1;
   w.held = held;
   w.own = held + warp * w.slots;
 
@@ -602,19 +601,22 @@ inline int cluster_for(int rows, int n) {
 
 // Warps of a CTA.  With few rows 16, so that a row ends early; with more, and
 // with shorter rows, fewer: more rows are on an SM at once and one's joins pass
-// under another's chunks.  With four rows an SM 8, of which an SM holds just
-// four CTAs: CTAs of 4 gather on some SMs.  us with 4 / 8 / 16 warps:
-//   8 alternatives, bf16: 148x32000 16.7 / 12.3 / 10.5; 296x8000 9.0 / 7.9 / 8.5;
-//   296x32000 18.3 / 15.0 / 14.6; 400x32000 20.2 / 20.7 / 21.3; 592x32000 29.0 /
-//   22.1 / 26.1; 1000x32000 31.6 / 34.9 / 43.3; 444x128256 48.6 / 45.3 / 44.2;
-//   1000x128256 80.7 / 82.4 / 91.5.  20, f32: 2048x128256 203 / 187 / 199;
-//   4096x32000 116 / 133 / 177.
-inline int warps_for(int rows, int n, int cl) {
+// under another's chunks.  8 where there are four to six rows an SM, which hold
+// just four CTAs of it at once: CTAs of 4 gather on some SMs.  us with 4 / 8 / 16
+// warps:
+//   5 alternatives, f32: 148x32000 13.1 / 10.2 / 9.8; 296x8000 8.2 / 7.5 / 8.1;
+//   300x32003 15.7 / 16.8 / 17.7; 700x32000 25.9 / 23.2 / 28.9; 4096x32000 86.6 /
+//   92.4 / 134.7; 296x128256 34.7 / 29.6 / 29.8; 2048x128256 162 / 157 / 157.
+//   bf16: 300x128256 35.9 / 37.0 / 33.8; with 20 38.7 with 16, 43.1 with 8;
+//   2048x128256 with 20 135.6 / 144.1 / 160.6 (bound by issue, f32 rows by HBM).
+template <typename T>
+int warps_for(int rows, int n, int cl) {
   const int per_sm = (int)(((long)rows + 147) / 148);
+  const bool wide = n > 65536;
   const int most = cl > 1 || per_sm == 1 ? 16
-                   : per_sm == 2         ? (n > 16384 ? 16 : 8)
-                   : n > 65536           ? (per_sm == 3 ? 16 : 8)
-                                         : (per_sm == 4 ? 8 : 4);
+                   : per_sm <= 3         ? (wide ? 16 : per_sm == 2 ? 8 : 4)
+                   : per_sm <= 6         ? 8
+                                         : (wide && (sizeof(T) == 4 || per_sm <= 8) ? 8 : 4);
   const int chunks = (n / cl + 32 * kChunk - 1) / (32 * kChunk);
   int warps = 1;
   while (warps < most && warps < chunks) warps *= 2;
@@ -624,7 +626,7 @@ inline int warps_for(int rows, int n, int cl) {
 template <typename T>
 int launch_logprobs(LogprobArgs a, int rows, cudaStream_t st) {
   a.cl = cluster_for(rows, a.n);
-  const int warps = warps_for(rows, a.n, a.cl);
+  const int warps = warps_for<T>(rows, a.n, a.cl);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)rows * a.cl);
   cfg.blockDim = dim3(warps * 32);
