@@ -8,8 +8,9 @@
 //
 // Bytes bound both (a few operations a byte), so a row is read once and held
 // in registers, F values a thread, until its scale is known (rows_kernel).
-// CTAs walk over rows; the next row is copied into shared memory while this
-// one is reduced and stored, so loads stay under way through the reductions.
+// A row comes through shared memory by asynchronous copies.  CTAs that share an
+// SM take one row each and cover one another; one alone on its SM walks over
+// rows, the next one's copies under way while this one is reduced and stored.
 // Aligned rows: every thread copies and reads back its own 16-byte pieces, and
 // needs no barrier for them.  Others are copied at their own alignment (the
 // ends element by element) and read back in pieces that are aligned in the
@@ -19,7 +20,7 @@
 // One B200, inputs from HBM: residual + norm of 8192x8192 f32 132 us (6.6 TB/s,
 // the copy peak), bf16 80 us (5.9 TB/s, 72% of the issue slots); SwiGLU of
 // 4096x28672 bf16 97 us (6.0 TB/s); one row of 4096 2.3 us, two barriers and a
-// memory round trip over an empty launch.
+// memory round trip over an empty launch; 333x5003 f16 norm, unaligned, 6.3 us.
 #include <type_traits>
 
 #include "typed.cuh"
@@ -617,52 +618,50 @@ inline bool aligned(const void* p, long ld, size_t esize, size_t to) {
 
 constexpr size_t kStageMax = 224 * 1024;  // an SM's shared memory, less the reductions'
 
-// How the rows are handled: values a thread, and rows a CTA.
-struct Shape {
-  int f;
-  int rows_per_cta;  // where several CTAs share an SM
-};
-
-// Few rows: 8 values a thread, more threads hide a row's latency (us, norm,
+// Values a thread.  Few rows: 8, more threads hide a row's latency (us, norm,
 // 64x8192 bf16: 3.3 with 8, 3.6 with 16, 4.9 with 32).  Many: 16 of f32 (8192x8192:
-// 132; 184 with 8, 149 with 32) and 32 of 16-bit rows (80; 155, 98), fewer
-// reductions a value, 16 of short ones; 16-bit rows two a CTA (SwiGLU 8192x1024:
-// 9.2; 9.8 with one).  Unaligned rows carry more a thread besides: 16, two a CTA
-// (4000x5003 bf16 norm: 55; 112 with 8, 57 with 32; 59 with one).
+// 132; 142 with 8, 145 with 32) and 32 of 16-bit rows (8192x4096: 43; 71 with 8, 49
+// with 16), fewer reductions a value; 16 of some rows an SM (333x4096: 4.5; 5.6 with
+// 8, 5.5 with 32) and of short ones.  Unaligned rows carry more a thread besides: 16
+// (200x5003 bf16: 6.5; 9.4 with 8, 7.7 with 32), 32 of many or long 16-bit ones
+// (4000x5003: 50; 59 with 16), 8 of short ones (300x1003: 4.4; 4.9 with 16).
 template <typename T>
-Shape shape_of(int rows, int n, bool vec) {
-  const bool few = rows < 148 * 2;
-  if (!vec) return Shape{16, few ? 1 : 2};
-  if (few) return Shape{8, 1};
-  if (sizeof(T) == 4) return Shape{16, 1};
-  return Shape{n >= 4096 ? 32 : 16, 2};
+int values_a_thread(int rows, int n, bool vec) {
+  const bool half = sizeof(T) == 2;
+  if (!vec) {
+    if (n < 2048 && rows < 148 * 8) return 8;
+    return half && (n >= 8192 || (n >= 4096 && rows >= 148 * 4)) ? 32 : 16;
+  }
+  if (rows < 148 * 2 || (n < 4096 && rows < 148 * 4)) return 8;
+  return half && n >= 4096 && rows >= 148 * 4 ? 32 : 16;
 }
 
 // Launches the kernel of the row's alignment and size; `wide` where a row fits
 // neither the registers nor the shared memory.  `extra`: shared memory for the
 // weights.
 template <typename T, typename Args, typename Pick>
-int rows_launch(Args a, bool vec, Shape s, size_t extra, void (*wide)(Args), Pick pick,
+int rows_launch(Args a, bool vec, int f, size_t extra, void (*wide)(Args), Pick pick,
                 cudaStream_t st) {
   constexpr int per = 16 / (int)sizeof(T);
   const int span = vec ? a.n : a.n + per - 1;  // with the lead
-  while (s.f < 32 && span > s.f * kMaxThr) s.f *= 2;
+  while (f < 32 && span > f * kMaxThr) f *= 2;
   if (!vec) extra += Part<T, 8, false>::bytes(a.n);
   const size_t pair = 2 * (vec ? Part<T, 8, true>::room(a.n) : Part<T, 8, false>::room(a.n));
-  a.buffers = !vec && extra + 2 * pair <= kStageMax ? 2 : 1;
-  const size_t smem = extra + a.buffers * pair;
-  if (span > s.f * kMaxThr || smem > kStageMax)
+  size_t smem = extra + pair;
+  if (span > f * kMaxThr || smem > kStageMax)
     return launch(wide, a, a.rows, kWideThr, (size_t)a.n * 4, st);
-  const int threads = ((span + s.f - 1) / s.f + 31) / 32 * 32;
+  const int threads = ((span + f - 1) / f + 31) / 32 * 32;
   // CTAs that an SM holds: by threads (64 registers each) and shared memory.
   // Alone on its SM a CTA walks all its rows, the next one's copies under this
   // one's reductions (4096x28672 bf16 SwiGLU: 95 us; 125 with one row a CTA).
   // Several on an SM cover one another, and rows handed out as CTAs end even
-  // out the SMs' different speeds (8192x8192 f32 norm: 132; 163 walking).
+  // out the SMs' different speeds (8192x8192 f32 norm: 132; 163 walking); two
+  // rows a CTA were slower too (333x5003 bf16: 10.2; 8.1 with one).
   const bool alone = kMaxThr / threads < 2 || kStageMax / (smem + 1024) < 2;
-  const int grid = alone ? (a.rows < 148 ? a.rows : 148)
-                         : (a.rows + s.rows_per_cta - 1) / s.rows_per_cta;
-  return launch(pick(s.f, vec), a, grid, threads, smem, st);
+  a.buffers = alone && !vec && smem + pair <= kStageMax ? 2 : 1;
+  if (a.buffers == 2) smem += pair;
+  const int grid = alone && a.rows > 148 ? 148 : a.rows;
+  return launch(pick(f, vec), a, grid, threads, smem, st);
 }
 
 template <typename T>
@@ -672,9 +671,9 @@ int norm_rows(const NormArgs& a, cudaStream_t st) {
                    (!a.r || aligned(a.r, a.ldr, sizeof(T), 16)) &&
                    (!a.h || aligned(a.h, a.ldh, sizeof(T), 16)) &&
                    (!a.w || aligned(a.w, 0, 2, 2 * per)) && aligned(a.q, a.ldq, 1, per);
-  const Shape s = shape_of<T>(a.rows, a.n, vec);
+  const int f = values_a_thread<T>(a.rows, a.n, vec);
   const size_t extra = !vec && a.w ? Part<__nv_bfloat16, 8, false>::room(a.n) : 0;
-  return rows_launch<T>(a, vec, s, extra, norm_wide_kernel<T>, [](int f, bool v) {
+  return rows_launch<T>(a, vec, f, extra, norm_wide_kernel<T>, [](int f, bool v) {
     return v ? (f == 8 ? norm_rows_kernel<T, 8, true>
                        : f == 16 ? norm_rows_kernel<T, 16, true> : norm_rows_kernel<T, 32, true>)
              : (f == 8 ? norm_rows_kernel<T, 8, false>
@@ -687,8 +686,8 @@ int silu_rows(const SiluArgs& a, cudaStream_t st) {
   constexpr int per = 16 / (int)sizeof(T);
   const bool vec = a.n % per == 0 && aligned(a.g, a.ld, sizeof(T), 16) &&
                    aligned(a.u, a.ld, sizeof(T), 16) && aligned(a.q, a.ldq, 1, per);
-  const Shape s = shape_of<T>(a.rows, a.n, vec);
-  return rows_launch<T>(a, vec, s, 0, silu_wide_kernel<T>, [](int f, bool v) {
+  const int f = values_a_thread<T>(a.rows, a.n, vec);
+  return rows_launch<T>(a, vec, f, 0, silu_wide_kernel<T>, [](int f, bool v) {
     return v ? (f == 8 ? silu_rows_kernel<T, 8, true>
                        : f == 16 ? silu_rows_kernel<T, 16, true> : silu_rows_kernel<T, 32, true>)
              : (f == 8 ? silu_rows_kernel<T, 8, false>
