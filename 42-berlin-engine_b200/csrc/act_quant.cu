@@ -166,15 +166,6 @@ __device__ __forceinline__ uint32_t narrow(uint64_t v) {  // to the nearest, tie
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi_f(v)), "f"(lo_f(v)));
   return w;
 }
-// a pair rounded to T
-template <typename T>
-__device__ __forceinline__ uint64_t rounded(uint64_t v) {
-  if constexpr (sizeof(T) == 4)
-    return v;
-  else
-    return widen<T>(narrow<T>(v));
-}
-
 // 16 bytes at any place of shared memory: two aligned reads, moved down by words
 // and by the rest.  The place within 16 bytes is the same for all of a row's
 // pieces, so the branches are uniform.
@@ -199,12 +190,17 @@ __device__ __forceinline__ uint4 read_shifted(const uint8_t* p) {
   return a;
 }
 
+// How a row lies: in whole pieces of 16 bytes, F values for every thread; in whole
+// pieces, of which some threads have fewer; anyhow.
+enum Lie { kFull, kPieces, kAnyhow };
+
 // A thread's part of a row: F values in pairs, in runs of one 16-byte piece
-// (kPer elements), every kPer * blockDim.x apart.  VEC: the row is whole
-// pieces.  Else its first piece starts `lead` elements before the row, and
-// what lies outside the row counts as zero.
-template <typename T, int F, bool VEC>
+// (kPer elements), every kPer * blockDim.x apart.  kAnyhow: the row's first
+// piece starts `lead` elements before it, and what lies outside the row counts
+// as zero.
+template <typename T, int F, Lie L>
 struct Part {
+  static constexpr bool VEC = L != kAnyhow;
   static constexpr int kPer = 16 / (int)sizeof(T);
   static constexpr int kRuns = F / kPer;
   static constexpr int kPairs = kPer / 2;
@@ -215,6 +211,8 @@ struct Part {
     const int i = (run * (int)blockDim.x + (int)threadIdx.x) * kPer;
     return VEC ? i : i - lead;
   }
+  // whether the thread has no run that starts at element i
+  __device__ __forceinline__ bool beyond(int i) const { return L != kFull && i >= n; }
   __device__ __forceinline__ bool inside(int i) const { return VEC || (i >= 0 && i + kPer <= n); }
   // elements by which a row starts behind a 16-byte boundary
   static __device__ __forceinline__ int misplaced(const T* row) {
@@ -236,7 +234,7 @@ struct Part {
 #pragma unroll
       for (int run = 0; run < kRuns; run++) {
         const int i = at(run);
-        if (i < n) cp_async16(dst + i, row + i);
+        if (!beyond(i)) cp_async16(dst + i, row + i);
       }
     } else {
       const int mis = misplaced(row), head = min(n, mis ? kPer - mis : 0);
@@ -264,9 +262,11 @@ struct Part {
   // the run's values of a staged row
   __device__ __forceinline__ void load(const T* row, int run, uint64_t* v) const {
     const int i = at(run);
+    if constexpr (L != kFull) {
 #pragma unroll
-    for (int k = 0; k < kPairs; k++) v[k] = 0;
-    if (i >= n) return;
+      for (int k = 0; k < kPairs; k++) v[k] = 0;
+      if (i >= n) return;
+    }
     if constexpr (VEC)
       spread(*reinterpret_cast<const uint4*>(row + i), v);
     else
@@ -284,9 +284,11 @@ struct Part {
   // as they were staged
   __device__ __forceinline__ void load_w(const uint16_t* w, int run, uint64_t* v) const {
     const int i = at(run);
+    if constexpr (L != kFull) {
 #pragma unroll
-    for (int k = 0; k < kPairs; k++) v[k] = 0;
-    if (i >= n) return;
+      for (int k = 0; k < kPairs; k++) v[k] = 0;
+      if (i >= n) return;
+    }
     uint4 raw;
     if constexpr (VEC) {
       if constexpr (kPairs == 4) {
@@ -305,24 +307,26 @@ struct Part {
       v[3] = widen<__nv_bfloat16>(raw.w);
     }
   }
-  __device__ __forceinline__ void store(T* row, int run, const uint64_t* v) const {
-    const int i = at(run);
-    if (i >= n) return;
-    uint32_t raw[4];
+  // the run's values rounded to T, as they lie in memory (raw) and as they are
+  static __device__ __forceinline__ uint4 round_run(uint64_t* v) {
     if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int k = 0; k < 2; k++) {
-        raw[2 * k] = (uint32_t)v[k];
-        raw[2 * k + 1] = (uint32_t)(v[k] >> 32);
-      }
+      return make_uint4((uint32_t)v[0], (uint32_t)(v[0] >> 32), (uint32_t)v[1],
+                        (uint32_t)(v[1] >> 32));
     } else {
-#pragma unroll
-      for (int k = 0; k < 4; k++) raw[k] = narrow<T>(v[k]);
+      const uint4 raw = make_uint4(narrow<T>(v[0]), narrow<T>(v[1]), narrow<T>(v[2]),
+                                   narrow<T>(v[3]));
+      spread(raw, v);
+      return raw;
     }
+  }
+  __device__ __forceinline__ void store(T* row, int run, const uint4& raw) const {
+    const int i = at(run);
+    if (beyond(i)) return;
     if (inside(i)) {
-      *reinterpret_cast<uint4*>(row + i) = make_uint4(raw[0], raw[1], raw[2], raw[3]);
+      *reinterpret_cast<uint4*>(row + i) = raw;
     } else {
-      const T* e = reinterpret_cast<const T*>(raw);
+      const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
+      const T* e = reinterpret_cast<const T*>(word);
 #pragma unroll
       for (int k = 0; k < kPer; k++)
         if (i + k >= 0 && i + k < n) row[i + k] = e[k];
@@ -337,16 +341,17 @@ struct Part {
     const float f = quant_factor(amax_bits);
     if (threadIdx.x == 0) *scale = quant_scale(amax_bits);
     const uint64_t f2 = both(f);
+    const bool zeros = f == 0.0f;
     uint8_t* to = VEC ? reinterpret_cast<uint8_t*>(q) : held + 16 + lead;  // element 0's place
 #pragma unroll
     for (int run = 0; run < kRuns; run++) {
       const int i = at(run);
-      if (i >= n) continue;
+      if (beyond(i)) continue;
       const uint64_t* v = y + run * kPairs;
       uint32_t b[kPer / 4];
 #pragma unroll
       for (int k = 0; k < kPer / 4; k++)
-        b[k] = f != 0.0f ? quant4(v[2 * k], v[2 * k + 1], f2) : 0u;
+        b[k] = zeros ? 0u : quant4(v[2 * k], v[2 * k + 1], f2);
       if constexpr (kPer == 8)
         *reinterpret_cast<uint2*>(to + i) = make_uint2(b[0], b[1]);
       else
@@ -386,10 +391,10 @@ __device__ __forceinline__ void copies_wait() {
 //     fit), and a barrier before a row is read: all threads' copies of it have
 //     landed, and all have read the buffer that is filled next.
 // f(row, a, b, next): a, b the staged row; calls next() once they are read.
-template <typename T, int F, bool VEC, typename Body>
+template <typename T, int F, Lie L, typename Body>
 __device__ __forceinline__ void walk_rows(uint8_t* smem, const T* a, long lda, const T* b, long ldb,
                                           int n, int rows, int buffers, Body f) {
-  using P = Part<T, F, VEC>;
+  using P = Part<T, F, L>;
   const P part{n, 0};
   const size_t room = P::room(n);
   const int step = gridDim.x;
@@ -408,7 +413,7 @@ __device__ __forceinline__ void walk_rows(uint8_t* smem, const T* a, long lda, c
     const T* pa = P::place(from, a + row * lda);
     const T* pb = b ? P::place(from + room, b + row * ldb) : nullptr;
     copies_wait<0>();
-    if constexpr (VEC) {
+    if constexpr (P::VEC) {
       f(row, pa, pb, [&] { stage(row + step, 0); });
     } else {
       __syncthreads();
@@ -424,9 +429,9 @@ __device__ __forceinline__ void walk_rows(uint8_t* smem, const T* a, long lda, c
 
 // --------------------------------------------------------------- the kernels --
 
-template <typename T, int F, bool VEC>
+template <typename T, int F, Lie L>
 __global__ void __launch_bounds__(kMaxThr) norm_rows_kernel(NormArgs a) {
-  using P = Part<T, F, VEC>;
+  using P = Part<T, F, L>;
   extern __shared__ __align__(16) uint8_t stage_mem[];
   __shared__ double red[32];
   __shared__ unsigned redu[32];
@@ -435,9 +440,9 @@ __global__ void __launch_bounds__(kMaxThr) norm_rows_kernel(NormArgs a) {
   uint8_t* held = stage_mem;  // the row's bytes
   uint8_t* rows_mem = stage_mem + P::bytes(a.n);
   const uint16_t* w = a.w;
-  if constexpr (!VEC) {
+  if constexpr (L == kAnyhow) {
     // the weights too are read shifted: staged once, before any row's barrier
-    using W = Part<__nv_bfloat16, 8, false>;
+    using W = Part<__nv_bfloat16, 8, kAnyhow>;
     if (a.w) {
       const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(a.w);
       W{a.n, 0}.stage(rows_mem, src, 2);
@@ -445,7 +450,7 @@ __global__ void __launch_bounds__(kMaxThr) norm_rows_kernel(NormArgs a) {
       rows_mem += W::room(a.n);
     }
   }
-  walk_rows<T, F, VEC>(
+  walk_rows<T, F, L>(
       rows_mem, static_cast<const T*>(a.x), a.ldx, static_cast<const T*>(a.r), a.ldr, a.n, a.rows,
       a.buffers, [&](long row, const T* x, const T* r, auto next) {
         T* h = a.h ? static_cast<T*>(a.h) + row * a.ldh : nullptr;
@@ -459,7 +464,11 @@ __global__ void __launch_bounds__(kMaxThr) norm_rows_kernel(NormArgs a) {
             uint64_t b[P::kPairs];
             part.load(r, run, b);
 #pragma unroll
-            for (int k = 0; k < P::kPairs; k++) vr[k] = rounded<T>(add2(vr[k], b[k]));
+            for (int k = 0; k < P::kPairs; k++) vr[k] = add2(vr[k], b[k]);
+          }
+          if (r || h) {
+            const uint4 raw = P::round_run(vr);
+            if (h) part.store(h, run, raw);
           }
         }
         next();
@@ -471,10 +480,6 @@ __global__ void __launch_bounds__(kMaxThr) norm_rows_kernel(NormArgs a) {
 #pragma unroll
           for (int k = 1; k < P::kPairs; k++) fma2(s, vr[k], vr[k]);
           ss += (double)__fadd_rn(lo_f(s), hi_f(s));
-        }
-        if (h) {
-#pragma unroll
-          for (int run = 0; run < P::kRuns; run++) part.store(h, run, v + run * P::kPairs);
         }
         const float inv = norm_factor(block_sum(ss, red), a.inv_n, a.eps);
         float m = 0.0f;
@@ -500,15 +505,15 @@ __global__ void __launch_bounds__(kMaxThr) norm_rows_kernel(NormArgs a) {
       });
 }
 
-template <typename T, int F, bool VEC>
+template <typename T, int F, Lie L>
 __global__ void __launch_bounds__(kMaxThr) silu_rows_kernel(SiluArgs a) {
-  using P = Part<T, F, VEC>;
+  using P = Part<T, F, L>;
   extern __shared__ __align__(16) uint8_t stage_mem[];
   __shared__ unsigned redu[2][32];  // by the row's parity: one barrier a row
   int parity = 0;
   pdl_wait();
   pdl_launch_dependents();
-  walk_rows<T, F, VEC>(
+  walk_rows<T, F, L>(
       stage_mem + P::bytes(a.n), static_cast<const T*>(a.g), a.ld, static_cast<const T*>(a.u), a.ld, a.n, a.rows,
       a.buffers, [&](long row, const T* g, const T* u, auto next) {
         const P part{a.n, P::misplaced(static_cast<const T*>(a.g) + row * a.ld)};
@@ -645,8 +650,8 @@ int rows_launch(Args a, bool vec, int f, size_t extra, void (*wide)(Args), Pick 
   constexpr int per = 16 / (int)sizeof(T);
   const int span = vec ? a.n : a.n + per - 1;  // with the lead
   while (f < 32 && span > f * kMaxThr) f *= 2;
-  if (!vec) extra += Part<T, 8, false>::bytes(a.n);
-  const size_t pair = 2 * (vec ? Part<T, 8, true>::room(a.n) : Part<T, 8, false>::room(a.n));
+  if (!vec) extra += Part<T, 8, kAnyhow>::bytes(a.n);
+  const size_t pair = 2 * (vec ? Part<T, 8, kPieces>::room(a.n) : Part<T, 8, kAnyhow>::room(a.n));
   size_t smem = extra + pair;
   if (span > f * kMaxThr || smem > kStageMax)
     return launch(wide, a, a.rows, kWideThr, (size_t)a.n * 4, st);
@@ -661,7 +666,21 @@ int rows_launch(Args a, bool vec, int f, size_t extra, void (*wide)(Args), Pick 
   a.buffers = alone && !vec && smem + pair <= kStageMax ? 2 : 1;
   if (a.buffers == 2) smem += pair;
   const int grid = alone && a.rows > 148 ? 148 : a.rows;
-  return launch(pick(f, vec), a, grid, threads, smem, st);
+  return launch(pick(f, !vec ? kAnyhow : f * threads == a.n ? kFull : kPieces), a, grid, threads,
+                smem, st);
+}
+
+template <typename T, int F>
+auto norm_kernel_of(Lie l) {
+  return l == kFull     ? norm_rows_kernel<T, F, kFull>
+         : l == kPieces ? norm_rows_kernel<T, F, kPieces>
+                        : norm_rows_kernel<T, F, kAnyhow>;
+}
+template <typename T, int F>
+auto silu_kernel_of(Lie l) {
+  return l == kFull     ? silu_rows_kernel<T, F, kFull>
+         : l == kPieces ? silu_rows_kernel<T, F, kPieces>
+                        : silu_rows_kernel<T, F, kAnyhow>;
 }
 
 template <typename T>
@@ -672,12 +691,9 @@ int norm_rows(const NormArgs& a, cudaStream_t st) {
                    (!a.h || aligned(a.h, a.ldh, sizeof(T), 16)) &&
                    (!a.w || aligned(a.w, 0, 2, 2 * per)) && aligned(a.q, a.ldq, 1, per);
   const int f = values_a_thread<T>(a.rows, a.n, vec);
-  const size_t extra = !vec && a.w ? Part<__nv_bfloat16, 8, false>::room(a.n) : 0;
-  return rows_launch<T>(a, vec, f, extra, norm_wide_kernel<T>, [](int f, bool v) {
-    return v ? (f == 8 ? norm_rows_kernel<T, 8, true>
-                       : f == 16 ? norm_rows_kernel<T, 16, true> : norm_rows_kernel<T, 32, true>)
-             : (f == 8 ? norm_rows_kernel<T, 8, false>
-                       : f == 16 ? norm_rows_kernel<T, 16, false> : norm_rows_kernel<T, 32, false>);
+  const size_t extra = !vec && a.w ? Part<__nv_bfloat16, 8, kAnyhow>::room(a.n) : 0;
+  return rows_launch<T>(a, vec, f, extra, norm_wide_kernel<T>, [](int f, Lie l) {
+    return f == 8 ? norm_kernel_of<T, 8>(l) : f == 16 ? norm_kernel_of<T, 16>(l) : norm_kernel_of<T, 32>(l);
   }, st);
 }
 
@@ -687,11 +703,8 @@ int silu_rows(const SiluArgs& a, cudaStream_t st) {
   const bool vec = a.n % per == 0 && aligned(a.g, a.ld, sizeof(T), 16) &&
                    aligned(a.u, a.ld, sizeof(T), 16) && aligned(a.q, a.ldq, 1, per);
   const int f = values_a_thread<T>(a.rows, a.n, vec);
-  return rows_launch<T>(a, vec, f, 0, silu_wide_kernel<T>, [](int f, bool v) {
-    return v ? (f == 8 ? silu_rows_kernel<T, 8, true>
-                       : f == 16 ? silu_rows_kernel<T, 16, true> : silu_rows_kernel<T, 32, true>)
-             : (f == 8 ? silu_rows_kernel<T, 8, false>
-                       : f == 16 ? silu_rows_kernel<T, 16, false> : silu_rows_kernel<T, 32, false>);
+  return rows_launch<T>(a, vec, f, 0, silu_wide_kernel<T>, [](int f, Lie l) {
+    return f == 8 ? silu_kernel_of<T, 8>(l) : f == 16 ? silu_kernel_of<T, 16>(l) : silu_kernel_of<T, 32>(l);
   }, st);
 }
 
