@@ -147,7 +147,7 @@ __device__ __forceinline__ uint64_t silu_mul(uint64_t g, uint64_t u) {
   return mul2(mul2(g, pack2(__float_as_uint(s0), __float_as_uint(s1))), u);
 }
 
-// two elements of T in a word (f32: in two) <-> a pair of f32
+// two elements of T in a word as a pair of f32
 template <typename T>
 __device__ __forceinline__ uint64_t widen(uint32_t w) {
   if constexpr (sizeof(T) == 2) {
@@ -157,15 +157,26 @@ __device__ __forceinline__ uint64_t widen(uint32_t w) {
   }
   return 0;
 }
+// Sums of a 16-byte piece's elements, rounded to T once: in 16 bits the exact sum
+// is, and the f32 sum rounded again gives the same (what f32 cannot hold of it
+// lies far below half a step of T).
 template <typename T>
-__device__ __forceinline__ uint32_t narrow(uint64_t v) {  // to the nearest, ties to even
-  uint32_t w;
-  if constexpr (std::is_same<T, __nv_bfloat16>::value)
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi_f(v)), "f"(lo_f(v)));
+__device__ __forceinline__ uint32_t sum_word(uint32_t a, uint32_t b) {
+  uint32_t s;
+  if constexpr (std::is_same<T, float>::value)
+    s = __float_as_uint(__fadd_rn(__uint_as_float(a), __uint_as_float(b)));
+  else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(s) : "r"(a), "r"(b));
   else
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi_f(v)), "f"(lo_f(v)));
-  return w;
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(s) : "r"(a), "r"(b));
+  return s;
 }
+template <typename T>
+__device__ __forceinline__ uint4 sum_piece(const uint4& a, const uint4& b) {
+  return make_uint4(sum_word<T>(a.x, b.x), sum_word<T>(a.y, b.y), sum_word<T>(a.z, b.z),
+                    sum_word<T>(a.w, b.w));
+}
+
 // 16 bytes at any place of shared memory: two aligned reads, moved down by words
 // and by the rest.  The place within 16 bytes is the same for all of a row's
 // pieces, so the branches are uniform.
@@ -190,6 +201,27 @@ __device__ __forceinline__ uint4 read_shifted(const uint8_t* p) {
   return a;
 }
 
+// What lies `bytes` behind a base that all threads share: an unsigned 32-bit
+// offset, which the hardware adds to it.
+template <typename U>
+__device__ __forceinline__ const U& behind(const void* base, uint32_t bytes) {
+  return *reinterpret_cast<const U*>(static_cast<const uint8_t*>(base) + bytes);
+}
+template <typename U>
+__device__ __forceinline__ U& behind(void* base, uint32_t bytes) {
+  return *reinterpret_cast<U*>(static_cast<uint8_t*>(base) + bytes);
+}
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ uint4 shared16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+
 // How a row lies: in whole pieces of 16 bytes, F values for every thread; in whole
 // pieces, of which some threads have fewer; anyhow.
 enum Lie { kFull, kPieces, kAnyhow };
@@ -210,6 +242,10 @@ struct Part {
   __device__ __forceinline__ int at(int run) const {
     const int i = (run * (int)blockDim.x + (int)threadIdx.x) * kPer;
     return VEC ? i : i - lead;
+  }
+  // VEC: the run's first 16-byte piece, counted in them
+  __device__ __forceinline__ uint32_t piece(int run) const {
+    return run * blockDim.x + threadIdx.x;
   }
   // whether the thread has no run that starts at element i
   __device__ __forceinline__ bool beyond(int i) const { return L != kFull && i >= n; }
@@ -232,10 +268,9 @@ struct Part {
     T* dst = place(room, row);
     if constexpr (VEC) {
 #pragma unroll
-      for (int run = 0; run < kRuns; run++) {
-        const int i = at(run);
-        if (!beyond(i)) cp_async16(dst + i, row + i);
-      }
+      for (int run = 0; run < kRuns; run++)
+        if (!beyond(at(run)))
+          copy16(smem_u32(room) + piece(run) * 16, &behind<uint4>(row, piece(run) * 16));
     } else {
       const int mis = misplaced(row), head = min(n, mis ? kPer - mis : 0);
       const int pieces = (n - head) / kPer, tail = n - head - pieces * kPer;
@@ -259,19 +294,29 @@ struct Part {
       v[3] = widen<T>(raw.w);
     }
   }
-  // the run's values of a staged row
-  __device__ __forceinline__ void load(const T* row, int run, uint64_t* v) const {
+  // the run of a staged row, zero where the row has nothing
+  __device__ __forceinline__ uint4 load(const T* row, int run) const {
     const int i = at(run);
-    if constexpr (L != kFull) {
-#pragma unroll
-      for (int k = 0; k < kPairs; k++) v[k] = 0;
-      if (i >= n) return;
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (beyond(i)) return raw;
+    if constexpr (VEC) {
+      raw = shared16(smem_u32(row) + piece(run) * 16);
+    } else {
+      raw = read_shifted(reinterpret_cast<const uint8_t*>(row + i));
+      if (!inside(i)) {
+        raw.x = only_inside(raw.x, i);
+        raw.y = only_inside(raw.y, i + kPer / 4);
+        raw.z = only_inside(raw.z, i + kPer / 2);
+        raw.w = only_inside(raw.w, i + kPer * 3 / 4);
+      }
     }
-    if constexpr (VEC)
-      spread(*reinterpret_cast<const uint4*>(row + i), v);
-    else
-      spread(read_shifted(reinterpret_cast<const uint8_t*>(row + i)), v);
-    if (!inside(i)) clear_outside(run, v);
+    return raw;
+  }
+  // a word whose first element is the row's i-th, without what lies outside
+  __device__ __forceinline__ uint32_t only_inside(uint32_t word, int i) const {
+    if constexpr (sizeof(T) == 4) return i >= 0 && i < n ? word : 0u;
+    return word & ((i >= 0 && i < n ? 0xffffu : 0u) |
+                   (i + 1 >= 0 && i + 1 < n ? 0xffff0000u : 0u));
   }
   __device__ __forceinline__ void clear_outside(int run, uint64_t* v) const {
     const int i = at(run);
@@ -292,9 +337,9 @@ struct Part {
     uint4 raw;
     if constexpr (VEC) {
       if constexpr (kPairs == 4) {
-        raw = *reinterpret_cast<const uint4*>(w + i);
+        raw = behind<uint4>(w, piece(run) * 16);
       } else {
-        const uint2 two = *reinterpret_cast<const uint2*>(w + i);
+        const uint2 two = behind<uint2>(w, piece(run) * 8);
         raw = make_uint4(two.x, two.y, 0, 0);
       }
     } else {
@@ -307,22 +352,12 @@ struct Part {
       v[3] = widen<__nv_bfloat16>(raw.w);
     }
   }
-  // the run's values rounded to T, as they lie in memory (raw) and as they are
-  static __device__ __forceinline__ uint4 round_run(uint64_t* v) {
-    if constexpr (sizeof(T) == 4) {
-      return make_uint4((uint32_t)v[0], (uint32_t)(v[0] >> 32), (uint32_t)v[1],
-                        (uint32_t)(v[1] >> 32));
-    } else {
-      const uint4 raw = make_uint4(narrow<T>(v[0]), narrow<T>(v[1]), narrow<T>(v[2]),
-                                   narrow<T>(v[3]));
-      spread(raw, v);
-      return raw;
-    }
-  }
   __device__ __forceinline__ void store(T* row, int run, const uint4& raw) const {
     const int i = at(run);
     if (beyond(i)) return;
-    if (inside(i)) {
+    if constexpr (VEC) {
+      behind<uint4>(row, piece(run) * 16) = raw;
+    } else if (inside(i)) {
       *reinterpret_cast<uint4*>(row + i) = raw;
     } else {
       const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
@@ -342,7 +377,7 @@ struct Part {
     if (threadIdx.x == 0) *scale = quant_scale(amax_bits);
     const uint64_t f2 = both(f);
     const bool zeros = f == 0.0f;
-    uint8_t* to = VEC ? reinterpret_cast<uint8_t*>(q) : held + 16 + lead;  // element 0's place
+    uint8_t* to = held + 16 + lead;  // element 0's place (not VEC)
 #pragma unroll
     for (int run = 0; run < kRuns; run++) {
       const int i = at(run);
@@ -352,10 +387,14 @@ struct Part {
 #pragma unroll
       for (int k = 0; k < kPer / 4; k++)
         b[k] = zeros ? 0u : quant4(v[2 * k], v[2 * k + 1], f2);
-      if constexpr (kPer == 8)
+      if constexpr (VEC && kPer == 8)
+        behind<uint2>(q, piece(run) * 8) = make_uint2(b[0], b[1]);
+      else if constexpr (VEC)
+        behind<uint32_t>(q, piece(run) * 4) = b[0];
+      else if constexpr (kPer == 8)
         *reinterpret_cast<uint2*>(to + i) = make_uint2(b[0], b[1]);
       else
-        *reinterpret_cast<unsigned*>(to + i) = b[0];
+        *reinterpret_cast<uint32_t*>(to + i) = b[0];
     }
     if constexpr (!VEC) {
       __syncthreads();
@@ -383,15 +422,15 @@ __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// A CTA's walk over its rows with two operands a row (the second may be
-// missing): the next row is under way while f works on this one.
+// A CTA's row with two operands (the second may be missing).  kWalk: its walk over
+// rows, the next one under way while f works on this one.
 //   VEC: one buffer an operand.  A thread's pieces are its own, so it starts
 //     the next row's as soon as f has taken this row's into registers.
 //   else: two buffers (or one, filled again after f's barriers, where two do not
 //     fit), and a barrier before a row is read: all threads' copies of it have
 //     landed, and all have read the buffer that is filled next.
 // f(row, a, b, next): a, b the staged row; calls next() once they are read.
-template <typename T, int F, Lie L, typename Body>
+template <typename T, int F, Lie L, bool kWalk, typename Body>
 __device__ __forceinline__ void walk_rows(uint8_t* smem, const T* a, long lda, const T* b, long ldb,
                                           int n, int rows, int buffers, Body f) {
   using P = Part<T, F, L>;
@@ -408,28 +447,36 @@ __device__ __forceinline__ void walk_rows(uint8_t* smem, const T* a, long lda, c
     copies_commit();
   };
   stage(row, 0);
-  for (; row < rows; row += step) {
-    uint8_t* from = smem + at * 2 * room;
-    const T* pa = P::place(from, a + row * lda);
-    const T* pb = b ? P::place(from + room, b + row * ldb) : nullptr;
+  if constexpr (!kWalk) {
+    const T* pa = P::place(smem, a + row * lda);
+    const T* pb = b ? P::place(smem + room, b + row * ldb) : nullptr;
     copies_wait<0>();
-    if constexpr (P::VEC) {
-      f(row, pa, pb, [&] { stage(row + step, 0); });
-    } else {
-      __syncthreads();
-      if (buffers == 2) {
-        at ^= 1;
-        stage(row + step, at);
+    if constexpr (!P::VEC) __syncthreads();
+    f(row, pa, pb, [] {});
+  } else {
+    for (; row < rows; row += step) {
+      uint8_t* from = smem + at * 2 * room;
+      const T* pa = P::place(from, a + row * lda);
+      const T* pb = b ? P::place(from + room, b + row * ldb) : nullptr;
+      copies_wait<0>();
+      if constexpr (P::VEC) {
+        f(row, pa, pb, [&] { stage(row + step, 0); });
+      } else {
+        __syncthreads();
+        if (buffers == 2) {
+          at ^= 1;
+          stage(row + step, at);
+        }
+        f(row, pa, pb, [] {});
+        if (buffers == 1) stage(row + step, 0);
       }
-      f(row, pa, pb, [] {});
-      if (buffers == 1) stage(row + step, 0);
     }
   }
 }
 
 // --------------------------------------------------------------- the kernels --
 
-template <typename T, int F, Lie L>
+template <typename T, int F, Lie L, bool kWalk>
 __global__ void __launch_bounds__(kMaxThr) norm_rows_kernel(NormArgs a) {
   using P = Part<T, F, L>;
   extern __shared__ __align__(16) uint8_t stage_mem[];
@@ -450,7 +497,7 @@ __global__ void __launch_bounds__(kMaxThr) norm_rows_kernel(NormArgs a) {
       rows_mem += W::room(a.n);
     }
   }
-  walk_rows<T, F, L>(
+  walk_rows<T, F, L, kWalk>(
       rows_mem, static_cast<const T*>(a.x), a.ldx, static_cast<const T*>(a.r), a.ldr, a.n, a.rows,
       a.buffers, [&](long row, const T* x, const T* r, auto next) {
         T* h = a.h ? static_cast<T*>(a.h) + row * a.ldh : nullptr;
@@ -459,17 +506,10 @@ __global__ void __launch_bounds__(kMaxThr) norm_rows_kernel(NormArgs a) {
 #pragma unroll
         for (int run = 0; run < P::kRuns; run++) {
           uint64_t* vr = v + run * P::kPairs;
-          part.load(x, run, vr);
-          if (r) {
-            uint64_t b[P::kPairs];
-            part.load(r, run, b);
-#pragma unroll
-            for (int k = 0; k < P::kPairs; k++) vr[k] = add2(vr[k], b[k]);
-          }
-          if (r || h) {
-            const uint4 raw = P::round_run(vr);
-            if (h) part.store(h, run, raw);
-          }
+          uint4 raw = part.load(x, run);
+          if (r) raw = sum_piece<T>(raw, part.load(r, run));
+          if (h) part.store(h, run, raw);
+          P::spread(raw, vr);
         }
         next();
         double ss = 0.0;
@@ -505,7 +545,7 @@ __global__ void __launch_bounds__(kMaxThr) norm_rows_kernel(NormArgs a) {
       });
 }
 
-template <typename T, int F, Lie L>
+template <typename T, int F, Lie L, bool kWalk>
 __global__ void __launch_bounds__(kMaxThr) silu_rows_kernel(SiluArgs a) {
   using P = Part<T, F, L>;
   extern __shared__ __align__(16) uint8_t stage_mem[];
@@ -513,7 +553,7 @@ __global__ void __launch_bounds__(kMaxThr) silu_rows_kernel(SiluArgs a) {
   int parity = 0;
   pdl_wait();
   pdl_launch_dependents();
-  walk_rows<T, F, L>(
+  walk_rows<T, F, L, kWalk>(
       stage_mem + P::bytes(a.n), static_cast<const T*>(a.g), a.ld, static_cast<const T*>(a.u), a.ld, a.n, a.rows,
       a.buffers, [&](long row, const T* g, const T* u, auto next) {
         const P part{a.n, P::misplaced(static_cast<const T*>(a.g) + row * a.ld)};
@@ -523,8 +563,8 @@ __global__ void __launch_bounds__(kMaxThr) silu_rows_kernel(SiluArgs a) {
         for (int run = 0; run < P::kRuns; run++) {
           uint64_t* vr = v + run * P::kPairs;
           uint64_t gv[P::kPairs], uv[P::kPairs];
-          part.load(g, run, gv);
-          part.load(u, run, uv);
+          P::spread(part.load(g, run), gv);
+          P::spread(part.load(u, run), uv);
 #pragma unroll
           for (int k = 0; k < P::kPairs; k++) {
             vr[k] = silu_mul(gv[k], uv[k]);
@@ -662,25 +702,25 @@ int rows_launch(Args a, bool vec, int f, size_t extra, void (*wide)(Args), Pick 
   // Several on an SM cover one another, and rows handed out as CTAs end even
   // out the SMs' different speeds (8192x8192 f32 norm: 132; 163 walking); two
   // rows a CTA were slower too (333x5003 bf16: 10.2; 8.1 with one).
-  const bool alone = kMaxThr / threads < 2 || kStageMax / (smem + 1024) < 2;
-  a.buffers = alone && !vec && smem + pair <= kStageMax ? 2 : 1;
+  // (8 values a thread: few rows, of which no CTA has several worth a walk.)
+  const bool walk = f > 8 && a.rows > 148 && (kMaxThr / threads < 2 || kStageMax / (smem + 1024) < 2);
+  a.buffers = walk && !vec && smem + pair <= kStageMax ? 2 : 1;
   if (a.buffers == 2) smem += pair;
-  const int grid = alone && a.rows > 148 ? 148 : a.rows;
-  return launch(pick(f, !vec ? kAnyhow : f * threads == a.n ? kFull : kPieces), a, grid, threads,
-                smem, st);
+  return launch(pick(f, !vec ? kAnyhow : f * threads == a.n ? kFull : kPieces, walk), a,
+                walk ? 148 : a.rows, threads, smem, st);
 }
 
-template <typename T, int F>
+template <typename T, int F, bool kWalk>
 auto norm_kernel_of(Lie l) {
-  return l == kFull     ? norm_rows_kernel<T, F, kFull>
-         : l == kPieces ? norm_rows_kernel<T, F, kPieces>
-                        : norm_rows_kernel<T, F, kAnyhow>;
+  return l == kFull     ? norm_rows_kernel<T, F, kFull, kWalk>
+         : l == kPieces ? norm_rows_kernel<T, F, kPieces, kWalk>
+                        : norm_rows_kernel<T, F, kAnyhow, kWalk>;
 }
-template <typename T, int F>
+template <typename T, int F, bool kWalk>
 auto silu_kernel_of(Lie l) {
-  return l == kFull     ? silu_rows_kernel<T, F, kFull>
-         : l == kPieces ? silu_rows_kernel<T, F, kPieces>
-                        : silu_rows_kernel<T, F, kAnyhow>;
+  return l == kFull     ? silu_rows_kernel<T, F, kFull, kWalk>
+         : l == kPieces ? silu_rows_kernel<T, F, kPieces, kWalk>
+                        : silu_rows_kernel<T, F, kAnyhow, kWalk>;
 }
 
 template <typename T>
@@ -692,8 +732,11 @@ int norm_rows(const NormArgs& a, cudaStream_t st) {
                    (!a.w || aligned(a.w, 0, 2, 2 * per)) && aligned(a.q, a.ldq, 1, per);
   const int f = values_a_thread<T>(a.rows, a.n, vec);
   const size_t extra = !vec && a.w ? Part<__nv_bfloat16, 8, kAnyhow>::room(a.n) : 0;
-  return rows_launch<T>(a, vec, f, extra, norm_wide_kernel<T>, [](int f, Lie l) {
-    return f == 8 ? norm_kernel_of<T, 8>(l) : f == 16 ? norm_kernel_of<T, 16>(l) : norm_kernel_of<T, 32>(l);
+  return rows_launch<T>(a, vec, f, extra, norm_wide_kernel<T>, [](int f, Lie l, bool walk) {
+    if (walk) return f == 16 ? norm_kernel_of<T, 16, true>(l) : norm_kernel_of<T, 32, true>(l);
+    return f == 8    ? norm_kernel_of<T, 8, false>(l)
+           : f == 16 ? norm_kernel_of<T, 16, false>(l)
+                     : norm_kernel_of<T, 32, false>(l);
   }, st);
 }
 
@@ -703,8 +746,11 @@ int silu_rows(const SiluArgs& a, cudaStream_t st) {
   const bool vec = a.n % per == 0 && aligned(a.g, a.ld, sizeof(T), 16) &&
                    aligned(a.u, a.ld, sizeof(T), 16) && aligned(a.q, a.ldq, 1, per);
   const int f = values_a_thread<T>(a.rows, a.n, vec);
-  return rows_launch<T>(a, vec, f, 0, silu_wide_kernel<T>, [](int f, Lie l) {
-    return f == 8 ? silu_kernel_of<T, 8>(l) : f == 16 ? silu_kernel_of<T, 16>(l) : silu_kernel_of<T, 32>(l);
+  return rows_launch<T>(a, vec, f, 0, silu_wide_kernel<T>, [](int f, Lie l, bool walk) {
+    if (walk) return f == 16 ? silu_kernel_of<T, 16, true>(l) : silu_kernel_of<T, 32, true>(l);
+    return f == 8    ? silu_kernel_of<T, 8, false>(l)
+           : f == 16 ? silu_kernel_of<T, 16, false>(l)
+                     : silu_kernel_of<T, 32, false>(l);
   }, st);
 }
 
