@@ -17,10 +17,10 @@
 // sum (or the first operand): two aligned reads and a shift.
 // Rows past 1024 threads' registers stay in shared memory as f32 (wide_kernel).
 //
-// One B200, inputs from HBM: residual + norm of 8192x8192 f32 132 us (6.6 TB/s,
-// the copy peak), bf16 80 us (5.9 TB/s, 72% of the issue slots); SwiGLU of
-// 4096x28672 bf16 97 us (6.0 TB/s); one row of 4096 2.3 us, two barriers and a
-// memory round trip over an empty launch; 333x5003 f16 norm, unaligned, 6.3 us.
+// One B200, inputs from HBM: residual + norm of 8192x8192 f32 128 us (6.8 TB/s, the
+// copy peak), bf16 74 us (6.3 TB/s); SwiGLU of 4096x28672 bf16 90-94 us (6.3-6.5
+// TB/s); one row of 4096 2.0 us, two barriers and a memory round trip over an
+// empty launch; 333x5003 f16 norm, unaligned, 6.4 us.
 #include <type_traits>
 
 #include "typed.cuh"
@@ -663,22 +663,21 @@ inline bool aligned(const void* p, long ld, size_t esize, size_t to) {
 
 constexpr size_t kStageMax = 224 * 1024;  // an SM's shared memory, less the reductions'
 
-// Values a thread.  Few rows: 8, more threads hide a row's latency (us, norm,
-// 64x8192 bf16: 3.3 with 8, 3.6 with 16, 4.9 with 32).  Many: 16 of f32 (8192x8192:
-// 132; 142 with 8, 145 with 32) and 32 of 16-bit rows (8192x4096: 43; 71 with 8, 49
-// with 16), fewer reductions a value; 16 of some rows an SM (333x4096: 4.5; 5.6 with
-// 8, 5.5 with 32) and of short ones.  Unaligned rows carry more a thread besides: 16
-// (200x5003 bf16: 6.5; 9.4 with 8, 7.7 with 32), 32 of many or long 16-bit ones
-// (4000x5003: 50; 59 with 16), 8 of short ones (300x1003: 4.4; 4.9 with 16).
+// Values a thread: some 256 threads a row, so that an SM holds several rows and a
+// thread's part of the reductions is small beside its values; few rows 8 (more
+// threads hide a row's latency).  us with 8 / 16 / 32, norm:
+//   whole pieces, bf16: 148x4096 2.7 / 3.0 / 3.7; 600x4096 6.1 / 5.1 / 5.9; 8192x8192
+//   96 / 87 / 74; 600x1024 2.6 / 2.8 / 3.6.  f32: 8192x8192 128 / 128 / 134;
+//   1000x8192 21 / 20 / 23; 300x1024 2.5 / 2.5 / 3.9.
+//   anyhow, bf16: 1000x1003 7.6 / 8.2 / 9.8; 8000x1003 31.6 / 29.9 / 39.7; 200x5003
+//   6.7 / 6.1 / 6.9; 4000x5003 67 / 57 / 44.  f32: 600x5003 15.2 / 16.2 / 16.8;
+//   4000x5003 78 / 73 / 68; 2000x14331 - / 106 / 124.
 template <typename T>
 int values_a_thread(int rows, int n, bool vec) {
-  const bool half = sizeof(T) == 2;
-  if (!vec) {
-    if (n < 2048 && rows < 148 * 8) return 8;
-    return half && (n >= 8192 || (n >= 4096 && rows >= 148 * 4)) ? 32 : 16;
-  }
-  if (rows < 148 * 2 || (n < 4096 && rows < 148 * 4)) return 8;
-  return half && n >= 4096 && rows >= 148 * 4 ? 32 : 16;
+  const bool few = rows < 148 * 2, many = rows >= 148 * 8;
+  if (vec) return few || n <= 2048 ? 8 : sizeof(T) == 2 && n > 6144 ? 32 : 16;
+  if (sizeof(T) == 2) return n >= 8192 || (n >= 4096 && !few) ? 32 : n < 2048 && !many ? 8 : 16;
+  return !many ? 8 : n >= 4096 && n < 8192 ? 32 : 16;
 }
 
 // Launches the kernel of the row's alignment and size; `wide` where a row fits
@@ -698,12 +697,13 @@ int rows_launch(Args a, bool vec, int f, size_t extra, void (*wide)(Args), Pick 
   const int threads = ((span + f - 1) / f + 31) / 32 * 32;
   // CTAs that an SM holds: by threads (64 registers each) and shared memory.
   // Alone on its SM a CTA walks all its rows, the next one's copies under this
-  // one's reductions (4096x28672 bf16 SwiGLU: 95 us; 125 with one row a CTA).
-  // Several on an SM cover one another, and rows handed out as CTAs end even
-  // out the SMs' different speeds (8192x8192 f32 norm: 132; 163 walking); two
-  // rows a CTA were slower too (333x5003 bf16: 10.2; 8.1 with one).
-  // (8 values a thread: few rows, of which no CTA has several worth a walk.)
-  const bool walk = f > 8 && a.rows > 148 && (kMaxThr / threads < 2 || kStageMax / (smem + 1024) < 2);
+  // one's reductions (4096x28672 bf16 SwiGLU: 90 us; 120 with one row a CTA); rows
+  // of f32 that fill the shared memory gain nothing by it (267 and 243 for the
+  // norm), nor few rows.  Several on an SM cover one another, and rows handed out
+  // as CTAs end even out the SMs' different speeds (8192x8192 f32 norm: 132; 163
+  // walking); two rows a CTA were slower too (333x5003 bf16: 10.2; 8.1 with one).
+  const bool alone = kMaxThr / threads < 2 || kStageMax / (smem + 1024) < 2;
+  const bool walk = alone && f > 8 && a.rows > 148 && !(sizeof(T) == 4 && a.n > 16384);
   a.buffers = walk && !vec && smem + pair <= kStageMax ? 2 : 1;
   if (a.buffers == 2) smem += pair;
   return launch(pick(f, !vec ? kAnyhow : f * threads == a.n ? kFull : kPieces, walk), a,
