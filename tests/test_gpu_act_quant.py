@@ -302,3 +302,50 @@ def test_equal_calls_give_equal_bits(eng, torch):
     assert all(torch.equal(a, b) for a, b in zip(one, two))
     alone = run_norm(eng, torch, "bf16", x[77:78].contiguous(), r[77:78].contiguous(), w, 1e-5)
     assert torch.equal(alone[1][0], one[1][77]) and alone[2][0] == one[2][77]  # whatever the batch
+
+
+MANY = [(300, 28672), (300, 24008), (300, 27999), (300, 14336), (300, 12008), (300, 14331),
+        (700, 4096), (600, 8192), (1300, 1024), (1300, 1003), (600, 5000), (600, 5003)]
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows,n", MANY)
+def test_many_rows(eng, torch, kind, rows, n):
+    """More rows than the SMs take at once, in every layout; each row's result is
+    what it gives alone."""
+    x, r, w = inputs(torch, kind, rows, n, n + 1)
+    h, q, sc = run_norm(eng, torch, kind, x, r, w, 1e-5)
+    want = (x.float() + r.float()).to(x.dtype)
+    assert torch.equal(h, want)
+    check_rows(norm64(want, w, 1e-5), norm_rel(n), q.cpu().numpy().astype(np.float64),
+               sc.double().cpu().numpy())
+    qs, ss = run_silu(eng, torch, kind, x, r)
+    check_rows(silu64(x, r), silu_rel(x), qs.cpu().numpy().astype(np.float64),
+               ss.double().cpu().numpy())
+    for t in (0, 147, 148, rows - 1):
+        alone = run_silu(eng, torch, kind, x[t:t + 1].contiguous(), r[t:t + 1].contiguous())
+        assert torch.equal(alone[0][0], qs[t]) and alone[1][0] == ss[t]
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n", [4096, 4099])
+def test_sums_of_any_values(eng, torch, kind, n):
+    """Random bit patterns, subnormals, infinities and NaN among them: the sum is
+    the f32 sum rounded to the type."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    bits = torch.int32 if kind == "f32" else torch.int16
+    lo, hi = (-2 ** 31, 2 ** 31) if kind == "f32" else (-2 ** 15, 2 ** 15)
+
+    def rand():
+        v = torch.randint(lo, hi, (512, n), generator=g, device="cuda", dtype=torch.int64)
+        return v.to(bits).view(dtype(torch, kind))
+
+    x, r = rand(), rand()
+    near = torch.rand(512, n, generator=g, device="cuda") < 0.5  # of like size, where sums round
+    r = torch.where(near, (x.float() * (torch.rand(512, n, generator=g, device="cuda") * 4 - 2))
+                    .to(r.dtype), r)
+    h, _, _ = run_norm(eng, torch, kind, x, r, None, 1e-5)
+    want = (x.float() + r.float()).to(x.dtype)
+    nan = want.isnan()
+    assert torch.equal(h.isnan(), nan)
+    assert torch.equal(h.view(bits)[~nan], want.view(bits)[~nan])
