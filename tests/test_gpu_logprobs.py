@@ -208,6 +208,26 @@ def test_peaked_and_far_logits(eng, torch):
     assert np.all(np.abs(got[1] - en) < 8 * U)
 
 
+MANY = [(30, 70001), (200, 33003), (200, 70001), (300, 33003), (460, 66003), (700, 20001),
+        (1200, 9000), (1200, 66000)]
+
+
+@pytest.mark.parametrize("kind,top", [("f32", 5), ("f32", 20), ("bf16", 8), ("bf16", 32),
+                                      ("f16", 13)])
+@pytest.mark.parametrize("rows,n", MANY)
+def test_many_rows(eng, torch, kind, top, rows, n):
+    """More rows than the SMs take at once, of several lengths."""
+    g = torch.Generator(device="cuda").manual_seed(rows + n)
+    l = (torch.randn(rows, n, generator=g, device="cuda") * 3).to(dtype(torch, kind))
+    l[rows // 2:, ::3] = -INF
+    tokens = torch.randint(0, n, (rows,), generator=g, device="cuda").tolist()
+    got = run(eng, torch, kind, l, tokens, 0.8, top)
+    some = np.unique(np.linspace(0, rows - 1, 40).astype(int))  # 64 bits take time
+    check(l[torch.as_tensor(some, device="cuda")], [tokens[t] for t in some], 0.8, top,
+          tuple(v[some] for v in got), n)
+    assert all(np.isfinite(v).all() for v in got[1:2]) and (got[2] >= 0).all() and (got[2] < n).all()
+
+
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("n", [3, 1000, 70001])
 def test_ends_of_the_temperature(eng, torch, kind, n):
