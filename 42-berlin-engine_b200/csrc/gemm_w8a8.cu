@@ -24,12 +24,15 @@
 // The tensor cores bound it: 3.2-3.4 POP/s, and 2.75 where the power limit
 // holds the clock at 1.2 GHz.
 //
-// gemm_w8a8_kernel (few tokens): a tile is R <= 128 channels x up to 256 tokens.
-// The weights' bytes are the bound (1x128256x4096: 5.8-6.2 TB/s), and R is
+// gemm_few_kernel (one to eight tokens): byte dot products on the integer pipes as
+// the weights stream through registers.
+//
+// gemm_w8a8_kernel (fewer tokens): a tile is R <= 128 channels x up to 256 tokens.
+// The weights' bytes are the bound (8x128256x4096: 5.8-6.2 TB/s), and R is
 // chosen so that the tiles fill whole rounds of the SMs (every SM streams the
 // same share of the weights).  The MMA computes its 128 rows whatever R is, in
 // 66 cycles with few tokens; below 50 rows a tile that would bound it, and K is
-// split instead (1x4096x14336: 14 us with 125 rows over 4 CTAs, 24 with 28 rows
+// split instead (4x4096x14336: 14 us with 125 rows over 4 CTAs, 24 with 28 rows
 // alone).
 //
 // Both can split K over a cluster (256x4096x14336: 23 us over 2 pairs, 31
@@ -725,6 +728,145 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// ------------------------------------------------------- a few tokens --
+
+constexpr int kFewWarps = 16;
+constexpr int kFewStep = 512;  // bytes of K that a warp takes at once
+constexpr int kFewAhead = 4;   // steps of two channels that a warp has under way
+
+struct FewArgs {
+  const int8_t* x;
+  const int8_t* w;
+  long ldx, ldw;
+  const float* sx;
+  const float* sw;
+  void* y;
+  long ldy;
+  int m, k, nb;
+};
+
+__device__ __forceinline__ uint4 load_weights(const int8_t* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+// the 16 bytes of a row of k from `at` on, zero behind its end
+template <typename Load>
+__device__ __forceinline__ uint4 piece_of(const int8_t* row, int at, int k, Load load) {
+  if (at + 16 <= k) return load(row + at);
+  uint32_t word[4] = {0, 0, 0, 0};
+  for (int i = 0; at + i < k; i++)
+    word[i / 4] |= (uint32_t)(uint8_t)row[at + i] << (8 * (i & 3));
+  return make_uint4(word[0], word[1], word[2], word[3]);
+}
+
+// One to NB tokens: a byte of weights makes NB multiply-adds, which the integer
+// pipes do while it streams in; the tensor cores' way (copies into shared memory,
+// 128 rows a step, accumulators out of TMEM, a cluster's join) would add to it.
+// A CTA takes an equal range of the channels, two at a time; its warps share the
+// steps of 512 bytes of K of all of them equally, whatever channel they belong to,
+// and load kFewAhead of them ahead into registers.  A warp's part of a channel's
+// sum is added to the others' in shared memory: integers, so their order does not
+// matter.  Bound by HBM: 1x128256x4096 bf16 81 us (6.5 TB/s), 1x28672x4096 19.5
+// (18 at the copy peak), 1x6144x4096 5.7, 1x1024x1024 1.9.
+template <typename T, int NB>
+__global__ void __launch_bounds__(kFewWarps * 32, NB <= 2 ? 2 : 1) gemm_few_kernel(FewArgs a) {
+  extern __shared__ __align__(1024) uint8_t smem[];  // [NB][kpad] tokens, [channels][NB] sums
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const int steps = (a.k + kFewStep - 1) / kFewStep, kpad = steps * kFewStep;
+  const int c0 = (int)((long)a.m * blockIdx.x / gridDim.x);
+  const int channels = (int)((long)a.m * (blockIdx.x + 1) / gridDim.x) - c0;
+  int* sums = reinterpret_cast<int*>(smem + (size_t)NB * kpad);
+  const int units = (channels + 1) / 2 * steps;
+  const int u0 = (int)((long)units * warp / kFewWarps), u1 = (int)((long)units * (warp + 1) / kFewWarps);
+  for (int i = tid; i < channels * NB; i += kFewWarps * 32) sums[i] = 0;
+
+  // the unit to load next, and the one to work at: pair of channels, step of K
+  int lp = u0 / steps, ls = u0 - lp * steps, p = lp, s = ls;
+  auto rows_of = [&](int pair, int i) {
+    return a.w + (long)(c0 + min(2 * pair + i, channels - 1)) * a.ldw;
+  };
+  uint4 w[kFewAhead][2];
+  auto load = [&](int slot) {
+    const int at = ls * kFewStep + lane * 16;
+#pragma unroll
+    for (int i = 0; i < 2; i++) w[slot][i] = piece_of(rows_of(lp, i), at, a.k, load_weights);
+    if (++ls == steps) {
+      ls = 0;
+      lp++;
+    }
+  };
+  // the first steps into L2 (the copies themselves have to wait)
+  for (int u = u0; u < min(u1, u0 + kFewAhead); u++) {
+    const int q = u / steps, at = (u - q * steps) * kFewStep + lane * 16;
+    if (at < a.k && (lane & 7) == 0)
+      for (int i = 0; i < 2; i++)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(rows_of(q, i) + at));
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+#pragma unroll
+  for (int d = 0; d < kFewAhead; d++)
+    if (u0 + d < u1) load(d);
+  for (int i = tid; i < NB * (kpad / 16); i += kFewWarps * 32) {
+    const int t = i / (kpad / 16), at = (i - t * (kpad / 16)) * 16;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (t < a.nb && at < a.k)
+      v = piece_of(a.x + (long)t * a.ldx, at, a.k,
+                   [](const int8_t* q) { return *reinterpret_cast<const uint4*>(q); });
+    *reinterpret_cast<uint4*>(smem + (size_t)t * kpad + at) = v;
+  }
+  __syncthreads();
+
+  int acc[2][NB] = {};
+  auto flush = [&]() {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+#pragma unroll
+      for (int t = 0; t < NB; t++) {
+        const int sum = __reduce_add_sync(0xffffffffu, acc[i][t]);
+        if (lane == 0 && 2 * p + i < channels) atomicAdd(&sums[(2 * p + i) * NB + t], sum);
+        acc[i][t] = 0;
+      }
+    }
+  };
+#pragma unroll 1
+  for (int u = u0; u < u1; u += kFewAhead) {
+#pragma unroll
+    for (int d = 0; d < kFewAhead; d++) {
+      if (u + d >= u1) break;
+      const uint8_t* xs = smem + s * kFewStep + lane * 16;
+#pragma unroll
+      for (int t = 0; t < NB; t++) {
+        const uint4 v = *reinterpret_cast<const uint4*>(xs + (size_t)t * kpad);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          int sum = acc[i][t];
+          sum = __dp4a((int)v.x, (int)w[d][i].x, sum);
+          sum = __dp4a((int)v.y, (int)w[d][i].y, sum);
+          sum = __dp4a((int)v.z, (int)w[d][i].z, sum);
+          acc[i][t] = __dp4a((int)v.w, (int)w[d][i].w, sum);
+        }
+      }
+      if (u + d + kFewAhead < u1) load(d);
+      if (++s == steps) {
+        flush();
+        s = 0;
+        p++;
+      }
+    }
+  }
+  if (s > 0 && u0 < u1) flush();
+  __syncthreads();
+  for (int i = tid; i < channels * a.nb; i += kFewWarps * 32) {
+    const int t = i / channels, c = i - t * channels;
+    static_cast<T*>(a.y)[(long)t * a.ldy + c0 + c] =
+        from_f32<T>(scaled(sums[c * NB + t], a.sx[t], a.sw[c0 + c]));
+  }
+}
+
 // ------------------------------------------------------------------ host --
 
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
@@ -925,6 +1067,34 @@ int launch_pair(const int8_t* x, long ldx, const int8_t* w, long ldw, int k, W8A
   return EC_OK;
 }
 
+// Whether the tokens are few enough for gemm_few_kernel.  us, with it and with the
+// tensor cores: 1x6144x4096 5.7 / 8.5; 2x128256x4096 82 / 88; 2x4096x14336 12.1 /
+// 14.3; 4x4096x4096 6.4 / 7.0, 4x28672x4096 28 / 23; 8x2048x2048 4.8 / 5.7,
+// 8x4096x4096 8.8 / 7.0 (its multiply-adds grow with the tokens).
+inline bool few_tokens(int m, int k, int nb) {
+  const long weights = (long)m * k;
+  return nb <= 2 || (nb <= 4 && weights <= 1 << 25) || (nb <= 8 && weights <= 1 << 22);
+}
+
+template <typename T, int NB>
+int launch_few(const FewArgs& a, int grid, size_t smem, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kFewWarps * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (smem > 48 * 1024)
+    EC_CUDA_TRY(cudaFuncSetAttribute(gemm_few_kernel<T, NB>,
+                                     cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  EC_CUDA_TRY(cudaLaunchKernelEx(&cfg, gemm_few_kernel<T, NB>, a));
+  return EC_OK;
+}
+
 template <typename T>
 int launch(const int8_t* x, long ldx, const int8_t* w, long ldw, int k, W8A8Args a,
            cudaStream_t st) {
@@ -935,6 +1105,25 @@ int launch(const int8_t* x, long ldx, const int8_t* w, long ldw, int k, W8A8Args
   const Slots* slots = nullptr;
   EC_CUDA_TRY(device_slots(&slots));
   const int n_sm = slots->clusters[1];
+  if (few_tokens(a.m, k, a.nb)) {
+    const int NB = a.nb <= 2 ? a.nb : a.nb <= 4 ? 4 : 8;
+    const size_t x_bytes = (size_t)NB * ceil_div(k, kFewStep) * kFewStep;
+    // two CTAs an SM (NB <= 2: 64 registers) keep more of a long stream under way
+    // (1x28672x4096: 19.5 us; 23.3 with one), one starts a short one sooner
+    // (1x2048x2048: 2.4 and 2.7)
+    int grid = NB <= 2 && (long)a.m * k > (1 << 23) && x_bytes < 64 * 1024 ? 2 * n_sm : n_sm;
+    if ((a.m + 1) / 2 < grid) grid = (a.m + 1) / 2;
+    const size_t smem = x_bytes + (size_t)ceil_div(a.m, grid) * NB * 4;
+    if (smem <= 200 * 1024) {
+      const FewArgs f{x, w, ldx, ldw, a.sx, a.sw, a.y, a.ldy, a.m, k, a.nb};
+      switch (NB) {
+        case 1: return launch_few<T, 1>(f, grid, smem, st);
+        case 2: return launch_few<T, 2>(f, grid, smem, st);
+        case 4: return launch_few<T, 4>(f, grid, smem, st);
+        default: return launch_few<T, 8>(f, grid, smem, st);
+      }
+    }
+  }
   a.chunks = ceil_div(k, kKb);
   const Plan p = plan_of(a.m, a.chunks, a.nb, *slots);
   a.R = p.R;

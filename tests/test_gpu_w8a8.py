@@ -100,6 +100,22 @@ def test_product(eng, torch, kind, nb, m, k):
     check(torch, kind, y, exact(torch, x, w, sx, sw, k))
 
 
+FEW = [(1, 1), (2, 15), (3, 16), (5, 17), (64, 512), (77, 511), (129, 513), (297, 1025),
+       (600, 100), (1000, 4099), (64, 28672), (2048, 2048), (4097, 4096), (14336, 512),
+       (128256, 128), (33, 131071), (200001, 40)]
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("nb", [1, 2, 3, 4, 5, 8])
+@pytest.mark.parametrize("m,k", FEW)
+def test_few_tokens(eng, torch, kind, nb, m, k):
+    ld = (k + 15) // 16 * 16
+    x, w = int8_rows(torch, nb, k, ld + 32, k), int8_rows(torch, m, k, ld + 16 * (m % 2), m)
+    sx, sw = scales(torch, nb, m, 9)
+    y = run(eng, torch, kind, x, w, sx, sw, k, ldy=m + 3, offset=1)
+    check(torch, kind, y, exact(torch, x, w, sx, sw, k))
+
+
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("nb", [1, 20, 100, 300, 600])
 def test_strides(eng, torch, kind, nb):
