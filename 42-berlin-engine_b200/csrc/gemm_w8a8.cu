@@ -27,18 +27,19 @@
 // gemm_few_kernel (one to eight tokens): byte dot products on the integer pipes as
 // the weights stream through registers.
 //
-// gemm_w8a8_kernel (fewer tokens): a tile is R <= 128 channels x up to 256 tokens.
-// The weights' bytes are the bound (8x128256x4096: 5.8-6.2 TB/s), and R is
+// gemm_w8a8_kernel (up to some tens of tokens): a tile is R <= 128 channels x up to 256 tokens.
+// The weights' bytes are the bound (8x128256x4096: 5.4-5.8 TB/s), and R is
 // chosen so that the tiles fill whole rounds of the SMs (every SM streams the
 // same share of the weights).  The MMA computes its 128 rows whatever R is, in
 // 66 cycles with few tokens; below 50 rows a tile that would bound it, and K is
 // split instead (4x4096x14336: 14 us with 125 rows over 4 CTAs, 24 with 28 rows
 // alone).
 //
-// Both can split K over a cluster (256x4096x14336: 23 us over 2 pairs, 31
+// These two can split K over a cluster (256x4096x14336: 23 us over 2 pairs, 31
 // without): the partial accumulators meet in distributed shared memory, each
-// CTA finishing a part of the token columns.  Warp 0 streams, warp 1 issues the MMAs, the others drain
-// TMEM; two TMEM buffers let a tile's epilogue run under the next one's MMAs.
+// CTA finishing a part of the token columns.  Warp 0 streams, warp 1 issues the
+// MMAs, the others drain TMEM; two TMEM buffers let a tile's epilogue run under the
+// next one's MMAs.
 #include <atomic>
 #include <mutex>
 
